@@ -216,6 +216,46 @@ void iris_dev_linear_bf16_qknorm(uint16_t *y, const uint16_t *x, const uint16_t 
                                  int q_heads, int k_heads, int head_dim, const float *wq, const float *wk,
                                  const float *rope_cos, const float *rope_sin, float eps, int split_half);
 
+/* ---- linear layers over groups of rows ----
+ * y[m, :] = x[m, :] @ W[g]^T for the rows first_row[g] <= m < first_row[g + 1] of group g: iris_dev_linear_f32 / _bf16 once per
+ * group, as one launch. The text rows and the image rows of a double-stream block (two groups), rows sorted by the expert or the adapter
+ * that they go to. x [rows, in], y [rows, out], W [groups, out, in], all contiguous; first_row: device int [groups + 1], not
+ * decreasing, read when the layer runs. Groups may be empty. Rows of y in front of first_row[0] and from first_row[groups] on stay as
+ * they were. A value of first_row below one before it counts as that one, values are limited to 0 .. rows: no call reads or writes
+ * outside its matrices. Any sizes and alignment. groups 0 does nothing.
+ * The f32 sums of a row are taken in an order that may differ from the plain layer's; a call gives the same bits every time. */
+void iris_dev_linear_f32_grouped(float *y, const uint16_t *x, const uint16_t *W, const int *first_row,
+                                 int groups, int rows, int in, int out);
+void iris_dev_linear_bf16_grouped(uint16_t *y, const uint16_t *x, const uint16_t *W, const int *first_row,
+                                  int groups, int rows, int in, int out);
+
+/* ---- microscaled 4-bit floating point (MXFP4 of the OCP Microscaling formats 1.0) ----
+ * A row of `cols` values is held in blocks of 32 columns, nb = (cols + 31) / 32 of them, the last one filled up with zeros:
+ *   scales [rows, nb]       a byte s a block: 2^(s - 127), 255 stands for NaN
+ *   codes  [rows, 16 * nb]  four bits a value, sign then one of 0, 0.5, 1, 1.5, 2, 3, 4, 6; the even column in the low half of its byte
+ * and a value is its code times its block's scale. Both contiguous, codes 16-byte aligned. */
+
+/* Rows of stride lds to codes and scales. The scale of a block is 2^(floor(log2(largest magnitude)) - 2) (and at least 2^-127; 2^-127
+ * for a block of zeros), the code the nearest one to value / scale, ties to the even code, 6 for what is above it. A block with
+ * an infinity or a NaN in it becomes NaN as a whole (scale 255, codes 0). */
+void iris_dev_f32_to_mxfp4(uint8_t *codes, uint8_t *scales, const float *src, int lds, int rows, int cols);
+void iris_dev_bf16_to_mxfp4(uint8_t *codes, uint8_t *scales, const uint16_t *src, int lds, int rows, int cols);
+/* Back, into rows of stride ldd: exact where the value is one that f32 / bf16 has. Columns from cols on stay as they were. */
+void iris_dev_mxfp4_to_f32(float *dst, int ldd, const uint8_t *codes, const uint8_t *scales, int rows, int cols);
+void iris_dev_mxfp4_to_bf16(uint16_t *dst, int ldd, const uint8_t *codes, const uint8_t *scales, int rows, int cols);
+
+/* iris_dev_linear_f32 / _bf16 on rows and weights held in MXFP4: y[rows, out] = x[rows, in] @ W[out, in]^T, f32 accumulation. A last block
+ * that `in` ends inside is multiplied as a whole: its zeros are for the caller to keep, as the conversions above do. */
+void iris_dev_linear_mxfp4_f32(float *y, const uint8_t *x, const uint8_t *x_scales, const uint8_t *W, const uint8_t *W_scales,
+                               int rows, int in, int out);
+void iris_dev_linear_mxfp4_bf16(uint16_t *y, const uint8_t *x, const uint8_t *x_scales, const uint8_t *W, const uint8_t *W_scales,
+                                int rows, int in, int out);
+/* Both together: rows of group g take W[g] (codes [groups, out, 16 * nb], scales [groups, out, nb]). */
+void iris_dev_linear_mxfp4_f32_grouped(float *y, const uint8_t *x, const uint8_t *x_scales, const uint8_t *W, const uint8_t *W_scales,
+                                       const int *first_row, int groups, int rows, int in, int out);
+void iris_dev_linear_mxfp4_bf16_grouped(uint16_t *y, const uint8_t *x, const uint8_t *x_scales, const uint8_t *W, const uint8_t *W_scales,
+                                        const int *first_row, int groups, int rows, int in, int out);
+
 /* The library's stream as a hipStream_t, for callers that time kernels with
  * HIP events or order their own work after the library's. */
 void *iris_dev_stream(void);

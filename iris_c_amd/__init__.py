@@ -51,6 +51,16 @@ ABI = {
     "iris_dev_upsample2x": (None, [_vp, _vp, _i, _i, _i]),
     "iris_dev_head_norm_rope_qk": (None, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _i]),
     "iris_dev_head_norm_rope_qk_streams": (None, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _f, _i]),
+    "iris_dev_linear_f32_grouped": (None, [_vp, _vp, _vp, _vp, _i, _i, _i, _i]),
+    "iris_dev_linear_bf16_grouped": (None, [_vp, _vp, _vp, _vp, _i, _i, _i, _i]),
+    "iris_dev_f32_to_mxfp4": (None, [_vp, _vp, _vp, _i, _i, _i]),
+    "iris_dev_bf16_to_mxfp4": (None, [_vp, _vp, _vp, _i, _i, _i]),
+    "iris_dev_mxfp4_to_f32": (None, [_vp, _i, _vp, _vp, _i, _i]),
+    "iris_dev_mxfp4_to_bf16": (None, [_vp, _i, _vp, _vp, _i, _i]),
+    "iris_dev_linear_mxfp4_f32": (None, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i]),
+    "iris_dev_linear_mxfp4_bf16": (None, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i]),
+    "iris_dev_linear_mxfp4_f32_grouped": (None, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i]),
+    "iris_dev_linear_mxfp4_bf16_grouped": (None, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i]),
     "iris_dev_stream": (_vp, []),
     "iris_dev_last_error": (_i, []),
     "iris_dev_last_kernel": (C.c_char_p, []),

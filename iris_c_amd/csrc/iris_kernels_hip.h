@@ -156,6 +156,23 @@ float iris_hip_gemm_tiles_plan(int M, int N, int K, int out_size, size_t part_by
 int iris_hip_gemm_tiles(void *stream, void *y, int out_size, const uint16_t *x, const uint16_t *W, int M, int N, int K,
                         const float *bias, int shape, int splits, float *part);
 
+/* The same for groups of rows with weights of their own, W [groups, out, in]: rows [first_row[g], first_row[g + 1]) take W[g], rows in no
+ * group are left alone; first_row: device int [groups + 1] (gemm_grouped_gfx950.hip). Any sizes and alignment. */
+int iris_hip_linear_f32_grouped(void *stream, float *y, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int rows, int in, int out);
+int iris_hip_linear_bf16_grouped(void *stream, uint16_t *y, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int rows, int in, int out);
+
+/* ---- microscaled 4-bit floating point (mxfp4_ops.hip, gemm_mxfp4_gfx950.hip) ---- */
+/* rows [rows, cols] of stride ld at any alignment <-> codes [rows, 16 * blocks] (4-byte aligned), scales [rows, blocks]; blocks = cols / 32, rounded up */
+int iris_hip_f32_to_mxfp4(void *stream, uint8_t *codes, uint8_t *scales, const float *src, int ld, int rows, int cols);
+int iris_hip_bf16_to_mxfp4(void *stream, uint8_t *codes, uint8_t *scales, const uint16_t *src, int ld, int rows, int cols);
+int iris_hip_mxfp4_to_f32(void *stream, float *dst, int ld, const uint8_t *codes, const uint8_t *scales, int rows, int cols);
+int iris_hip_mxfp4_to_bf16(void *stream, uint16_t *dst, int ld, const uint8_t *codes, const uint8_t *scales, int rows, int cols);
+/* y[rows, out] = x W^T, x and W as codes (16-byte aligned) and scales; first_row NULL: one W for all rows, otherwise as above */
+int iris_hip_linear_mxfp4_f32(void *stream, float *y, const uint8_t *x, const uint8_t *xs, const uint8_t *W, const uint8_t *Ws, const int *first_row, int groups,
+                              int rows, int in, int out);
+int iris_hip_linear_mxfp4_bf16(void *stream, uint16_t *y, const uint8_t *x, const uint8_t *xs, const uint8_t *W, const uint8_t *Ws, const int *first_row,
+                               int groups, int rows, int in, int out);
+
 /* 1: the tiles normalise themselves, 0: the norm kernel runs behind the layer, -1: not taken; host arithmetic only */
 int iris_hip_linear_qknorm_plan(int rows, int in, int out, int q_cols, int k_cols);
 /* -2 = shape not taken, nothing enqueued */

@@ -540,6 +540,99 @@ void iris_dev_linear_bf16_qknorm(uint16_t *y, const uint16_t *x, const uint16_t 
         norm_rope(y, NULL, out, wk, NULL, rope_cos, rope_sin, rows, k_heads, 0, head_dim, eps, split_half);
 }
 
+/* ---- linear layers over groups of rows, and in microscaled 4-bit floating point ---- */
+
+static int grouped_args(const char *what, const int *first_row, int groups, int in) {
+    if (in <= 0) { fail(-1, what, "in must be positive"); return 0; }
+    if (groups < 0 || (groups && !first_row)) { fail(-1, what, "need the first rows of groups >= 0 groups"); return 0; }
+    return 1;
+}
+
+/* rows <= 0 and the like: nothing to do, as for the plain layers; no groups: no row is in one */
+#define GROUPED(what, name, launcher)                                                                           \
+    do {                                                                                                        \
+        if (rows <= 0 || out <= 0 || !grouped_args(what, first_row, groups, in) || !groups) return;             \
+        if (!y || !x || !W) { fail(-1, what, "y, x or W is missing"); return; }                                 \
+        if (!need_ready(what)) return;                                                                          \
+        g_last_kernel = name;                                                                                   \
+        LAUNCH(what, launcher(g_stream, y, x, W, first_row, groups, rows, in, out));                            \
+    } while (0)
+
+void iris_dev_linear_f32_grouped(float *y, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int rows, int in, int out) {
+    GROUPED("linear_grouped", "linear_grouped", iris_hip_linear_f32_grouped);
+}
+
+void iris_dev_linear_bf16_grouped(uint16_t *y, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int rows, int in, int out) {
+    GROUPED("linear_grouped", "linear_grouped", iris_hip_linear_bf16_grouped);
+}
+
+/* 0 after reporting what is wrong; also where there is nothing to do */
+static int mxfp4_rows_args(const char *what, const void *values, const uint8_t *codes, const uint8_t *scales, int ld, int rows, int cols) {
+    if (rows <= 0 || cols <= 0) return 0;
+    if (!values || !codes || !scales) { fail(-1, what, "values, codes or scales are missing"); return 0; }
+    if (ld < cols) { fail(-1, what, "need ld >= cols"); return 0; }
+    if (!aligned(codes, 16)) { fail(-1, what, "codes must be 16-byte aligned"); return 0; }
+    return need_ready(what);
+}
+
+void iris_dev_f32_to_mxfp4(uint8_t *codes, uint8_t *scales, const float *src, int lds, int rows, int cols) {
+    if (!mxfp4_rows_args("f32_to_mxfp4", src, codes, scales, lds, rows, cols)) return;
+    LAUNCH("f32_to_mxfp4", iris_hip_f32_to_mxfp4(g_stream, codes, scales, src, lds, rows, cols));
+}
+
+void iris_dev_bf16_to_mxfp4(uint8_t *codes, uint8_t *scales, const uint16_t *src, int lds, int rows, int cols) {
+    if (!mxfp4_rows_args("bf16_to_mxfp4", src, codes, scales, lds, rows, cols)) return;
+    LAUNCH("bf16_to_mxfp4", iris_hip_bf16_to_mxfp4(g_stream, codes, scales, src, lds, rows, cols));
+}
+
+void iris_dev_mxfp4_to_f32(float *dst, int ldd, const uint8_t *codes, const uint8_t *scales, int rows, int cols) {
+    if (!mxfp4_rows_args("mxfp4_to_f32", dst, codes, scales, ldd, rows, cols)) return;
+    LAUNCH("mxfp4_to_f32", iris_hip_mxfp4_to_f32(g_stream, dst, ldd, codes, scales, rows, cols));
+}
+
+void iris_dev_mxfp4_to_bf16(uint16_t *dst, int ldd, const uint8_t *codes, const uint8_t *scales, int rows, int cols) {
+    if (!mxfp4_rows_args("mxfp4_to_bf16", dst, codes, scales, ldd, rows, cols)) return;
+    LAUNCH("mxfp4_to_bf16", iris_hip_mxfp4_to_bf16(g_stream, dst, ldd, codes, scales, rows, cols));
+}
+
+static int linear_mxfp4_args(const char *what, const void *y, const uint8_t *x, const uint8_t *xs, const uint8_t *W, const uint8_t *Ws, int rows, int in, int out) {
+    if (rows <= 0 || out <= 0) return 0;
+    if (in <= 0) { fail(-1, what, "in must be positive"); return 0; }
+    if (!y || !x || !xs || !W || !Ws) { fail(-1, what, "y, or codes or scales of x or W are missing"); return 0; }
+    if (!aligned(x, 16) || !aligned(W, 16)) { fail(-1, what, "codes must be 16-byte aligned"); return 0; }
+    return need_ready(what);
+}
+
+void iris_dev_linear_mxfp4_f32(float *y, const uint8_t *x, const uint8_t *x_scales, const uint8_t *W, const uint8_t *W_scales, int rows, int in, int out) {
+    if (!linear_mxfp4_args("linear_mxfp4", y, x, x_scales, W, W_scales, rows, in, out)) return;
+    g_last_kernel = "linear_mxfp4";
+    LAUNCH("linear_mxfp4", iris_hip_linear_mxfp4_f32(g_stream, y, x, x_scales, W, W_scales, NULL, 1, rows, in, out));
+}
+
+void iris_dev_linear_mxfp4_bf16(uint16_t *y, const uint8_t *x, const uint8_t *x_scales, const uint8_t *W, const uint8_t *W_scales, int rows, int in, int out) {
+    if (!linear_mxfp4_args("linear_mxfp4", y, x, x_scales, W, W_scales, rows, in, out)) return;
+    g_last_kernel = "linear_mxfp4";
+    LAUNCH("linear_mxfp4", iris_hip_linear_mxfp4_bf16(g_stream, y, x, x_scales, W, W_scales, NULL, 1, rows, in, out));
+}
+
+void iris_dev_linear_mxfp4_f32_grouped(float *y, const uint8_t *x, const uint8_t *x_scales, const uint8_t *W, const uint8_t *W_scales, const int *first_row,
+                                       int groups, int rows, int in, int out) {
+    if (rows <= 0 || out <= 0 || !grouped_args("linear_mxfp4_grouped", first_row, groups, in) || !groups ||
+        !linear_mxfp4_args("linear_mxfp4_grouped", y, x, x_scales, W, W_scales, rows, in, out))
+        return;
+    g_last_kernel = "linear_mxfp4_grouped";
+    LAUNCH("linear_mxfp4_grouped", iris_hip_linear_mxfp4_f32(g_stream, y, x, x_scales, W, W_scales, first_row, groups, rows, in, out));
+}
+
+void iris_dev_linear_mxfp4_bf16_grouped(uint16_t *y, const uint8_t *x, const uint8_t *x_scales, const uint8_t *W, const uint8_t *W_scales, const int *first_row,
+                                        int groups, int rows, int in, int out) {
+    if (rows <= 0 || out <= 0 || !grouped_args("linear_mxfp4_grouped", first_row, groups, in) || !groups ||
+        !linear_mxfp4_args("linear_mxfp4_grouped", y, x, x_scales, W, W_scales, rows, in, out))
+        return;
+    g_last_kernel = "linear_mxfp4_grouped";
+    LAUNCH("linear_mxfp4_grouped", iris_hip_linear_mxfp4_bf16(g_stream, y, x, x_scales, W, W_scales, first_row, groups, rows, in, out));
+}
+
 void iris_dev_layer_norm_mod(uint16_t *out, const float *x, const float *shift, const float *scale,
                              int rows, int dim, float eps) {
     LAUNCH("layer_norm_mod", iris_hip_layer_norm_mod(g_stream, out, x, shift, scale, rows, dim, eps));
