@@ -141,7 +141,8 @@ def check_exact(got, want, out):
 
 LAYERS = [(1, 32, 1), (1, 5, 3), (1, 4096, 512), (1, 4096, 515), (2, 64, 16), (3, 100, 17), (16, 256, 128), (17, 288, 129), (33, 1000, 111), (64, 2560, 384),
           (65, 2560, 257), (128, 512, 256), (129, 544, 260), (200, 768, 520), (256, 1024, 1024), (300, 1280, 448), (513, 256, 777), (640, 2560, 1536), (777, 1000, 1111),
-          (1024, 2304, 2048), (2050, 640, 2304)]
+          (1024, 2304, 2048), (2050, 640, 2304),
+          (256, 512, 192), (257, 768, 256), (511, 512, 200), (768, 1792, 3000)]
 
 
 @pytest.mark.parametrize("out", ["f32", "bf16"])
