@@ -39,6 +39,7 @@
 
 #include "iris_kernels_hip.h"
 #include "norm_rope_math.h"
+#include "row_groups.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -464,27 +465,40 @@ struct Wide {
     static constexpr int LDS = 2 * (2 * XS + 3 * WS) > 128 * 1024 ? 2 * (2 * XS + 3 * WS) : 128 * 1024;   /* the epilogue takes 128 KB */
 };
 
-template <typename OUT, int NA, bool QKN>
+template <typename OUT, int NA, bool QKN, bool GROUPED>
 __global__ void __launch_bounds__(512, 2)
 k_gemm_wide(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t *__restrict__ W, int M, int N, int K,
-            int tiles_m, int total, int per_xcd, int turns, QkNorm qn, const float *__restrict__ bias, int streaming_out) {
+            int tiles_m, int total, int per_xcd, int turns, QkNorm qn, const float *__restrict__ bias, int streaming_out, RowGroupsArg grouped) {
     using T = Wide<NA>;
     constexpr int TM = T::TM, TN = T::TN, XS = T::XS, WS = T::WS, WP = T::WP, H0 = (NA + 1) / 2, H1 = NA / 2;
     static_assert(WP <= 4 && H1 >= 2, "");
     extern __shared__ __align__(16) uint16_t dlds[];           /* x, x, W, W, W */
+    const int tiles_n = total / tiles_m;
+    RowGroups<TM> all;                                         /* GROUPED: only the device knows the row tiles, the grid has room for the most there can be */
+    if constexpr (GROUPED) {
+        tiles_m = all.count(grouped.first_row, grouped.groups, M);
+        total = tiles_m * tiles_n;
+        per_xcd = (total + 7) / 8;
+        if ((int)(blockIdx.x / 8) >= per_xcd) return;
+    }
     const int work = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
     if (work >= total) return;
     constexpr int BAND = 4;
-    const int tiles_n = total / tiles_m;
     const int band = work / (BAND * tiles_n), in_band = work - band * (BAND * tiles_n);
     const int band_rows = min(tiles_m - band * BAND, BAND);
-    const int m0 = (band * BAND + in_band % band_rows) * TM, n0 = in_band / band_rows * TN;
+    const int tm = band * BAND + in_band % band_rows, n0 = in_band / band_rows * TN;
+    RowTile rows = {tm * TM, M, 0};
+    if constexpr (GROUPED) {
+        rows = all.tile(tm);
+        W += (size_t)rows.group * N * K;
+    }
+    const int m0 = rows.m0, m_end = rows.end;
     const int last_tile = K / TK - 1;
     /* The workgroups that share rows of W or x run in step; they take the k tiles of a group of four in different orders, so
      * that one of them brings a line from HBM and the others find it in the L2 (gemm_tiles_gfx950.hip has the reasons, and where
      * not); by the tile row alone, so that all widths add in the same order. All in one order / turned, us: 512 x 2560 -> 19456 49.1 / 47.4,
      * 512 x 3072 -> 27648 73.8 / 71.2, 1024 x 2560 -> 19456 96.3 / 92.5; 4608 rows within 1 %. */
-    const int turn = (m0 / TM) & turns, turned = (last_tile + 1) & ~3;
+    const int turn = tm & turns, turned = (last_tile + 1) & ~3;
     auto source = [&](int kt) { return (size_t)(kt < turned ? kt ^ turn : kt) * TK; };
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4, wm = wave & 3, wn = wave >> 2;
@@ -496,7 +510,7 @@ k_gemm_wide(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t 
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int r = 8 * (4 * wave + j) + (lane >> 3);
-        xoff[j] = ((uint32_t)(min(m0 + r, M - 1) - m0) * (uint32_t)K + 8u * ((lane & 7) ^ ((r >> 1) & 7))) * 2u;
+        xoff[j] = ((uint32_t)(min(m0 + r, m_end - 1) - m0) * (uint32_t)K + 8u * ((lane & 7) ^ ((r >> 1) & 7))) * 2u;
     }
 #pragma unroll
     for (int j = 0; j < WP; j++) {
@@ -628,7 +642,7 @@ k_gemm_wide(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t 
 #pragma unroll 4
             for (int pass = 0; pass < DT / 16; pass++) {
                 const int row = 16 * pass + row_in, m = m0 + row;
-                if (m >= M || n_head >= N) continue;            /* the same for the 16 lanes of a vector */
+                if (m >= m_end || n_head >= N) continue;            /* the same for the 16 lanes of a vector */
                 u32x4 v = *reinterpret_cast<const u32x4 *>(&dlds[row * 256 + 8 * ((chunk & 16) | ((chunk ^ row) & 15))]);
                 if (normed) {
                     const float *cr = qn.rope_cos + (size_t)m * 64 + tcol, *sr = qn.rope_sin + (size_t)m * 64 + tcol;
@@ -666,7 +680,7 @@ k_gemm_wide(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t 
             for (int it = 0; it < 16; it++) {
                 const int row = 2 * it + (lane >> 5), c = lane & 31, m = mw + 32 * half + row, n = nw + PER16 * c;
                 f32x4 v = *reinterpret_cast<const f32x4 *>(&buf[row * 128 + 4 * ((c & 16) | ((c ^ row) & 15))]);
-                if (c < 4 * NA && m < M && n < N) {
+                if (c < 4 * NA && m < m_end && n < N) {
                     if (bias) v += *reinterpret_cast<const f32x4 *>(bias + n);
                     f32x4 *dst = reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(y) + (size_t)m * N + n);
                     if (streaming_out) __builtin_nontemporal_store(v, dst);
@@ -688,7 +702,7 @@ k_gemm_wide(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t 
         for (int it = 0; it < 16; it++) {
             const int row = 4 * it + (lane >> 4), c = lane & 15, m = mw + row, n = nw + PER16 * c;
             const u32x4 v = *reinterpret_cast<const u32x4 *>(&buf[row * 128 + 8 * (c ^ (row & 15))]);
-            if (c < 2 * NA && m < M && n < N) {
+            if (c < 2 * NA && m < m_end && n < N) {
                 u32x4 *dst = reinterpret_cast<u32x4 *>(reinterpret_cast<uint16_t *>(y) + (size_t)m * N + n);
                 if (streaming_out) __builtin_nontemporal_store(v, dst);
                 else *dst = v;
@@ -735,25 +749,26 @@ k_gemm_scalar(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_
 static long wide_wgs(int M, int N, int na) { return (long)((M + DT - 1) / DT) * ((N + 32 * na - 1) / (32 * na)); }
 
 /* in_order: all workgroups take the k tiles in one order; otherwise that goes by the grid of 256-column tiles, whatever the width */
-template <typename OUT, int NA, bool QKN = false>
+template <typename OUT, int NA, bool QKN = false, bool GROUPED = false>
 int launch_gemm_wide(hipStream_t st, OUT *y, const uint16_t *x, const uint16_t *W, int M, int N, int K, const float *bias, const QkNorm &qn = QkNorm{},
-                     bool in_order = false) {
+                     bool in_order = false, RowGroupsArg grouped = {}) {
     static bool configured = false;
     if (!configured) {
-        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k_gemm_wide<OUT, NA, QKN>),
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k_gemm_wide<OUT, NA, QKN, GROUPED>),
                                            hipFuncAttributeMaxDynamicSharedMemorySize, Wide<NA>::LDS);
         if (e != hipSuccess) return (int)e;
         configured = true;
     }
-    const int tiles_m = (M + DT - 1) / DT, tiles_n = (N + 32 * NA - 1) / (32 * NA), total = tiles_m * tiles_n;
+    const int tiles_m = GROUPED ? (int)row_tiles_at_most(M, grouped.groups, DT) : (M + DT - 1) / DT, tiles_n = (N + 32 * NA - 1) / (32 * NA),
+              total = tiles_m * tiles_n;
     const int per_xcd = (total + 7) / 8;
     /* An output of 192 MB or more cannot stay in the 256 MB Infinity Cache next to the operands: stored with the
      * streaming hint it does not push the weights out on its way (4608 x 3072 -> 27648: f32 output 671 -> 626 us, bf16
      * 594 -> 585 when it was introduced; smaller outputs are within 1 % either way and keep the plain stores, which leave
      * them cached for the operator that reads them next). */
     const int streaming_out = (size_t)M * N * sizeof(OUT) >= ((size_t)192 << 20);
-    hipLaunchKernelGGL((k_gemm_wide<OUT, NA, QKN>), dim3((unsigned)per_xcd * 8), dim3(512), Wide<NA>::LDS, st, y, x, W, M, N, K,
-                       tiles_m, total, per_xcd, in_order ? 0 : iris_hip_gemm_turns(wide_wgs(M, N, 8), (size_t)N * K * 2), qn, bias, streaming_out);
+    hipLaunchKernelGGL((k_gemm_wide<OUT, NA, QKN, GROUPED>), dim3((unsigned)per_xcd * 8), dim3(512), Wide<NA>::LDS, st, y, x, W, M, N, K,
+                       tiles_m, total, per_xcd, in_order ? 0 : iris_hip_gemm_turns(wide_wgs(M, N, 8), (size_t)N * K * 2), qn, bias, streaming_out, grouped);
     return (int)hipGetLastError();
 }
 
@@ -769,8 +784,7 @@ static bool wide_shape(int M, int N, int K, size_t out_size) {
  * rounds x width. 4608 x 9216 outputs: 648 tiles of 256 columns are 2.53 rounds, 756 of 224 are 2.95. 160 columns read half as
  * much again from the LDS per product as 256 and are only taken where they fill one round that wider tiles leave a fifth idle,
  * 512 rows: 2560 -> 19456 204 tiles of 192 columns 52.5 us, 244 of 160 51.3; 3072 -> 18432 57.5 / 56.0, 4096 -> 20480 78.2 / 74.9. */
-static int wide_width(int M, int N) {
-    const long tiles_m = (M + DT - 1) / DT;
+static int wide_width_of(long tiles_m, int N) {
     int best = 8;
     long best_cost = 0;
     for (int na = 8; na >= 5; na--) {
@@ -782,11 +796,14 @@ static int wide_width(int M, int N) {
     return best;
 }
 
+static int wide_width(int M, int N) { return wide_width_of((M + DT - 1) / DT, N); }
+
 /* the estimated time of a grid of k_gemm_wide with tiles of 32 na columns */
-static float wide_us(int M, int N, int K, int na) {
-    const long wgs = wide_wgs(M, N, na), rounds = (wgs + 255) / 256;
+static float wide_us_of(long wgs, int K, int na) {
+    const long rounds = (wgs + 255) / 256;
     return 4.0f + (float)rounds * ((float)(K / TK) * (wgs <= 128 ? 0.145f : 0.175f) * (float)na + 4.0f);
 }
+static float wide_us(int M, int N, int K, int na) { return wide_us_of(wide_wgs(M, N, na), K, na); }
 
 /* Which kernel a linear layer takes, host arithmetic only: 4 = k_gemm_tiles (gemm_tiles_gfx950.hip) with its tile `na` and
  * `splits` ranges of K, 3 = k_gemm_wide with tiles of 32 na columns, 2 = k_gemm_dma, 1 = k_gemm_bf16, 0 = k_gemm_scalar.
@@ -909,6 +926,23 @@ int iris_hip_linear_f32(void *stream, float *part, float *y, const uint16_t *x, 
 }
 int iris_hip_linear_bf16(void *stream, float *part, uint16_t *y, const uint16_t *x, const uint16_t *W, int rows, int in, int out) {
     return gemm<uint16_t>((hipStream_t)stream, y, x, W, rows, out, in, part, part ? IRIS_LINEAR_PART_BYTES : 0);
+}
+
+/* Rows in groups in tiles of 256 rows, for products that k_gemm_wide takes: their width and estimated time, negative where it does not */
+float iris_hip_gemm_wide_grouped_plan(int groups, int M, int N, int K, int out_size, int *na) {
+    if (!wide_shape(M, N, K, (size_t)out_size) || N < DT) return -1.0f;
+    const long tiles_m = row_tiles_about(M, groups, DT);
+    *na = wide_width_of(tiles_m, N);
+    return wide_us_of(tiles_m * ((N + 32 * *na - 1) / (32 * *na)), K, *na);
+}
+int iris_hip_gemm_wide_grouped(void *stream, void *y, int out_size, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int M, int N, int K, int na) {
+    hipStream_t st = (hipStream_t)stream;
+    const RowGroupsArg g = {first_row, groups};
+    const QkNorm none = {};
+#define WIDE(NA) (out_size == 2 ? launch_gemm_wide<uint16_t, NA, false, true>(st, (uint16_t *)y, x, W, M, N, K, nullptr, none, false, g) \
+                                : launch_gemm_wide<float, NA, false, true>(st, (float *)y, x, W, M, N, K, nullptr, none, false, g))
+    return na == 8 ? WIDE(8) : na == 7 ? WIDE(7) : na == 6 ? WIDE(6) : WIDE(5);
+#undef WIDE
 }
 
 /* How the projection that normalises its own columns runs, host arithmetic only: 1 k_gemm_wide in tiles of 256 columns that

@@ -42,6 +42,7 @@
 #include <type_traits>
 
 #include "iris_kernels_hip.h"
+#include "row_groups.h"
 #include "write_through.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -77,14 +78,22 @@ struct Tile {
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"                          /* M0 in a clobber list */
-template <typename OUT, int NB, int WM, int NA, int WN, int KG, int STAGES, bool THROUGH>
+template <typename OUT, int NB, int WM, int NA, int WN, int KG, int STAGES, bool THROUGH, bool GROUPED>
 __global__ void __launch_bounds__(64 * WM * WN * KG, WM * WN * KG / 4)
 k_gemm_tiles(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t *__restrict__ W, int M, int N, int K,
-             const float *__restrict__ bias, int tiles_m, int tiles_n, int splits, int total, int per_xcd, int turns) {
+             const float *__restrict__ bias, int tiles_m, int tiles_n, int splits, int total, int per_xcd, int turns, RowGroupsArg grouped) {
     using T = Tile<NB, WM, NA, WN, KG, STAGES>;
     constexpr int TM = T::TM, TN = T::TN, STAGE = T::STAGE, PIECES = T::PIECES;
     static_assert(T::LDS <= 160 * 1024 && NA <= 8 && (KG == 1 || (KG == 2 && NB % 2 == 0)), "");
     extern __shared__ __align__(16) uint16_t lds[];
+    /* GROUPED: only the device knows the row tiles, the grid has room for the most there can be */
+    RowGroups<TM> all;
+    if constexpr (GROUPED) {
+        tiles_m = all.count(grouped.first_row, grouped.groups, M);
+        total = tiles_m * tiles_n * splits;
+        per_xcd = (total + 7) / 8;
+        if ((int)(blockIdx.x / 8) >= per_xcd) return;
+    }
     /* An XCD (own L2) takes a contiguous range of the work list: K ranges outermost, then bands of 8 tile rows, inside a
      * band m fastest: its 32 CUs share the W tiles and each other's x rows. */
     const int work = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
@@ -93,13 +102,19 @@ k_gemm_tiles(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t
     const int per_split = tiles_m * tiles_n, split = work / per_split, in_split = work - split * per_split;
     const int band = in_split / (BAND * tiles_n), in_band = in_split - band * (BAND * tiles_n);
     const int band_rows = min(tiles_m - band * BAND, BAND);
-    const int m0 = (band * BAND + in_band % band_rows) * TM, n0 = in_band / band_rows * TN;
+    const int tm = band * BAND + in_band % band_rows, n0 = in_band / band_rows * TN;
+    RowTile rows = {tm * TM, M, 0};
+    if constexpr (GROUPED) {
+        rows = all.tile(tm);
+        W += (size_t)rows.group * N * K;
+    }
+    const int m0 = rows.m0, m_end = rows.end;
     const int nk_all = K / TK, kt0 = (int)((long)nk_all * split / splits), nk = (int)((long)nk_all * (split + 1) / splits) - kt0;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4;
     /* the order of this workgroup's k tiles, see above: tile kt of the order is k tile kt ^ turn inside whole groups of four */
-    const int turn = (m0 / TM ^ n0 / TN) & turns, turned = nk & ~3;
+    const int turn = (tm ^ n0 / TN) & turns, turned = nk & ~3;
     const int wm = wave % WM, wn = wave / WM % WN, kg = wave / (WM * WN);
 
     /* this wave's pieces of a stage: row 8 (PIECES wave + j) + lane / 8 of [W tile | x tile]; rows past the end of a matrix
@@ -110,7 +125,7 @@ k_gemm_tiles(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t
     for (int j = 0; j < PIECES; j++) {
         piece[j] = min(PIECES * wave + j, (TM + TN) / 8 - 1);
         const int r = 8 * piece[j] + (lane >> 3);
-        const int row = r < TN ? min(n0 + r, N - 1) : min(m0 + r - TN, M - 1);
+        const int row = r < TN ? min(n0 + r, N - 1) : min(m0 + r - TN, m_end - 1);
         off[j] = ((uint32_t)row * (uint32_t)K + 8u * ((lane & 7) ^ ((r >> 1) & 7))) * 2u;
     }
     auto request_one = [&](int j, int kt, uint16_t *stage) {
@@ -255,7 +270,7 @@ k_gemm_tiles(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t
             for (int it = 0; it < 4 * NBS; it++) {
                 const int row = 4 * it + (lane >> 4), c = lane & 15, m = mw + row, n = nc + 4 * c;
                 f32x4 v = *reinterpret_cast<const f32x4 *>(&buf[row * 64 + 4 * (c ^ (row & 15))]);
-                if (c < 4 * na && m < M && n < N) {
+                if (c < 4 * na && m < m_end && n < N) {
                     if (bias) v += *reinterpret_cast<const f32x4 *>(bias + n);
                     if constexpr (THROUGH) store_through(dst + (size_t)m * N + n, v);
                     else *reinterpret_cast<f32x4 *>(dst + (size_t)m * N + n) = v;
@@ -275,7 +290,7 @@ k_gemm_tiles(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t
             for (int it = 0; it < 2 * NBS; it++) {
                 const int row = 8 * it + (lane >> 3), c = lane & 7, m = mw + row, n = nc + 8 * c;
                 const u32x4 v = *reinterpret_cast<const u32x4 *>(&buf[row * 64 + 8 * (c ^ (row & 7))]);
-                if (c < 2 * na && m < M && n < N) *reinterpret_cast<u32x4 *>(dst + (size_t)m * N + n) = v;
+                if (c < 2 * na && m < m_end && n < N) *reinterpret_cast<u32x4 *>(dst + (size_t)m * N + n) = v;
             }
         }
     }
@@ -287,10 +302,15 @@ k_gemm_tiles(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t
  * the layer in front of it, us, eight values a thread and one after the other / now: 512 x 9728 -> 2560 (6 ranges) 36.5 / 36.0,
  * 512 x 9216 -> 3072 (4) 39.7 / 38.9, 700 x 12288 -> 3072 (3) 62.2 / 61.1, 1000 x 9728 -> 2560 (3) 56.4 / 54.9; 100 and 320 rows the same. */
 constexpr int SUM_MOST = 8;
-template <typename OUT, int AT_ONCE>
+template <typename OUT, int AT_ONCE, bool GROUPED>
 __global__ void __launch_bounds__(256)
-k_gemm_sum(OUT *__restrict__ y, const float *__restrict__ part, size_t n, int splits) {
+k_gemm_sum(OUT *__restrict__ y, const float *__restrict__ part, size_t n, int splits, RowGroupsArg grouped, int M, int N) {
     const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if constexpr (GROUPED) {                                   /* rows in no group have no sums */
+        int from, to;
+        row_groups_span(grouped.first_row, grouped.groups, M, &from, &to);
+        if (i < (size_t)from * N || i >= (size_t)to * N) return;
+    }
     if (i >= n) return;
     f32x4 v[AT_ONCE];
 #pragma unroll
@@ -303,11 +323,12 @@ k_gemm_sum(OUT *__restrict__ y, const float *__restrict__ part, size_t n, int sp
     else *reinterpret_cast<uint2 *>(y + i) = make_uint2(pack_bf16(v[0][0], v[0][1]), pack_bf16(v[0][2], v[0][3]));
 }
 
-template <typename OUT, int AT_ONCE = SUM_MOST>
-int launch_sum(hipStream_t st, OUT *y, const float *part, size_t n, int splits) {
+template <typename OUT, bool GROUPED = false, int AT_ONCE = SUM_MOST>
+int launch_sum(hipStream_t st, OUT *y, const float *part, int M, int N, int splits, RowGroupsArg grouped = {}) {
     if constexpr (AT_ONCE > 2)
-        if (splits < AT_ONCE) return launch_sum<OUT, AT_ONCE - 1>(st, y, part, n, splits);
-    hipLaunchKernelGGL((k_gemm_sum<OUT, AT_ONCE>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, y, part, n, splits);
+        if (splits < AT_ONCE) return launch_sum<OUT, GROUPED, AT_ONCE - 1>(st, y, part, M, N, splits, grouped);
+    const size_t n = (size_t)M * N;
+    hipLaunchKernelGGL((k_gemm_sum<OUT, AT_ONCE, GROUPED>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, y, part, n, splits, grouped, M, N);
     return (int)hipGetLastError();
 }
 
@@ -320,21 +341,22 @@ static int turns(int M, int N, int K, int wgs) {
 
 /* THROUGH is a template's choice: with a test in front of every store of one kernel, plain ones took 0.5 - 2 % longer. us, one kernel / two / one that
  * only stores plainly: 96 x 2560 -> 6144 16.12 / 15.74 / 15.79, 150 x 12288 -> 3072 29.27 / 29.04 / 28.99, 900 x 12288 -> 3072 77.6 / 76.6 / 76.7. */
-template <typename OUT, int NB, int WM, int NA, int WN, int KG, int STAGES, bool THROUGH = false>
-int launch_tiles(hipStream_t st, OUT *y, const uint16_t *x, const uint16_t *W, int M, int N, int K, const float *bias, int splits, bool through) {
+template <typename OUT, bool GROUPED, int NB, int WM, int NA, int WN, int KG, int STAGES, bool THROUGH = false>
+int launch_tiles(hipStream_t st, OUT *y, const uint16_t *x, const uint16_t *W, int M, int N, int K, const float *bias, int splits, bool through, RowGroupsArg grouped) {
     if constexpr (sizeof(OUT) == 4 && !THROUGH)
-        if (through) return launch_tiles<OUT, NB, WM, NA, WN, KG, STAGES, true>(st, y, x, W, M, N, K, bias, splits, true);
+        if (through) return launch_tiles<OUT, GROUPED, NB, WM, NA, WN, KG, STAGES, true>(st, y, x, W, M, N, K, bias, splits, true, grouped);
     using T = Tile<NB, WM, NA, WN, KG, STAGES>;
     static bool configured = false;
     if (!configured) {
-        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k_gemm_tiles<OUT, NB, WM, NA, WN, KG, STAGES, THROUGH>),
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k_gemm_tiles<OUT, NB, WM, NA, WN, KG, STAGES, THROUGH, GROUPED>),
                                            hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
         if (e != hipSuccess) return (int)e;
         configured = true;
     }
-    const int tiles_m = (M + T::TM - 1) / T::TM, tiles_n = (N + T::TN - 1) / T::TN, total = tiles_m * tiles_n * splits, per_xcd = (total + 7) / 8;
-    hipLaunchKernelGGL((k_gemm_tiles<OUT, NB, WM, NA, WN, KG, STAGES, THROUGH>), dim3((unsigned)per_xcd * 8), dim3(T::THREADS), T::LDS, st, y, x, W, M, N, K,
-                       bias, tiles_m, tiles_n, splits, total, per_xcd, turns(M, N, K, total));
+    const int tiles_m = GROUPED ? (int)row_tiles_at_most(M, grouped.groups, T::TM) : (M + T::TM - 1) / T::TM, tiles_n = (N + T::TN - 1) / T::TN,
+              total = tiles_m * tiles_n * splits, per_xcd = (total + 7) / 8;
+    hipLaunchKernelGGL((k_gemm_tiles<OUT, NB, WM, NA, WN, KG, STAGES, THROUGH, GROUPED>), dim3((unsigned)per_xcd * 8), dim3(T::THREADS), T::LDS, st, y, x, W, M, N, K,
+                       bias, tiles_m, tiles_n, splits, total, per_xcd, turns(M, N, K, total), grouped);
     return (int)hipGetLastError();
 }
 
@@ -351,20 +373,48 @@ constexpr Shape SHAPES[] = {{128, 128, 0.44f, 0.50f, 0.55f, 100}, {128, 192, 0.5
                             {160, 224, 0.836f, 0.87f, 0.89f, 64}, {128, 96, 0.39f, 0.45f, 0.50f, 64}};
 constexpr int NSHAPES = sizeof(SHAPES) / sizeof(SHAPES[0]);
 
-template <typename OUT>
+template <typename OUT, bool GROUPED = false>
 int launch_shape(hipStream_t st, int shape, OUT *y, const uint16_t *x, const uint16_t *W, int M, int N, int K, const float *bias, int splits,
-                 bool through = false) {
+                 bool through = false, RowGroupsArg grouped = {}) {
     switch (shape) {
-    case 0: return launch_tiles<OUT, 4, 2, 4, 2, 2, 4>(st, y, x, W, M, N, K, bias, splits, through);
-    case 1: return launch_tiles<OUT, 4, 2, 3, 4, 1, 4>(st, y, x, W, M, N, K, bias, splits, through);
-    case 2: return launch_tiles<OUT, 4, 2, 4, 4, 1, 3>(st, y, x, W, M, N, K, bias, splits, through);
-    case 3: return launch_tiles<OUT, 4, 1, 4, 4, 2, 4>(st, y, x, W, M, N, K, bias, splits, through);
-    case 4: return launch_tiles<OUT, 5, 2, 3, 4, 1, 3>(st, y, x, W, M, N, K, bias, splits, through);
-    case 5: return launch_tiles<OUT, 5, 2, 4, 4, 1, 3>(st, y, x, W, M, N, K, bias, splits, through);
-    case 6: return launch_tiles<OUT, 5, 2, 7, 2, 1, 3>(st, y, x, W, M, N, K, bias, splits, through);
-    case 7: return launch_tiles<OUT, 4, 2, 3, 2, 2, 4>(st, y, x, W, M, N, K, bias, splits, through);
+    case 0: return launch_tiles<OUT, GROUPED, 4, 2, 4, 2, 2, 4>(st, y, x, W, M, N, K, bias, splits, through, grouped);
+    case 1: return launch_tiles<OUT, GROUPED, 4, 2, 3, 4, 1, 4>(st, y, x, W, M, N, K, bias, splits, through, grouped);
+    case 2: return launch_tiles<OUT, GROUPED, 4, 2, 4, 4, 1, 3>(st, y, x, W, M, N, K, bias, splits, through, grouped);
+    case 3: return launch_tiles<OUT, GROUPED, 4, 1, 4, 4, 2, 4>(st, y, x, W, M, N, K, bias, splits, through, grouped);
+    case 4: return launch_tiles<OUT, GROUPED, 5, 2, 3, 4, 1, 3>(st, y, x, W, M, N, K, bias, splits, through, grouped);
+    case 5: return launch_tiles<OUT, GROUPED, 5, 2, 4, 4, 1, 3>(st, y, x, W, M, N, K, bias, splits, through, grouped);
+    case 6: return launch_tiles<OUT, GROUPED, 5, 2, 7, 2, 1, 3>(st, y, x, W, M, N, K, bias, splits, through, grouped);
+    case 7: return launch_tiles<OUT, GROUPED, 4, 2, 3, 2, 2, 4>(st, y, x, W, M, N, K, bias, splits, through, grouped);
     default: return (int)hipErrorInvalidValue;
     }
+}
+
+/* The cheapest tile and number of K ranges for a product, and its estimated time in us; negative where these kernels do
+ * not take it: they want rows of 16-byte chunks (N % 8), whole k tiles and enough of them to fill the ring, and 32-bit
+ * byte offsets. Partial sums take splits * M * N floats of the workspace. Host arithmetic only. */
+float plan_tiles(int M, int N, int K, int out_size, size_t part_bytes, int groups, int *shape, int *splits) {
+    constexpr int MIN_TILES = 6;                               /* k tiles of a range */
+    if (M <= 0 || N < 128 || N % 8 || K % TK || K < 8 * TK || ((size_t)M * K * 2) >> 32 || ((size_t)N * K * 2) >> 32) return -1.0f;
+    const int nk = K / TK;
+    float best = -1.0f;
+    for (int i = 0; i < NSHAPES; i++) {
+        const long tiles_m = groups == 1 ? (M + SHAPES[i].tm - 1) / SHAPES[i].tm : row_tiles_about(M, groups, SHAPES[i].tm);
+        const long tiles = tiles_m * ((N + SHAPES[i].tn - 1) / SHAPES[i].tn);
+        for (int s = 1; s == 1 || (s * MIN_TILES <= nk && (size_t)s * M * N * 4 <= part_bytes && tiles * s <= 512); s++) {
+            const long wgs = tiles * s, rounds = (wgs + 255) / 256;
+            /* Rows of a multiple of 32 KB cut into ranges of a multiple of 4 KB: the lines that a single row of tiles fetches at a time
+             * lie as far apart, and come slower. 112 x 16384 -> 4096 in eight ranges of 128 x 128 41.7 us, 16448 -> 4096 36.6; in
+             * sixteen of 128 x 256 36.9. */
+            const float far_apart = M <= SHAPES[i].tm && K % 16384 == 0 && ((nk + s - 1) / s) % 32 == 0 ? 1.3f : 1.0f;
+            const float step = rounds > 2 ? SHAPES[i].step_more : rounds > 1 ? SHAPES[i].step_two : SHAPES[i].step;
+            /* the sum: a launch, and its reads at 5 TB/s; with groups 4 us more, while it finds the rows that have one: 2 groups of 100 rows, 2560 -> 6144,
+             * five ranges of 128 x 256 26.4 us, K whole in 128 x 96 19.3 */
+            const float sum = s > 1 ? (groups > 1 ? 7.0f : 3.0f) + ((float)s * 4.0f + (float)out_size) * (float)M * (float)N / 5e6f : 0.0f;
+            const float cost = 4.0f + (float)rounds * ((float)((nk + s - 1) / s) * step * far_apart + 3.5f) + sum;
+            if (best < 0.0f || cost < best) { best = cost; *shape = i; *splits = s; }
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -400,30 +450,8 @@ int iris_hip_gemm_tiles_through(int shape, int splits, int M, int N, int K) {
     return splits > 1 && (size_t)splits * M * N * 4 <= (size_t)20 << 20 && (size_t)N * K * 2 <= (size_t)SHAPES[shape].through << 20;
 }
 
-/* The cheapest tile and number of K ranges for a product, and its estimated time in us; negative where these kernels do
- * not take it: they want rows of 16-byte chunks (N % 8), whole k tiles and enough of them to fill the ring, and 32-bit
- * byte offsets. Partial sums take splits * M * N floats of the workspace. Host arithmetic only. */
 float iris_hip_gemm_tiles_plan(int M, int N, int K, int out_size, size_t part_bytes, int *shape, int *splits) {
-    constexpr int MIN_TILES = 6;                               /* k tiles of a range */
-    if (M <= 0 || N < 128 || N % 8 || K % TK || K < 8 * TK || ((size_t)M * K * 2) >> 32 || ((size_t)N * K * 2) >> 32) return -1.0f;
-    const int nk = K / TK;
-    float best = -1.0f;
-    for (int i = 0; i < NSHAPES; i++) {
-        const long tiles = (long)((M + SHAPES[i].tm - 1) / SHAPES[i].tm) * ((N + SHAPES[i].tn - 1) / SHAPES[i].tn);
-        for (int s = 1; s == 1 || (s * MIN_TILES <= nk && (size_t)s * M * N * 4 <= part_bytes && tiles * s <= 512); s++) {
-            const long wgs = tiles * s, rounds = (wgs + 255) / 256;
-            /* Rows of a multiple of 32 KB cut into ranges of a multiple of 4 KB: the lines that a single row of tiles fetches at a time
-             * lie as far apart, and come slower. 112 x 16384 -> 4096 in eight ranges of 128 x 128 41.7 us, 16448 -> 4096 36.6; in
-             * sixteen of 128 x 256 36.9. */
-            const float far_apart = M <= SHAPES[i].tm && K % 16384 == 0 && ((nk + s - 1) / s) % 32 == 0 ? 1.3f : 1.0f;
-            const float step = rounds > 2 ? SHAPES[i].step_more : rounds > 1 ? SHAPES[i].step_two : SHAPES[i].step;
-            /* the sum: a launch, and its reads at 5 TB/s */
-            const float sum = s > 1 ? 3.0f + ((float)s * 4.0f + (float)out_size) * (float)M * (float)N / 5e6f : 0.0f;
-            const float cost = 4.0f + (float)rounds * ((float)((nk + s - 1) / s) * step * far_apart + 3.5f) + sum;
-            if (best < 0.0f || cost < best) { best = cost; *shape = i; *splits = s; }
-        }
-    }
-    return best;
+    return plan_tiles(M, N, K, out_size, part_bytes, 1, shape, splits);
 }
 
 /* part: splits * M * N floats, 16-byte aligned, when splits > 1. x, W, y, bias 16-byte aligned; bias (or null) [N], with f32
@@ -436,8 +464,25 @@ int iris_hip_gemm_tiles(void *stream, void *y, int out_size, const uint16_t *x, 
                              : launch_shape<float>(st, shape, (float *)y, x, W, M, N, K, bias, 1);
     int e = launch_shape<float>(st, shape, part, x, W, M, N, K, nullptr, splits, iris_hip_gemm_tiles_through(shape, splits, M, N, K) != 0);
     if (e) return e;
-    const size_t n = (size_t)M * N;
-    return out_size == 2 ? launch_sum(st, (uint16_t *)y, part, n, splits) : launch_sum(st, (float *)y, part, n, splits);
+    return out_size == 2 ? launch_sum(st, (uint16_t *)y, part, M, N, splits) : launch_sum(st, (float *)y, part, M, N, splits);
+}
+
+/* The same for rows in groups, W [groups, N, K]. */
+int iris_hip_gemm_tiles_grouped(void *stream, void *y, int out_size, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int M, int N, int K,
+                                int shape, int splits, float *part) {
+    hipStream_t st = (hipStream_t)stream;
+    const RowGroupsArg g = {first_row, groups};
+    if (splits == 1)
+        return out_size == 2 ? launch_shape<uint16_t, true>(st, shape, (uint16_t *)y, x, W, M, N, K, nullptr, 1, false, g)
+                             : launch_shape<float, true>(st, shape, (float *)y, x, W, M, N, K, nullptr, 1, false, g);
+    int e = launch_shape<float, true>(st, shape, part, x, W, M, N, K, nullptr, splits, iris_hip_gemm_tiles_through(shape, splits, M, N, K) != 0, g);
+    if (e) return e;
+    return out_size == 2 ? launch_sum<uint16_t, true>(st, (uint16_t *)y, part, M, N, splits, g) : launch_sum<float, true>(st, (float *)y, part, M, N, splits, g);
+}
+
+/* Its tile and K ranges, from about how many tiles there will be: a negative time where these kernels do not take the product. */
+float iris_hip_gemm_tiles_grouped_plan(int groups, int M, int N, int K, int out_size, size_t part_bytes, int *shape, int *splits) {
+    return plan_tiles(M, N, K, out_size, part_bytes, groups, shape, splits);
 }
 
 }  // extern "C"

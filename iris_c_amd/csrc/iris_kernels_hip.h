@@ -156,10 +156,18 @@ float iris_hip_gemm_tiles_plan(int M, int N, int K, int out_size, size_t part_by
 int iris_hip_gemm_tiles(void *stream, void *y, int out_size, const uint16_t *x, const uint16_t *W, int M, int N, int K,
                         const float *bias, int shape, int splits, float *part);
 
+/* rows in groups (row_groups.h) on the tiles of both, for products whose operands are 16-byte aligned; a plan is negative where they do not take one */
+float iris_hip_gemm_tiles_grouped_plan(int groups, int M, int N, int K, int out_size, size_t part_bytes, int *shape, int *splits);
+int iris_hip_gemm_tiles_grouped(void *stream, void *y, int out_size, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int M, int N, int K,
+                                int shape, int splits, float *part);
+float iris_hip_gemm_wide_grouped_plan(int groups, int M, int N, int K, int out_size, int *na);
+int iris_hip_gemm_wide_grouped(void *stream, void *y, int out_size, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int M, int N, int K, int na);
+
 /* The same for groups of rows with weights of their own, W [groups, out, in]: rows [first_row[g], first_row[g + 1]) take W[g], rows in no
  * group are left alone; first_row: device int [groups + 1] (gemm_grouped_gfx950.hip). Any sizes and alignment. */
-int iris_hip_linear_f32_grouped(void *stream, float *y, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int rows, int in, int out);
-int iris_hip_linear_bf16_grouped(void *stream, uint16_t *y, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int rows, int in, int out);
+void iris_hip_linear_grouped_plan(int groups, int rows, int in, int out, int out_bytes, int *plan);
+int iris_hip_linear_f32_grouped(void *stream, float *part, float *y, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int rows, int in, int out);
+int iris_hip_linear_bf16_grouped(void *stream, float *part, uint16_t *y, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int rows, int in, int out);
 
 /* ---- microscaled 4-bit floating point (mxfp4_ops.hip, gemm_mxfp4_gfx950.hip) ---- */
 /* rows [rows, cols] of stride ld at any alignment <-> codes [rows, 16 * blocks] (4-byte aligned), scales [rows, blocks]; blocks = cols / 32, rounded up */

@@ -12,6 +12,8 @@
 #ifndef IRIS_ROW_GROUPS_H
 #define IRIS_ROW_GROUPS_H
 
+struct RowGroupsArg { const int *first_row; int groups; };    /* the kernels' argument */
+
 struct RowTile { int m0, end, group; };          /* rows [m0, min(m0 + height, end)) */
 
 template <int HEIGHT>
@@ -68,10 +70,27 @@ struct RowGroups {
     }
 };
 
+/* the rows that are in a group, [*from, *to): what the whole wave finds */
+__device__ __forceinline__ void row_groups_span(const int *first, int groups, int rows, int *from, int *to) {
+    int most = first[0];
+    const int lo = min(max(most, 0), rows);
+    for (int i = threadIdx.x & 63; i <= groups; i += 64) most = max(most, first[i]);
+    for (int d = 32; d > 0; d >>= 1) most = max(most, __shfl_xor(most, d, 64));
+    *from = lo;
+    *to = min(max(most, 0), rows);
+}
+
 /* the most tiles that `rows` rows in `groups` groups can have */
 static inline long row_tiles_at_most(int rows, int groups, int height) {
     const long some = groups < rows ? groups : rows;
     return (rows + some * (height - 1)) / height;
+}
+
+/* about how many they have: where groups are long, those of rows without groups and half a tile more for each further group (none, if
+ * groups end with their tiles); where they are short, one a group */
+static inline long row_tiles_about(int rows, int groups, int height) {
+    const long some = groups < rows ? groups : rows, filled = (rows + height - 1L) / height + (some - 1) / 2;
+    return filled > some ? filled : some;
 }
 
 #endif

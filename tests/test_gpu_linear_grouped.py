@@ -123,3 +123,40 @@ def test_random_values_are_as_near_as_f32_sums_are(dev, out):
     if out == "bf16":
         bound = bound + 2.0 ** -8 * (np.abs(want) + bound)
     assert (np.abs(got - want) <= bound).all()
+
+
+def plan_of(groups, rows, k, n, size):
+    import ctypes as C
+
+    import iris_c_amd
+    plan = (C.c_int * 3)()
+    iris_c_amd.load().iris_hip_linear_grouped_plan(groups, rows, k, n, size, plan)
+    return tuple(plan)
+
+
+# rows of each group, k, n, and the kernel that the layer takes (3 tiles of 256 rows, 2 the smaller tiles, 1 a few rows, 0 any size)
+ROUTES = [([1, 0, 2, 1], 1024, 512, 1), ([3] * 40, 512, 768, 1), ([16, 16], 2560, 6144, 1), ([130, 200], 2560, 1536, 2), ([60] * 24, 1024, 1024, 2),
+          ([90, 38], 4096, 2560, 2), ([600, 2500], 512, 8192, 3), ([1000, 0, 3000], 512, 6144, 3), ([900, 1200], 1000, 1600, 0)]
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("sizes,k,n,kernel", ROUTES)
+def test_every_route(dev, sizes, k, n, kernel, out):
+    first = np.concatenate([[2], 2 + np.cumsum(sizes)])
+    rows = int(first[-1]) + 5
+    assert plan_of(len(sizes), rows, k, n, 4 if out == "f32" else 2)[0] == kernel
+    rng = np.random.default_rng(rows)
+    x, w = whole(rng, rows, k), whole(rng, len(sizes), n, k)
+    check(run(dev, x, w, first, rows, k, n, out), reference(x, w, first, rows, n), out)
+
+
+def test_ranges_of_k_leave_rows_in_no_group_alone(dev):
+    """A product whose ranges of K are added by a second kernel, which has to find the rows that are in a group"""
+    sizes, k, n = [40, 0, 70], 16384, 512
+    first = np.concatenate([[7], 7 + np.cumsum(sizes)])
+    rows = int(first[-1]) + 20
+    assert plan_of(len(sizes), rows, k, n, 2)[0] == 2 and plan_of(len(sizes), rows, k, n, 2)[2] > 1
+    rng = np.random.default_rng(3)
+    x, w = whole(rng, rows, k), whole(rng, len(sizes), n, k)
+    for out in ("f32", "bf16"):
+        check(run(dev, x, w, first, rows, k, n, out), reference(x, w, first, rows, n), out)
