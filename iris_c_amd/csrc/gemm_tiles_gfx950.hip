@@ -109,7 +109,8 @@ k_gemm_tiles(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t
         W += (size_t)rows.group * N * K;
     }
     const int m0 = rows.m0, m_end = rows.end;
-    const int nk_all = K / TK, kt0 = (int)((long)nk_all * split / splits), nk = (int)((long)nk_all * (split + 1) / splits) - kt0;
+    /* 32 bits hold the products: K < 2^24 (N >= 128, 32-bit byte offsets into W), at most 512 ranges */
+    const int nk_all = K / TK, kt0 = nk_all * split / splits, nk = nk_all * (split + 1) / splits - kt0;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4;
