@@ -221,3 +221,57 @@ def test_grouped_layer(dev, name, k, n, out):
     for g in range(groups):
         want[first[g]:first[g + 1]] = x[first[g]:first[g + 1]] @ w[g].T
     check_exact(got, want, out)
+
+
+# ----------------------------------------------------------------------------------------------------------------- routes
+def plan_of(groups, rows, k, n, out):
+    import iris_c_amd
+    return iris_c_amd.load().iris_hip_linear_mxfp4_plan(groups, rows, k, n, 4 if out == "f32" else 2)
+
+
+# rows of each group (one: no groups), k, n, and the kernel: -1, -2 a few rows, 0 - 3 the smaller tiles, 4 and 5 those of 256 rows
+ROUTES = [([2], 2560, 640, -1), ([10], 512, 16384, -2), ([100], 2560, 2560, 0), ([300], 2560, 2560, 1), ([500], 2560, 2560, 2), ([1000], 2560, 2560, 3),
+          ([500], 512, 16384, 4), ([3000], 768, 5120, 5), ([1, 3, 0, 2], 1024, 512, -1), ([3] * 40, 512, 768, -2), ([60, 32], 4096, 2560, 0),
+          ([150, 142], 4096, 2560, 1), ([400, 92], 4096, 2560, 2), ([200] * 9 + [192], 1024, 1024, 3), ([512, 0, 480], 768, 5120, 4), ([300, 2692], 768, 5120, 5),
+          ([300], 1100, 1400, 0), ([700], 1100, 1400, 1), ([1000], 1100, 1400, 2), ([1500], 1100, 1400, 3), ([50] * 9 + [42], 1100, 1000, 0),
+          ([100] * 6 + [92, 0, 0, 0], 1100, 1000, 1), ([100] * 9 + [92], 1100, 1000, 2), ([200] * 9 + [192], 1100, 1000, 3)]
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("sizes,k,n,route", ROUTES)
+def test_every_route(dev, sizes, k, n, route, out):
+    grouped = len(sizes) > 1
+    first = np.concatenate([[3], 3 + np.cumsum(sizes)]) if grouped else np.array([0, sizes[0]])
+    rows = int(first[-1]) + (5 if grouped else 0)
+    assert plan_of(len(sizes), rows, k, n, out) == route
+    rng = np.random.default_rng(rows + k)
+    cx, sx = exact_inputs(rng, rows, k)
+    cw, sw = exact_inputs(rng, len(sizes) * n, k)
+    got = run_layer(dev, cx, sx, cw, sw, rows, k, n, out, first if grouped else None)
+    x, w = mx.decode(cx, sx, k), mx.decode(cw, sw, k).reshape(len(sizes), n, k)
+    want = np.full((rows, n), 7.0)
+    for g in range(len(sizes)):
+        want[first[g]:first[g + 1]] = x[first[g]:first[g + 1]] @ w[g].T
+    check_exact(got, want, out)
+
+
+@pytest.mark.parametrize("rows,k,n", [(3, 1024, 64), (70, 1024, 512), (300, 768, 512)])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_scales_and_results_that_start_anywhere(dev, rows, k, n, off):
+    """Scales are bytes, and y needs no more than its own type's alignment"""
+    rng = np.random.default_rng(off)
+    cx, sx = exact_inputs(rng, rows, k)
+    cw, sw = exact_inputs(rng, n, k)
+
+    def shifted(a):
+        d = dev.alloc(a.nbytes + 16)
+        dev.lib.iris_dev_upload(ptr_add(d, off), a.ctypes.data, a.nbytes)
+        return ptr_add(d, off)
+
+    y = dev.put(np.full(rows * n + 8, 7.0, np.float32))
+    dev.lib.iris_dev_linear_mxfp4_f32(ptr_add(y, 4 * off), dev.put(cx), shifted(sx), dev.put(cw), shifted(sw), rows, k, n)
+    dev.check()
+    got = dev.get(y, (rows * n + 8,), np.float32)
+    dev.free_all()
+    assert (got[:off] == 7).all() and (got[off + rows * n:] == 7).all()
+    check_exact(got[off:off + rows * n].reshape(rows, n), mx.decode(cx, sx, k) @ mx.decode(cw, sw, k).T, "f32")
