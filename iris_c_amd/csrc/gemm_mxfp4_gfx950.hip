@@ -201,7 +201,7 @@ __device__ __forceinline__ int swizzle(int r) {
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"                          /* M0 in a clobber list */
-template <typename OUT, int NA, bool GROUPED>
+template <typename OUT, int NA, bool STREAM, bool GROUPED>
 __global__ void __launch_bounds__(512, 2)
 k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *__restrict__ xs, const uint8_t *__restrict__ W,
              const uint8_t *__restrict__ Ws, int M, int N, int nb, const int *__restrict__ first_row, int groups) {
@@ -375,7 +375,11 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
             for (int it = 0; it < 16; it++) {
                 const int row = 2 * it + (lane >> 5), c = lane & 31, m = mw + 32 * half + row, n = nw + PER16 * c;
                 const f32x4 v = *reinterpret_cast<const f32x4 *>(&buf[row * 128 + 4 * ((c & 16) | ((c ^ row) & 15))]);
-                if (c < 4 * NA && m < m_end && n < N) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(y) + (size_t)m * N + n) = v;
+                if (c < 4 * NA && m < m_end && n < N) {
+                    f32x4 *to = reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(y) + (size_t)m * N + n);
+                    if constexpr (STREAM) __builtin_nontemporal_store(v, to);
+                    else *to = v;
+                }
             }
         }
     } else {
@@ -392,7 +396,11 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
         for (int it = 0; it < 16; it++) {
             const int row = 4 * it + (lane >> 4), c = lane & 15, m = mw + row, n = nw + PER16 * c;
             const i32x4 v = *reinterpret_cast<const i32x4 *>(&buf[row * 128 + 8 * (c ^ (row & 15))]);
-            if (c < 2 * NA && m < m_end && n < N) *reinterpret_cast<i32x4 *>(reinterpret_cast<uint16_t *>(y) + (size_t)m * N + n) = v;
+            if (c < 2 * NA && m < m_end && n < N) {
+                i32x4 *to = reinterpret_cast<i32x4 *>(reinterpret_cast<uint16_t *>(y) + (size_t)m * N + n);
+                if constexpr (STREAM) __builtin_nontemporal_store(v, to);
+                else *to = v;
+            }
         }
     }
 }
@@ -649,18 +657,26 @@ long tiles_at_most(int M, int N, int groups, int tm, int tn) {
     return (GROUPED ? row_tiles_at_most(M, groups, tm) : ((long)M + tm - 1) / tm) * ((N + tn - 1L) / tn);
 }
 
-template <typename OUT, int NA, bool GROUPED>
+/* An output of 100 MB or more is stored with the streaming hint, past the Infinity Cache (256 MB), which then keeps the operands. us, plain / streaming:
+ * 4608 x 4096 -> 36864 (340 MB) 360 / 341, with its conversion to MXFP4 behind it 427 / 419; -> 12288 (113 MB) 147 / 122 and 171.5 / 170.7; smaller
+ * ones lose by what reads them next: -> 10240 (94 MB) 121.8 / 122.6 with the conversion, -> 8192 107.7 / 110.7. Kernels of their own: of a test in front
+ * of two stores to one place the compiler keeps one, the plain one. */
+constexpr size_t STREAM_BYTES = (size_t)100 << 20;
+
+template <typename OUT, int NA, bool GROUPED, bool STREAM = false>
 int launch_wide(hipStream_t st, KERNEL_PARAMS) {
+    if constexpr (!STREAM)
+        if ((size_t)M * N * sizeof(OUT) >= STREAM_BYTES) return launch_wide<OUT, NA, GROUPED, true>(st, KERNEL_ARGS);
     using T = Wide<NA>;
     static bool configured = false;
     if (!configured) {
-        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k_mxfp4_wide<OUT, NA, GROUPED>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k_mxfp4_wide<OUT, NA, STREAM, GROUPED>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
         if (e != hipSuccess) return (int)e;
         configured = true;
     }
     const long most = tiles_at_most<GROUPED>(M, N, groups, T::TM, T::TN);
     if (most >> 30) return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_mxfp4_wide<OUT, NA, GROUPED>), dim3((unsigned)(most + 7) / 8 * 8), dim3(512), T::LDS, st, KERNEL_ARGS);
+    hipLaunchKernelGGL((k_mxfp4_wide<OUT, NA, STREAM, GROUPED>), dim3((unsigned)(most + 7) / 8 * 8), dim3(512), T::LDS, st, KERNEL_ARGS);
     return (int)hipGetLastError();
 }
 

@@ -275,3 +275,16 @@ def test_scales_and_results_that_start_anywhere(dev, rows, k, n, off):
     dev.free_all()
     assert (got[:off] == 7).all() and (got[off + rows * n:] == 7).all()
     check_exact(got[off:off + rows * n].reshape(rows, n), mx.decode(cx, sx, k) @ mx.decode(cw, sw, k).T, "f32")
+
+
+def test_results_too_large_for_the_cache_to_keep(dev):
+    """Outputs of 100 MB and more leave past the Infinity Cache, from kernels of their own; rows here and there are compared"""
+    for rows, n, out in ((4352, 12288, "bf16"), (2300, 12320, "f32")):
+        assert rows * n * (2 if out == "bf16" else 4) >= 100 << 20 and plan_of(1, rows, 512, n, out) >= 4
+        rng = np.random.default_rng(rows)
+        cx, sx = exact_inputs(rng, rows, 512)
+        cw, sw = exact_inputs(rng, n, 512)
+        got = run_layer(dev, cx, sx, cw, sw, rows, 512, n, out)
+        some = np.unique(np.concatenate([rng.integers(0, rows, 24), [0, 255, 256, rows - 1]]))
+        check_exact(got[some], mx.decode(cx[some], sx[some], 512) @ mx.decode(cw, sw, 512).T, out)
+        assert (got != 7.0).any(1).all()
