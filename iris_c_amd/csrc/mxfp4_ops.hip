@@ -35,10 +35,22 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(p, bf16x2));
 }
 
-/* 8 values, as the bits of floats; left: how many of them the row has (at least 1 here, zeros behind) */
+template <bool STREAM, typename V>
+__device__ __forceinline__ u32x4 load16(const V *p) {
+    if constexpr (STREAM) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+template <bool STREAM, typename V>
+__device__ __forceinline__ void store16(V *p, u32x4 v) {
+    if constexpr (STREAM) __builtin_nontemporal_store(v, p);
+    else *p = v;
+}
+
+/* 8 values, as the bits of floats; left: how many of them the row has (at least 1 here, zeros behind). STREAM: with the streaming hint. */
+template <bool STREAM>
 __device__ __forceinline__ void load8(const uint16_t *p, int left, uint32_t (&v)[8]) {
     if (left >= 8) {
-        const u32x4 r = *reinterpret_cast<const u32x4_at2 *>(p);
+        const u32x4 r = load16<STREAM>(reinterpret_cast<const u32x4_at2 *>(p));
 #pragma unroll
         for (int i = 0; i < 4; i++) { v[2 * i] = r[i] << 16; v[2 * i + 1] = r[i] & 0xffff0000u; }
     } else {
@@ -46,9 +58,11 @@ __device__ __forceinline__ void load8(const uint16_t *p, int left, uint32_t (&v)
         for (int i = 0; i < 8; i++) v[i] = i < left ? (uint32_t)p[i] << 16 : 0u;
     }
 }
+template <bool STREAM>
 __device__ __forceinline__ void load8(const float *p, int left, uint32_t (&v)[8]) {
     if (left >= 8) {
-        const u32x4 a = reinterpret_cast<const u32x4_at4 *>(p)[0], b = reinterpret_cast<const u32x4_at4 *>(p)[1];
+        const u32x4_at4 *q = reinterpret_cast<const u32x4_at4 *>(p);
+        const u32x4 a = load16<STREAM>(q), b = load16<STREAM>(q + 1);
 #pragma unroll
         for (int i = 0; i < 4; i++) { v[i] = a[i]; v[4 + i] = b[i]; }
     } else {
@@ -56,22 +70,24 @@ __device__ __forceinline__ void load8(const float *p, int left, uint32_t (&v)[8]
         for (int i = 0; i < 8; i++) v[i] = i < left ? __float_as_uint(p[i]) : 0u;
     }
 }
+template <bool STREAM>
 __device__ __forceinline__ void store8(uint16_t *p, int left, const float (&v)[8]) {
     const u32x4 r = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
     if (left >= 8) {
-        *reinterpret_cast<u32x4_at2 *>(p) = r;
+        store16<STREAM>(reinterpret_cast<u32x4_at2 *>(p), r);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++)
             if (i < left) p[i] = (uint16_t)(r[i / 2] >> (16 * (i & 1)));
     }
 }
+template <bool STREAM>
 __device__ __forceinline__ void store8(float *p, int left, const float (&v)[8]) {
     if (left >= 8) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const u32x4 r = {__float_as_uint(v[4 * h]), __float_as_uint(v[4 * h + 1]), __float_as_uint(v[4 * h + 2]), __float_as_uint(v[4 * h + 3])};
-            reinterpret_cast<u32x4_at4 *>(p)[h] = r;
+            store16<STREAM>(reinterpret_cast<u32x4_at4 *>(p) + h, r);
         }
     } else {
 #pragma unroll
@@ -93,7 +109,7 @@ __device__ __forceinline__ void place(size_t i, size_t groups, uint32_t per_row,
     else { const uint32_t q = (uint32_t)i / per_row; s = q; c = (uint32_t)i - q * per_row; }
 }
 
-template <typename T>
+template <typename T, bool STREAM>
 __global__ void __launch_bounds__(THREADS)
 k_to_mxfp4(uint32_t *__restrict__ codes, uint8_t *__restrict__ scales, const T *__restrict__ src, int ld, int cols, uint32_t per_row, size_t groups) {
     const size_t first = (size_t)blockIdx.x * (THREADS * UNROLL) + threadIdx.x;
@@ -105,7 +121,7 @@ k_to_mxfp4(uint32_t *__restrict__ codes, uint8_t *__restrict__ scales, const T *
         uint32_t c;
         place(i, groups, per_row, s, c);
         const int left = i < groups ? cols - 8 * (int)c : 0;
-        if (left > 0) load8(src + s * ld + 8 * c, left, v[u]);
+        if (left > 0) load8<STREAM>(src + s * ld + 8 * c, left, v[u]);
         else
 #pragma unroll
             for (int k = 0; k < 8; k++) v[u][k] = 0u;
@@ -131,7 +147,7 @@ k_to_mxfp4(uint32_t *__restrict__ codes, uint8_t *__restrict__ scales, const T *
     }
 }
 
-template <typename T>
+template <typename T, bool STREAM>
 __global__ void __launch_bounds__(THREADS)
 k_mxfp4_to(T *__restrict__ dst, int ld, const uint32_t *__restrict__ codes, const uint8_t *__restrict__ scales, int cols, uint32_t per_row, size_t groups) {
     const size_t first = (size_t)blockIdx.x * (THREADS * UNROLL) + threadIdx.x;
@@ -158,28 +174,43 @@ k_mxfp4_to(T *__restrict__ dst, int ld, const uint32_t *__restrict__ codes, cons
 #pragma unroll
         for (int k = 0; k < 8; k++)
             v[k] = scale[u] == 255 ? __uint_as_float(0x7fc00000u) : __builtin_amdgcn_ldexpf(p[k / 2][k & 1], scale[u] - 127);
-        store8(dst + s * ld + 8 * c, left, v);
+        store8<STREAM>(dst + s * ld + 8 * c, left, v);
     }
+}
+
+/* Values of 64 MB and more are read, of 100 MB and more written, with the streaming hint, past the Infinity Cache (256 MB): they do not all stay there, and the
+ * codes, which are read next, do. There and back, us, plain / streaming: 4608 x 16384 bf16 74.1 / 61.8 (6.2 TB/s with the codes),
+ * 4608 x 8192 40.3 / 34.6, f32 there and bf16 back 48.9 / 48.7; with both hints 4608 x 4096 18.8 / 19.7. */
+constexpr size_t STREAM_READ = (size_t)64 << 20, STREAM_WRITE = (size_t)100 << 20;
+
+template <typename T, bool STREAM>
+int launch_to(void *stream, uint8_t *codes, uint8_t *scales, const T *src, int ld, int rows, int cols) {
+    const uint32_t per_row = 4u * (((uint32_t)cols + 31) / 32);
+    const size_t groups = (size_t)rows * per_row, blocks = (groups + THREADS * UNROLL - 1) / (THREADS * UNROLL);
+    if (blocks >> 31) return (int)hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_to_mxfp4<T, STREAM>), dim3((unsigned)blocks), dim3(THREADS), 0, (hipStream_t)stream, reinterpret_cast<uint32_t *>(codes), scales, src, ld,
+                       cols, per_row, groups);
+    return (int)hipGetLastError();
+}
+template <typename T, bool STREAM>
+int launch_from(void *stream, T *dst, int ld, const uint8_t *codes, const uint8_t *scales, int rows, int cols) {
+    const uint32_t per_row = 4u * (((uint32_t)cols + 31) / 32);
+    const size_t groups = (size_t)rows * per_row, blocks = (groups + THREADS * UNROLL - 1) / (THREADS * UNROLL);
+    if (blocks >> 31) return (int)hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_mxfp4_to<T, STREAM>), dim3((unsigned)blocks), dim3(THREADS), 0, (hipStream_t)stream, dst, ld, reinterpret_cast<const uint32_t *>(codes), scales,
+                       cols, per_row, groups);
+    return (int)hipGetLastError();
 }
 
 template <typename T>
 int to_mxfp4(void *stream, uint8_t *codes, uint8_t *scales, const T *src, int ld, int rows, int cols) {
-    const uint32_t per_row = 4u * (((uint32_t)cols + 31) / 32);
-    const size_t groups = (size_t)rows * per_row, blocks = (groups + THREADS * UNROLL - 1) / (THREADS * UNROLL);
-    if (blocks >> 31) return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_to_mxfp4<T>), dim3((unsigned)blocks), dim3(THREADS), 0, (hipStream_t)stream, reinterpret_cast<uint32_t *>(codes), scales, src, ld, cols,
-                       per_row, groups);
-    return (int)hipGetLastError();
+    return (size_t)rows * cols * sizeof(T) >= STREAM_READ ? launch_to<T, true>(stream, codes, scales, src, ld, rows, cols)
+                                                          : launch_to<T, false>(stream, codes, scales, src, ld, rows, cols);
 }
-
 template <typename T>
 int mxfp4_to(void *stream, T *dst, int ld, const uint8_t *codes, const uint8_t *scales, int rows, int cols) {
-    const uint32_t per_row = 4u * (((uint32_t)cols + 31) / 32);
-    const size_t groups = (size_t)rows * per_row, blocks = (groups + THREADS * UNROLL - 1) / (THREADS * UNROLL);
-    if (blocks >> 31) return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_mxfp4_to<T>), dim3((unsigned)blocks), dim3(THREADS), 0, (hipStream_t)stream, dst, ld, reinterpret_cast<const uint32_t *>(codes), scales,
-                       cols, per_row, groups);
-    return (int)hipGetLastError();
+    return (size_t)rows * cols * sizeof(T) >= STREAM_WRITE ? launch_from<T, true>(stream, dst, ld, codes, scales, rows, cols)
+                                                           : launch_from<T, false>(stream, dst, ld, codes, scales, rows, cols);
 }
 
 }  // namespace

@@ -112,6 +112,32 @@ def test_back_from_mxfp4(dev, kind, rows, cols, ld):
     dev.free_all()
 
 
+@pytest.mark.parametrize("kind,rows,cols", [("bf16", 4100, 13001), ("f32", 4100, 6501)])
+def test_conversions_of_more_than_the_cache_keeps(dev, kind, rows, cols):
+    """100 MB and more of values go past the Infinity Cache both ways, in kernels of their own; odd rows that start anywhere"""
+    rng = np.random.default_rng(cols)
+    host = rng.integers(0, 1 << 16, (rows, cols), dtype=np.uint16)
+    host[(host & 0x7f80) == 0x7f80] = 0x3f80
+    if kind == "f32":
+        host = mx.bf16_value(host)
+    size = host.nbytes
+    assert size >= 100 << 20
+    d, nb = dev.put(host), mx.blocks(cols)
+    dc, ds, back = dev.alloc(rows * nb * 16), dev.alloc(rows * nb), dev.alloc(size)
+    getattr(dev.lib, f"iris_dev_{kind}_to_mxfp4")(dc, ds, d, cols, rows, cols)
+    getattr(dev.lib, f"iris_dev_mxfp4_to_{kind}")(back, cols, dc, ds, rows, cols)
+    dev.check()
+    got = dev.get(back, host.shape, host.dtype)
+    codes, scales = dev.get(dc, (rows, nb * 16), np.uint8), dev.get(ds, (rows, nb), np.uint8)
+    dev.free_all()
+    some = np.unique(np.concatenate([rng.integers(0, rows, 40), [0, 1, rows - 1]]))
+    value = host[some] if kind == "f32" else mx.bf16_value(host[some])
+    want_codes, want_scales = mx.encode(value)
+    assert np.array_equal(codes[some], want_codes) and np.array_equal(scales[some], want_scales)
+    want = mx.decode(want_codes, want_scales, cols).astype(np.float32)
+    assert np.array_equal(got[some] if kind == "f32" else mx.bf16_value(got[some]), want)
+
+
 # ----------------------------------------------------------------------------------------------------------------- layers
 def run_layer(dev, codes_x, scales_x, codes_w, scales_w, rows, k, n, out, first=None, fill=7.0):
     """y as float32, and the kernel's name"""
