@@ -727,7 +727,8 @@ int plan_mxfp4(int groups, int M, int N, int nb, bool tail, bool wide_stores) {
     if (best < 2.2f + fresh) best = 2.2f + fresh;
     /* two blocks of columns: 40 rows over 64 weight matrices of 2560 -> 1536 13.9 us with one, 12.7 with two; 1 row, 4096 -> 4096 3.7 / 4.9 */
     int plan = row_tiles(16) * ((N + 31L) / 32) >= 512 ? -2 : -1;
-    for (int i = 0; i < (tail || M < 256 || N < 192 || !wide_stores ? FIRST_WIDE : NSHAPES); i++) {
+    /* the tiles' offsets inside a tile of rows have 32 bits */
+    for (int i = 0; i < (nb >> 20 ? 0 : tail || M < 256 || N < 192 || !wide_stores ? FIRST_WIDE : NSHAPES); i++) {
         const Shape &s = SHAPES[i];
         const long wgs = row_tiles(s.tm) * ((N + s.tn - 1L) / s.tn), each = (wgs + 255) / 256, rounds = (wgs + 256L * s.resident - 1) / (256L * s.resident);
         const float shared = s.share * (float)each, step = shared > s.step ? shared : s.step;
@@ -751,7 +752,7 @@ int launch_shape(int shape, hipStream_t st, KERNEL_PARAMS) {
 
 template <typename OUT, bool GROUPED>
 int linear(hipStream_t st, KERNEL_PARAMS) {
-    const bool tail = nb % 8 != 0 || nb < 16 || (((uintptr_t)xs | (uintptr_t)Ws) & 3) != 0;
+    const bool tail = nb % 8 != 0 || nb < 16 || (((uintptr_t)xs | (uintptr_t)Ws) & 7) != 0;
     const bool wide_stores = N % (16 / (int)sizeof(OUT)) == 0 && ((uintptr_t)y & 15) == 0;
     const int plan = plan_mxfp4(GROUPED ? groups : 1, M, N, nb, tail, wide_stores);
     if (plan == -1) return launch_rows<OUT, 1, GROUPED>(st, KERNEL_ARGS);

@@ -208,7 +208,7 @@ def test_codes_in_every_place_meet_their_counterpart(dev):
     assert np.array_equal(got, mx.decode(cw, sw, k).T.astype(np.float32))
 
 
-@pytest.mark.parametrize("rows,k,n", [(4, 512, 64), (300, 1024, 512), (40, 1000, 100)])
+@pytest.mark.parametrize("rows,k,n", [(4, 512, 64), (300, 1024, 512), (40, 1000, 100), (300, 1100, 1400), (500, 512, 16384)])
 def test_nan_blocks_reach_their_rows_and_columns_alone(dev, rows, k, n):
     rng = np.random.default_rng(5)
     cx, sx = exact_inputs(rng, rows, k)
@@ -281,8 +281,8 @@ def test_every_route(dev, sizes, k, n, route, out):
     check_exact(got, want, out)
 
 
-@pytest.mark.parametrize("rows,k,n", [(3, 1024, 64), (70, 1024, 512), (300, 768, 512)])
-@pytest.mark.parametrize("off", [1, 2, 3])
+@pytest.mark.parametrize("rows,k,n", [(3, 1024, 64), (70, 1024, 512), (300, 768, 512), (500, 512, 16384)])
+@pytest.mark.parametrize("off", [1, 2, 3, 4, 8])
 def test_scales_and_results_that_start_anywhere(dev, rows, k, n, off):
     """Scales are bytes, and y needs no more than its own type's alignment"""
     rng = np.random.default_rng(off)
@@ -294,10 +294,10 @@ def test_scales_and_results_that_start_anywhere(dev, rows, k, n, off):
         dev.lib.iris_dev_upload(ptr_add(d, off), a.ctypes.data, a.nbytes)
         return ptr_add(d, off)
 
-    y = dev.put(np.full(rows * n + 8, 7.0, np.float32))
+    y = dev.put(np.full(rows * n + 16, 7.0, np.float32))
     dev.lib.iris_dev_linear_mxfp4_f32(ptr_add(y, 4 * off), dev.put(cx), shifted(sx), dev.put(cw), shifted(sw), rows, k, n)
     dev.check()
-    got = dev.get(y, (rows * n + 8,), np.float32)
+    got = dev.get(y, (rows * n + 16,), np.float32)
     dev.free_all()
     assert (got[:off] == 7).all() and (got[off + rows * n:] == 7).all()
     check_exact(got[off:off + rows * n].reshape(rows, n), mx.decode(cx, sx, k) @ mx.decode(cw, sw, k).T, "f32")
