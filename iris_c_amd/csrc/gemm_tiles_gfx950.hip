@@ -78,10 +78,11 @@ struct Tile {
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"                          /* M0 in a clobber list */
+/* the body of k_gemm_tiles and, GROUPED, of k_grouped_tiles below */
 template <typename OUT, int NB, int WM, int NA, int WN, int KG, int STAGES, bool THROUGH, bool GROUPED>
-__global__ void __launch_bounds__(64 * WM * WN * KG, WM * WN * KG / 4)
-k_gemm_tiles(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t *__restrict__ W, int M, int N, int K,
-             const float *__restrict__ bias, int tiles_m, int tiles_n, int splits, int total, int per_xcd, int turns, RowGroupsArg grouped) {
+__device__ __forceinline__ void
+gemm_tiles(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t *__restrict__ W, int M, int N, int K,
+           const float *__restrict__ bias, int tiles_m, int tiles_n, int splits, int total, int per_xcd, int turns, RowGroupsArg grouped) {
     using T = Tile<NB, WM, NA, WN, KG, STAGES>;
     constexpr int TM = T::TM, TN = T::TN, STAGE = T::STAGE, PIECES = T::PIECES;
     static_assert(T::LDS <= 160 * 1024 && NA <= 8 && (KG == 1 || (KG == 2 && NB % 2 == 0)), "");
@@ -298,6 +299,21 @@ k_gemm_tiles(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t
 }
 #pragma clang diagnostic pop
 
+template <typename OUT, int NB, int WM, int NA, int WN, int KG, int STAGES, bool THROUGH>
+__global__ void __launch_bounds__(64 * WM * WN * KG, WM * WN * KG / 4)
+k_gemm_tiles(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t *__restrict__ W, int M, int N, int K,
+             const float *__restrict__ bias, int tiles_m, int tiles_n, int splits, int total, int per_xcd, int turns) {
+    gemm_tiles<OUT, NB, WM, NA, WN, KG, STAGES, THROUGH, false>(y, x, W, M, N, K, bias, tiles_m, tiles_n, splits, total, per_xcd, turns, RowGroupsArg{});
+}
+
+/* rows in groups (row_groups.h), W [groups, N, K]; tiles_m and what follows from it are found on the device */
+template <typename OUT, int NB, int WM, int NA, int WN, int KG, int STAGES, bool THROUGH>
+__global__ void __launch_bounds__(64 * WM * WN * KG, WM * WN * KG / 4)
+k_grouped_tiles(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t *__restrict__ W, int M, int N, int K, int tiles_n, int splits, int turns,
+                RowGroupsArg grouped) {
+    gemm_tiles<OUT, NB, WM, NA, WN, KG, STAGES, THROUGH, true>(y, x, W, M, N, K, nullptr, 0, tiles_n, splits, 0, 0, turns, grouped);
+}
+
 /* y[i] = part[0][i] + part[1][i] + ..., four values a thread (n a multiple of 8). AT_ONCE (at most `splits`) sums are requested
  * before the first is used: what bounds it is the launch and one trip to memory, and one range after the other was a trip each. With
  * the layer in front of it, us, eight values a thread and one after the other / now: 512 x 9728 -> 2560 (6 ranges) 36.5 / 36.0,
@@ -347,17 +363,23 @@ int launch_tiles(hipStream_t st, OUT *y, const uint16_t *x, const uint16_t *W, i
     if constexpr (sizeof(OUT) == 4 && !THROUGH)
         if (through) return launch_tiles<OUT, GROUPED, NB, WM, NA, WN, KG, STAGES, true>(st, y, x, W, M, N, K, bias, splits, true, grouped);
     using T = Tile<NB, WM, NA, WN, KG, STAGES>;
+    const void *kernel;
+    if constexpr (GROUPED) kernel = reinterpret_cast<const void *>(k_grouped_tiles<OUT, NB, WM, NA, WN, KG, STAGES, THROUGH>);
+    else kernel = reinterpret_cast<const void *>(k_gemm_tiles<OUT, NB, WM, NA, WN, KG, STAGES, THROUGH>);
     static bool configured = false;
     if (!configured) {
-        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k_gemm_tiles<OUT, NB, WM, NA, WN, KG, STAGES, THROUGH, GROUPED>),
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+        hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
         if (e != hipSuccess) return (int)e;
         configured = true;
     }
     const int tiles_m = GROUPED ? (int)row_tiles_at_most(M, grouped.groups, T::TM) : (M + T::TM - 1) / T::TM, tiles_n = (N + T::TN - 1) / T::TN,
               total = tiles_m * tiles_n * splits, per_xcd = (total + 7) / 8;
-    hipLaunchKernelGGL((k_gemm_tiles<OUT, NB, WM, NA, WN, KG, STAGES, THROUGH, GROUPED>), dim3((unsigned)per_xcd * 8), dim3(T::THREADS), T::LDS, st, y, x, W, M, N, K,
-                       bias, tiles_m, tiles_n, splits, total, per_xcd, turns(M, N, K, total), grouped);
+    if constexpr (GROUPED)
+        hipLaunchKernelGGL((k_grouped_tiles<OUT, NB, WM, NA, WN, KG, STAGES, THROUGH>), dim3((unsigned)per_xcd * 8), dim3(T::THREADS), T::LDS, st, y, x, W, M, N, K, tiles_n,
+                           splits, turns(M, N, K, total), grouped);
+    else
+        hipLaunchKernelGGL((k_gemm_tiles<OUT, NB, WM, NA, WN, KG, STAGES, THROUGH>), dim3((unsigned)per_xcd * 8), dim3(T::THREADS), T::LDS, st, y, x, W, M, N, K,
+                           bias, tiles_m, tiles_n, splits, total, per_xcd, turns(M, N, K, total));
     return (int)hipGetLastError();
 }
 
