@@ -180,7 +180,8 @@ k_mxfp4_rows(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
  * A k tile is four steps: k-step 0 with the first and the second half of the columns, then k-step 1; the operands of a step are read
  * during the step before, the scales of the next tile in steps 0 and 2. Codes of k tile t + 2: the first half of W in steps 0 and 2 of
  * tile t, the rest in step 3, behind the one barrier of a tile, which frees the stage. Every memory instruction stands in a gap between two
- * products. Requests past the end of K ask for the last tile again, into a stage that nobody reads. */
+ * products. Requests past the end of K are issued all the same (a branch around each costs more, and the waits count them), but all lanes ask for
+ * one 16 B of the last tile, into a stage that nobody reads. */
 template <int NA>
 struct Wide {
     static constexpr int TM = 256, TN = 32 * NA, WP = (2 * NA + 7) / 8;                  /* WP: 8-row pieces of half of W per wave */
@@ -252,7 +253,9 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
     const uint8_t *x_tile = x + (size_t)m0 * nb * 16, *w_tile = W + (size_t)n0 * nb * 16;
     const uint8_t *s_tile = 64 * wave < TM ? xs + (size_t)m0 * nb : Ws + (size_t)n0 * nb;
     const uint32_t lds0 = lds_address(lds);
+    uint32_t lanes = ~0u;                                      /* 0 in the last two tiles, see above */
     auto load_lds = [&](uint32_t to, const uint8_t *from, uint32_t off) {
+        off &= lanes;
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds0 + to), "v"(off), "s"(from) : "memory", "m0");
     };
     auto request_x = [&](int j, int kt, int stage) { load_lds(stage * T::XS + (4 * wave + j) * 1024, x_tile + (size_t)min(kt, nk - 1) * 128, xoff[j]); };
@@ -318,6 +321,7 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
     auto tile = [&](auto odd, int t) {
         constexpr int ODD = decltype(odd)::value, S1 = (NA + 4 + 1) / 2;                 /* scales read in step 0 */
         const int mine = next(w_slot, wn), far = next(w_slot, 4), after = next(w_slot, 2 + wn);
+        lanes = t + 2 < nk ? ~0u : 0u;
         const int t1 = min(t + 1, nk - 1), s_at = ((t1 >> 1) & 1) * T::SC + 8 * (t1 - min(t1 & ~1, nk - 2));
         products(k0, ODD, 0, H0, [&](int g) {
             if (g < H1) read_a(0, H0 + g, mine);
@@ -476,17 +480,18 @@ k_mxfp4_tiles(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t 
         soff[j] = row_off(16 * spiece[j] + (lane >> 2));
     }
     const uint32_t lds0 = lds_address(lds);
-    auto request = [&](int i, int kt, int stage) {             /* piece i of this wave */
+    auto request = [&](int i, int kt, int stage) {             /* piece i of this wave; past the end of K all lanes ask for one 16 B of the last tile */
+        const uint32_t off = kt < nk ? coff[i] : 0u;
         if constexpr (TAIL) {
             kt = min(kt, nk - 1);
-            const uint8_t *from = (cpiece[i] < TM / 8 ? x_tile : w_tile) + coff[i] + (size_t)kt * 128;
+            const uint8_t *from = (cpiece[i] < TM / 8 ? x_tile : w_tile) + off + (size_t)kt * 128;
             const int r = 8 * cpiece[i] + (lane >> 3);
             if (8 * kt + ((lane & 7) ^ ((r >> 1) & 7)) >= nb) from = reinterpret_cast<const uint8_t *>(zero_line);
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds0 + stage * T::STAGE + cpiece[i] * 1024), "v"(from) : "memory", "m0");
             return;
         }
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                     ::"s"(lds0 + stage * T::STAGE + cpiece[i] * 1024), "v"(coff[i]), "s"((cpiece[i] < TM / 8 ? x_tile : w_tile) + (size_t)min(kt, nk - 1) * 128)
+                     ::"s"(lds0 + stage * T::STAGE + cpiece[i] * 1024), "v"(off), "s"((cpiece[i] < TM / 8 ? x_tile : w_tile) + (size_t)min(kt, nk - 1) * 128)
                      : "memory", "m0");
     };
     /* scales of k tiles 8 c .. 8 c + 7: part p is tiles 8 c + 2 p and the next, or the last two (there are two) */
@@ -582,7 +587,7 @@ k_mxfp4_tiles(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t 
          * are newer, and scales for much later ones. Those of eight tiles on are requested in the first of eight, when the stage's last readers
          * have passed the barrier. */
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * CP) : "memory");
-        if ((t & 7) == 0) request_scales((t >> 3) + 1);
+        if ((t & 7) == 0 && t + 8 < nk) request_scales((t >> 3) + 1);
         constexpr int LAST = NSTEP - 1, SET = NSTEP == 1 ? ODD : LAST & 1, ALL = 2 * OPS + CP;
         step(std::integral_constant<int, LAST>{}, SET, ODD, [&](int g) {
 #pragma unroll
