@@ -19,6 +19,7 @@
 
 #include "iris_kernels_hip.h"
 #include "row_groups.h"
+#include "write_through.h"
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -382,7 +383,7 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
                 if (c < 4 * NA && m < m_end && n < N) {
                     f32x4 *to = reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(y) + (size_t)m * N + n);
                     if constexpr (STREAM) __builtin_nontemporal_store(v, to);
-                    else *to = v;
+                    else store_through(to, v);
                 }
             }
         }
@@ -403,7 +404,7 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
             if (c < 2 * NA && m < m_end && n < N) {
                 i32x4 *to = reinterpret_cast<i32x4 *>(reinterpret_cast<uint16_t *>(y) + (size_t)m * N + n);
                 if constexpr (STREAM) __builtin_nontemporal_store(v, to);
-                else *to = v;
+                else store_through(to, v);
             }
         }
     }
@@ -638,12 +639,12 @@ k_mxfp4_tiles(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t 
         OUT *to = y + (size_t)m * N + n;
         const f32x4 v = sum(row, c);
         if constexpr (CHUNKS == 1) {
-            if (whole) *reinterpret_cast<f32x4 *>(to) = v;
+            if (whole) store_through(to, v);
             else store4(to, v, N - n);
         } else {
             const f32x4 w = sum(row, c + 1);
             if (whole) {
-                *reinterpret_cast<uint4 *>(to) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(w[0], w[1]), pack_bf16(w[2], w[3]));
+                store_through(to, i32x4{(int)pack_bf16(v[0], v[1]), (int)pack_bf16(v[2], v[3]), (int)pack_bf16(w[0], w[1]), (int)pack_bf16(w[2], w[3])});
             } else {
                 store4(to, v, N - n);
                 if (n + 4 < N) store4(to + 4, w, N - n - 4);
@@ -662,10 +663,11 @@ long tiles_at_most(int M, int N, int groups, int tm, int tn) {
     return (GROUPED ? row_tiles_at_most(M, groups, tm) : ((long)M + tm - 1) / tm) * ((N + tn - 1L) / tn);
 }
 
-/* An output of 100 MB or more is stored with the streaming hint, past the Infinity Cache (256 MB), which then keeps the operands. us, plain / streaming:
- * 4608 x 4096 -> 36864 (340 MB) 360 / 341, with its conversion to MXFP4 behind it 427 / 419; -> 12288 (113 MB) 147 / 122 and 171.5 / 170.7; smaller
- * ones lose by what reads them next: -> 10240 (94 MB) 121.8 / 122.6 with the conversion, -> 8192 107.7 / 110.7. Kernels of their own: of a test in front
- * of two stores to one place the compiler keeps one, the plain one. */
+/* Results leave the L2s as they are stored (write_through.h), those of 100 MB and more past the Infinity Cache (256 MB) too, with the streaming hint: it then
+ * keeps the operands. us, plain / through, and with the conversion of the result to MXFP4 behind: 512 x 2560 -> 19456 19.0 / 18.2 and 25.2 / 24.6,
+ * 2115 x 4096 -> 4096 25.2 / 24.4 and 30.8 / 29.9, 1000 x 1024 -> 9216 11.7 / 10.4 and 17.6 / 16.9, 300 x 512 -> 4096 6.0 / 6.0 and 10.4 / 10.2. Plain / streaming:
+ * 4608 x 4096 -> 36864 (340 MB) 360 / 341 and 427 / 419, -> 12288 (113 MB) 147 / 122 and 171.5 / 170.7, -> 10240 (94 MB) with the conversion
+ * 121.8 / 122.6, -> 8192 107.7 / 110.7. Kernels of their own: of a test in front of two stores to one place the compiler keeps one, the plain one. */
 constexpr size_t STREAM_BYTES = (size_t)100 << 20;
 
 template <typename OUT, int NA, bool GROUPED, bool STREAM = false>
