@@ -14,6 +14,8 @@
  * (bound by the chip's power: on random codes its matrix cores alone keep up 6880 TFLOP/s). plan_mxfp4 chooses.
  */
 #include <hip/hip_runtime.h>
+
+#include <climits>
 #include <stdint.h>
 #include <type_traits>
 
@@ -41,6 +43,31 @@ __device__ __forceinline__ void store4(float *p, f32x4 v, int n_left) {
 __device__ __forceinline__ void store4(uint16_t *p, f32x4 v, int n_left) {
     if (n_left >= 4 && ((uintptr_t)p & 7) == 0) { *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])); return; }
     for (int r = 0; r < 4 && r < n_left; r++) p[r] = (uint16_t)(pack_bf16(v[r], 0.0f) & 0xffffu);
+}
+/* 16 bytes of results at p, of which the row has `left` values: as one store whatever the alignment, through the L2s or with the streaming hint */
+typedef i32x4 i32x4_at2 __attribute__((aligned(2)));
+typedef i32x4 i32x4_at4 __attribute__((aligned(4)));
+template <bool STREAM>
+__device__ __forceinline__ void store16(uint16_t *p, i32x4 v, int left) {
+    if (left >= 8) {
+        if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<i32x4_at2 *>(p));
+        else store_through(p, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 7; i++)
+            if (i < left) p[i] = (uint16_t)((uint32_t)v[i / 2] >> (16 * (i & 1)));
+    }
+}
+template <bool STREAM>
+__device__ __forceinline__ void store16(float *p, i32x4 v, int left) {
+    if (left >= 4) {
+        if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<i32x4_at4 *>(p));
+        else store_through(p, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; i++)
+            if (i < left) p[i] = __int_as_float(v[i]);
+    }
 }
 /* scales: byte A_BYTE / B_BYTE of sa / sb; four bits an element on both sides */
 template <int A_BYTE, int B_BYTE>
@@ -165,9 +192,9 @@ k_mxfp4_rows(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
     store4(y + (size_t)m * N + n, v, N - n);
 }
 
-/* ---- tiles of 256 rows x 256, 224 or 192 columns ----
+/* ---- tiles of 256 rows x 256 or 192 columns ----
  *
- * For whole k tiles of 256 (in a multiple of 256, two at least): a k tile is 128 B of codes and 8 scales of every row. Eight waves, two per
+ * For whole k tiles of 256 (in a multiple of 256): a k tile is 128 B of codes and 8 scales of every row. Eight waves, two per
  * SIMD, 4 (rows of 64) x 2 (columns of 16 NA): a wave owns 64 rows x 16 NA columns = NA x 4 accumulator blocks. A k tile is two
  * k-steps of v_mfma_scale_f32_16x16x128: in k-step ks lane group g of the four holds block 2 g + ks of its row, so that its two scales are
  * neighbouring bytes. (32x32x64 products draw more power: on random codes the chip keeps up 6090 TFLOP/s of them and 6880 of these.)
@@ -182,7 +209,10 @@ k_mxfp4_rows(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
  * during the step before, the scales of the next tile in steps 0 and 2. Codes of k tile t + 2: the first half of W in steps 0 and 2 of
  * tile t, the rest in step 3, behind the one barrier of a tile, which frees the stage. Every memory instruction stands in a gap between two
  * products. Requests past the end of K are issued all the same (a branch around each costs more, and the waits count them), but all lanes ask for
- * one 16 B of the last tile, into a stage that nobody reads. */
+ * one 16 B of the last tile, into a stage that nobody reads.
+ *
+ * Any number of columns: of an unaligned row the pieces are stored as they lie (4608 x 4096 -> 9001, 112 us; with tiles of 128 x 128, 165). One k tile
+ * is taken too (2327 x 256 -> 16384, 24 us; 95). */
 template <int NA>
 struct Wide {
     static constexpr int TM = 256, TN = 32 * NA, WP = (2 * NA + 7) / 8;                  /* WP: 8-row pieces of half of W per wave */
@@ -250,9 +280,14 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
         }
     }
     const int srow = min(64 * wave, TM + TN - 64);             /* of [x | W] */
-    const uint32_t soff = (uint32_t)(64 * wave < TM ? min(m0 + srow + lane, m_end - 1) - m0 : min(n0 + srow - TM + lane, N - 1) - n0) * (uint32_t)nb;
+    uint32_t soff = (uint32_t)(64 * wave < TM ? min(m0 + srow + lane, m_end - 1) - m0 : min(n0 + srow - TM + lane, N - 1) - n0) * (uint32_t)nb;
     const uint8_t *x_tile = x + (size_t)m0 * nb * 16, *w_tile = W + (size_t)n0 * nb * 16;
-    const uint8_t *s_tile = 64 * wave < TM ? xs + (size_t)m0 * nb : Ws + (size_t)n0 * nb;
+    /* With one k tile a row has 8 scales, and the next row's come with them; behind the very last row there is none, it comes with the row in
+     * front. (Offsets are not negative: the base is 8 bytes lower.) */
+    const int one = nk == 1 ? 8 : 0, x_last = m_end == M ? M - 1 : INT_MAX, w_last = !GROUPED || rows.group == groups - 1 ? N - 1 : INT_MAX;
+    const int s_most = nk == 1 ? 0 : nk - 2;
+    const uint8_t *s_tile = (64 * wave < TM ? xs + (size_t)m0 * nb : Ws + (size_t)n0 * nb) - one;
+    soff += (64 * wave < TM ? m0 + srow + lane >= x_last : n0 + srow - TM + lane >= w_last) ? 0 : one;
     const uint32_t lds0 = lds_address(lds);
     uint32_t lanes = ~0u;                                      /* 0 in the last two tiles, see above */
     auto load_lds = [&](uint32_t to, const uint8_t *from, uint32_t off) {
@@ -264,7 +299,7 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
         load_lds(T::W0 + slot * T::WH + wpiece[j] * 1024, w_tile + (size_t)min(kt, nk - 1) * 128, woff[half][j]);
     };
     /* scales of k tiles 2 p and 2 p + 1, or of the last two */
-    auto request_s = [&](int p) { load_lds(T::S0 + (p & 1) * T::SC + srow * 16, s_tile + (size_t)min(2 * p, nk - 2) * 8, soff); };
+    auto request_s = [&](int p) { load_lds(T::S0 + (p & 1) * T::SC + srow * 16, s_tile + (size_t)min(2 * p, s_most) * 8, soff); };
 
     f32x4 acc[NA][4];                                          /* [16 columns][16 rows] */
 #pragma unroll
@@ -315,7 +350,8 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
 #pragma unroll
     for (int i = 0; i < 4 + H0; i++) read_first(0, i, 0, wn);
 #pragma unroll
-    for (int i = 0; i < NA + 4; i++) read_scale(0, i, 0);
+    for (int i = 0; i < NA + 4; i++)
+        read_scale(0, i, (i < NA ? n0 + 16 * (NA * wn + i) + li >= w_last : m0 + 64 * wm + 16 * (i - NA) + li >= x_last) ? one : 0);
 
     constexpr std::integral_constant<int, 0> k0{};
     constexpr std::integral_constant<int, 1> k1{};
@@ -362,7 +398,7 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
 
     /* acc[a][b][r] = y[m0 + 64 wm + 16 b + li][n0 + 16 NA wn + 16 a + 4 lg + r]. Through the LDS (16 KB a wave, its own region: no barrier), so
      * that a store instruction covers whole row segments. */
-    constexpr int PER16 = 16 / (int)sizeof(OUT);               /* outputs per 16 B; the launcher has N a multiple of it */
+    constexpr int PER16 = 16 / (int)sizeof(OUT);               /* outputs per 16 B */
     const int mw = m0 + 64 * wm, nw = n0 + 16 * NA * wn;
     uint8_t *mine = lds + wave * 16384;
     if constexpr (sizeof(OUT) == 4) {
@@ -379,12 +415,8 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
 #pragma unroll
             for (int it = 0; it < 16; it++) {
                 const int row = 2 * it + (lane >> 5), c = lane & 31, m = mw + 32 * half + row, n = nw + PER16 * c;
-                const f32x4 v = *reinterpret_cast<const f32x4 *>(&buf[row * 128 + 4 * ((c & 16) | ((c ^ row) & 15))]);
-                if (c < 4 * NA && m < m_end && n < N) {
-                    f32x4 *to = reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(y) + (size_t)m * N + n);
-                    if constexpr (STREAM) __builtin_nontemporal_store(v, to);
-                    else store_through(to, v);
-                }
+                const i32x4 v = *reinterpret_cast<const i32x4 *>(&buf[row * 128 + 4 * ((c & 16) | ((c ^ row) & 15))]);
+                if (c < 4 * NA && m < m_end && n < N) store16<STREAM>(y + (size_t)m * N + n, v, N - n);
             }
         }
     } else {
@@ -401,11 +433,7 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
         for (int it = 0; it < 16; it++) {
             const int row = 4 * it + (lane >> 4), c = lane & 15, m = mw + row, n = nw + PER16 * c;
             const i32x4 v = *reinterpret_cast<const i32x4 *>(&buf[row * 128 + 8 * (c ^ (row & 15))]);
-            if (c < 2 * NA && m < m_end && n < N) {
-                i32x4 *to = reinterpret_cast<i32x4 *>(reinterpret_cast<uint16_t *>(y) + (size_t)m * N + n);
-                if constexpr (STREAM) __builtin_nontemporal_store(v, to);
-                else store_through(to, v);
-            }
+            if (c < 2 * NA && m < m_end && n < N) store16<STREAM>(y + (size_t)m * N + n, v, N - n);
         }
     }
 }
@@ -631,24 +659,16 @@ k_mxfp4_tiles(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t 
         return v;
     };
     constexpr int CHUNKS = sizeof(OUT) == 4 ? 1 : 2, ACROSS = TN / 4 / CHUNKS;        /* chunks of four a thread stores at a time */
-    const bool whole = N % (4 * CHUNKS) == 0 && ((uintptr_t)y & 15) == 0;
 #pragma unroll 4
     for (int i = tid; i < TM * ACROSS; i += T::THREADS) {
         const int row = i / ACROSS, c = i % ACROSS * CHUNKS, m = m0 + row, n = n0 + 4 * c;
         if (m >= m_end || n >= N) continue;
-        OUT *to = y + (size_t)m * N + n;
         const f32x4 v = sum(row, c);
         if constexpr (CHUNKS == 1) {
-            if (whole) store_through(to, v);
-            else store4(to, v, N - n);
+            store16<false>(y + (size_t)m * N + n, __builtin_bit_cast(i32x4, v), N - n);
         } else {
             const f32x4 w = sum(row, c + 1);
-            if (whole) {
-                store_through(to, i32x4{(int)pack_bf16(v[0], v[1]), (int)pack_bf16(v[2], v[3]), (int)pack_bf16(w[0], w[1]), (int)pack_bf16(w[2], w[3])});
-            } else {
-                store4(to, v, N - n);
-                if (n + 4 < N) store4(to + 4, w, N - n - 4);
-            }
+            store16<false>(y + (size_t)m * N + n, i32x4{(int)pack_bf16(v[0], v[1]), (int)pack_bf16(v[2], v[3]), (int)pack_bf16(w[0], w[1]), (int)pack_bf16(w[2], w[3])}, N - n);
         }
     }
 }
@@ -721,9 +741,11 @@ constexpr Shape SHAPES[] = {{32, 32, 4, 3.36f, 0.129f, 0.098f, 1.6f},   {64, 64,
                             {128, 128, 1, 4.85f, 0.205f, 0.455f, 5.5f}, {256, 192, 1, 5.0f, 0.326f, 0.973f, 6.0f}, {256, 256, 1, 5.16f, 0.635f, 1.22f, 6.0f}};
 constexpr int NSHAPES = sizeof(SHAPES) / sizeof(SHAPES[0]), FIRST_WIDE = 4;
 
-/* -1 and -2: k_mxfp4_rows with that many blocks of columns, 0 - 3: k_mxfp4_tiles, 4 and 5: k_mxfp4_wide, in the order of SHAPES. tail: k_mxfp4_tiles in
- * its form for rows of any length, whose k tiles take a third and whose further rounds twice as long. */
-int plan_mxfp4(int groups, int M, int N, int nb, bool tail, bool wide_stores) {
+/* -1 and -2: k_mxfp4_rows with that many blocks of columns, 0 - 3: k_mxfp4_tiles, 4 and 5: k_mxfp4_wide, in the order of SHAPES. whole: rows of whole k tiles
+ * and aligned scales; otherwise, and with one k tile, k_mxfp4_tiles runs in its form for rows of any length, whose k tiles take a third and whose
+ * further rounds twice as long. */
+int plan_mxfp4(int groups, int M, int N, int nb, bool whole) {
+    const bool tail = !whole || nb < 16, wide = whole && M >= 256 && N >= 192;
     const long some = groups < M ? groups : M;
     auto row_tiles = [&](int tm) { return groups == 1 ? ((long)M + tm - 1) / tm : row_tiles_about(M, groups, tm); };
     const float weights = 17.0f * (float)nb * (float)N, fresh = (float)some * weights / 5.0e6f;    /* HBM's 5 TB/s */
@@ -735,11 +757,12 @@ int plan_mxfp4(int groups, int M, int N, int nb, bool tail, bool wide_stores) {
     /* two blocks of columns: 40 rows over 64 weight matrices of 2560 -> 1536 13.9 us with one, 12.7 with two; 1 row, 4096 -> 4096 3.7 / 4.9 */
     int plan = row_tiles(16) * ((N + 31L) / 32) >= 512 ? -2 : -1;
     /* the tiles' offsets inside a tile of rows have 32 bits */
-    for (int i = 0; i < (nb >> 20 ? 0 : tail || M < 256 || N < 192 || !wide_stores ? FIRST_WIDE : NSHAPES); i++) {
+    for (int i = 0; i < (nb >> 20 ? 0 : wide ? NSHAPES : FIRST_WIDE); i++) {
         const Shape &s = SHAPES[i];
         const long wgs = row_tiles(s.tm) * ((N + s.tn - 1L) / s.tn), each = (wgs + 255) / 256, rounds = (wgs + 256L * s.resident - 1) / (256L * s.resident);
         const float shared = s.share * (float)each, step = shared > s.step ? shared : s.step;
-        float us = s.fixed + (float)((nb + 7) / 8) * step * (tail ? 1.3f : 1.0f) + (float)(rounds - 1) * s.again * (tail ? 2.0f : 1.0f);
+        const bool slower = tail && i < FIRST_WIDE;
+        float us = s.fixed + (float)((nb + 7) / 8) * step * (slower ? 1.3f : 1.0f) + (float)(rounds - 1) * s.again * (slower ? 2.0f : 1.0f);
         if (us < s.fixed + fresh) us = s.fixed + fresh;
         if (us < best) { best = us; plan = i; }
     }
@@ -759,14 +782,13 @@ int launch_shape(int shape, hipStream_t st, KERNEL_PARAMS) {
 
 template <typename OUT, bool GROUPED>
 int linear(hipStream_t st, KERNEL_PARAMS) {
-    const bool tail = nb % 8 != 0 || nb < 16 || (((uintptr_t)xs | (uintptr_t)Ws) & 7) != 0;
-    const bool wide_stores = N % (16 / (int)sizeof(OUT)) == 0 && ((uintptr_t)y & 15) == 0;
-    const int plan = plan_mxfp4(GROUPED ? groups : 1, M, N, nb, tail, wide_stores);
+    const bool whole = nb % 8 == 0 && (((uintptr_t)xs | (uintptr_t)Ws) & 7) == 0;
+    const int plan = plan_mxfp4(GROUPED ? groups : 1, M, N, nb, whole);
     if (plan == -1) return launch_rows<OUT, 1, GROUPED>(st, KERNEL_ARGS);
     if (plan == -2) return launch_rows<OUT, 2, GROUPED>(st, KERNEL_ARGS);
     if (plan == 5) return launch_wide<OUT, 8, GROUPED>(st, KERNEL_ARGS);
     if (plan == 4) return launch_wide<OUT, 6, GROUPED>(st, KERNEL_ARGS);
-    return tail ? launch_shape<OUT, true, GROUPED>(plan, st, KERNEL_ARGS) : launch_shape<OUT, false, GROUPED>(plan, st, KERNEL_ARGS);
+    return !whole || nb < 16 ? launch_shape<OUT, true, GROUPED>(plan, st, KERNEL_ARGS) : launch_shape<OUT, false, GROUPED>(plan, st, KERNEL_ARGS);
 }
 
 template <typename OUT>
@@ -781,9 +803,9 @@ int linear(void *stream, OUT *y, const uint8_t *x, const uint8_t *xs, const uint
 extern "C" {
 
 /* The kernel a layer of these sizes takes with aligned operands, as plan_mxfp4 numbers them. No GPU needed. */
-int iris_hip_linear_mxfp4_plan(int groups, int rows, int in, int out, int out_bytes) {
+int iris_hip_linear_mxfp4_plan(int groups, int rows, int in, int out) {
     const int nb = (int)(((long)in + 31) / 32);
-    return plan_mxfp4(groups, rows, out, nb, nb % 8 != 0 || nb < 16, out % (16 / out_bytes) == 0);
+    return plan_mxfp4(groups, rows, out, nb, nb % 8 == 0);
 }
 
 int iris_hip_linear_mxfp4_f32(void *stream, float *y, const uint8_t *x, const uint8_t *xs, const uint8_t *W, const uint8_t *Ws, const int *first_row, int groups,

@@ -176,7 +176,7 @@ int iris_hip_bf16_to_mxfp4(void *stream, uint8_t *codes, uint8_t *scales, const 
 int iris_hip_mxfp4_to_f32(void *stream, float *dst, int ld, const uint8_t *codes, const uint8_t *scales, int rows, int cols);
 int iris_hip_mxfp4_to_bf16(void *stream, uint16_t *dst, int ld, const uint8_t *codes, const uint8_t *scales, int rows, int cols);
 /* Which kernel a layer takes, host arithmetic only: -1, -2 k_mxfp4_rows, 0 - 3 k_mxfp4_tiles, 4, 5 k_mxfp4_wide */
-int iris_hip_linear_mxfp4_plan(int groups, int rows, int in, int out, int out_bytes);
+int iris_hip_linear_mxfp4_plan(int groups, int rows, int in, int out);
 /* y[rows, out] = x W^T, x and W as codes (16-byte aligned) and scales; first_row NULL: one W for all rows, otherwise as above */
 int iris_hip_linear_mxfp4_f32(void *stream, float *y, const uint8_t *x, const uint8_t *xs, const uint8_t *W, const uint8_t *Ws, const int *first_row, int groups,
                               int rows, int in, int out);

@@ -252,7 +252,7 @@ def test_grouped_layer(dev, name, k, n, out):
 # ----------------------------------------------------------------------------------------------------------------- routes
 def plan_of(groups, rows, k, n, out):
     import iris_c_amd
-    return iris_c_amd.load().iris_hip_linear_mxfp4_plan(groups, rows, k, n, 4 if out == "f32" else 2)
+    return iris_c_amd.load().iris_hip_linear_mxfp4_plan(groups, rows, k, n)
 
 
 # rows of each group (one: no groups), k, n, and the kernel: -1, -2 a few rows, 0 - 3 the smaller tiles, 4 and 5 those of 256 rows
@@ -279,6 +279,24 @@ def test_every_route(dev, sizes, k, n, route, out):
     for g in range(len(sizes)):
         want[first[g]:first[g + 1]] = x[first[g]:first[g + 1]] @ w[g].T
     check_exact(got, want, out)
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [4007, 8001, 10820])
+@pytest.mark.parametrize("k", [256, 512, 768])
+@pytest.mark.parametrize("sizes", [[1300], [700, 0, 601], [1, 1299], [1299, 1]])
+def test_wide_tiles_at_any_width(dev, sizes, k, n, out):
+    """Rows of results that start anywhere, and one k tile, whose scales are fetched with their neighbours'; the groups reach the last row, where there
+    are none"""
+    rows, groups = sum(sizes), len(sizes)
+    assert plan_of(groups, rows, k, n, out) >= 4
+    rng = np.random.default_rng(n + k)
+    cx, sx = exact_inputs(rng, rows, k)
+    cw, sw = exact_inputs(rng, groups * n, k)
+    first = np.concatenate([[0], np.cumsum(sizes)])
+    got = run_layer(dev, cx, sx, cw, sw, rows, k, n, out, first if groups > 1 else None)
+    x, w = mx.decode(cx, sx, k), mx.decode(cw, sw, k).reshape(groups, n, k)
+    check_exact(got, np.concatenate([x[first[g]:first[g + 1]] @ w[g].T for g in range(groups)]), out)
 
 
 @pytest.mark.parametrize("rows,k,n", [(3, 1024, 64), (70, 1024, 512), (300, 768, 512), (500, 512, 16384)])
