@@ -160,3 +160,29 @@ def test_ranges_of_k_leave_rows_in_no_group_alone(dev):
     x, w = whole(rng, rows, k), whole(rng, len(sizes), n, k)
     for out in ("f32", "bf16"):
         check(run(dev, x, w, first, rows, k, n, out), reference(x, w, first, rows, n), out)
+
+
+# rows of each group, odd k, n, kernel and its shape
+ODD = [([3, 0, 1], 129, 1001, 1, 1), ([3, 4, 1], 4097, 1001, 1, 1), ([5] * 16, 777, 2560, 1, 2), ([600, 0], 1355, 512, 1, 2), ([3500, 0], 1355, 256, 0, 2), ([70, 81], 1601, 2661, 0, 2), ([1000, 1000], 833, 2561, 0, 4)]
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2])
+@pytest.mark.parametrize("sizes,k,n,kernel,shape", ODD)
+def test_rows_that_start_in_the_middle_of_four_bytes(dev, sizes, k, n, kernel, shape, offset):
+    first = np.concatenate([[0], np.cumsum(sizes)])
+    rows = int(first[-1])
+    assert plan_of(len(sizes), rows, k, n, 4)[:2] == (kernel, shape)
+    rng = np.random.default_rng(k)
+    x, w = whole(rng, rows, k), whole(rng, len(sizes), n, k)
+    for out in ("f32", "bf16"):
+        check(run(dev, x, w, first, rows, k, n, out, offset), reference(x, w, first, rows, n), out)
+
+
+@pytest.mark.parametrize("offset", [1, 2, 3, 8])
+@pytest.mark.parametrize("rows,k,n", [(3, 1024, 96), (40, 2560, 640), (300, 512, 1024)])
+def test_rows_of_even_length_from_any_start(dev, rows, k, n, offset):
+    rng = np.random.default_rng(k)
+    first = [0, rows // 3, rows]
+    x, w = whole(rng, rows, k), whole(rng, 2, n, k)
+    for out in ("f32", "bf16"):
+        check(run(dev, x, w, first, rows, k, n, out, offset), reference(x, w, first, rows, n), out)
