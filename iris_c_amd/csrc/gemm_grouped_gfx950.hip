@@ -266,7 +266,7 @@ bool halves(const uint16_t *x, const uint16_t *W, int in) { return (in & 1) || (
 template <typename OUT, int A, int U, int KW>
 int launch_rows(hipStream_t st, OUT *y, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int rows, int in, int out) {
     const long wgs = row_tiles_at_most(rows, groups, 16) * ((out + 16L * A - 1) / (16 * A));
-    if (wgs >> 30) return (int)hipErrorInvalidValue;
+    if (wgs * 64 * KW >> 32) return (int)hipErrorInvalidValue;  /* a launch has fewer than 2^32 threads */
     const dim3 grid((unsigned)(wgs + 7) / 8 * 8), block(64 * KW);
     if (halves(x, W, in)) hipLaunchKernelGGL((k_grouped_rows<OUT, A, U, KW, true>), grid, block, 0, st, y, x, W, rows, out, in, first_row, groups);
     else hipLaunchKernelGGL((k_grouped_rows<OUT, A, U, KW, false>), grid, block, 0, st, y, x, W, rows, out, in, first_row, groups);
@@ -276,7 +276,7 @@ int launch_rows(hipStream_t st, OUT *y, const uint16_t *x, const uint16_t *W, co
 template <typename OUT, int B>
 int launch_any(hipStream_t st, OUT *y, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int rows, int in, int out) {
     const long wgs = row_tiles_at_most(rows, groups, 32 * B) * ((out + 32L * B - 1) / (32 * B));
-    if (wgs >> 31) return (int)hipErrorInvalidValue;
+    if (wgs * 256 >> 32) return (int)hipErrorInvalidValue;
     hipLaunchKernelGGL((k_grouped_any<OUT, B>), dim3((unsigned)wgs), dim3(256), 0, st, y, x, W, rows, out, in, first_row, groups);
     return (int)hipGetLastError();
 }

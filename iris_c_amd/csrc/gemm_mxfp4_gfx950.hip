@@ -702,7 +702,7 @@ int launch_wide(hipStream_t st, KERNEL_PARAMS) {
         configured = true;
     }
     const long most = tiles_at_most<GROUPED>(M, N, groups, T::TM, T::TN);
-    if (most >> 30) return (int)hipErrorInvalidValue;
+    if (most * 512 >> 32) return (int)hipErrorInvalidValue;     /* a launch has fewer than 2^32 threads */
     hipLaunchKernelGGL((k_mxfp4_wide<OUT, NA, STREAM, GROUPED>), dim3((unsigned)(most + 7) / 8 * 8), dim3(512), T::LDS, st, KERNEL_ARGS);
     return (int)hipGetLastError();
 }
@@ -718,7 +718,7 @@ int launch_tiles(hipStream_t st, KERNEL_PARAMS) {
         configured = true;
     }
     const long most = tiles_at_most<GROUPED>(M, N, groups, T::TM, T::TN);
-    if (most >> 30) return (int)hipErrorInvalidValue;
+    if (most * T::THREADS >> 32) return (int)hipErrorInvalidValue;
     hipLaunchKernelGGL((k_mxfp4_tiles<OUT, NB, NA, WM, WN, KG, STAGES, TAIL, GROUPED>), dim3((unsigned)(most + 7) / 8 * 8), dim3(T::THREADS), T::LDS, st, KERNEL_ARGS);
     return (int)hipGetLastError();
 }
@@ -726,7 +726,7 @@ int launch_tiles(hipStream_t st, KERNEL_PARAMS) {
 template <typename OUT, int A, bool GROUPED>
 int launch_rows(hipStream_t st, KERNEL_PARAMS) {
     const long most = tiles_at_most<GROUPED>(M, N, groups, 16, 16 * A);
-    if (most >> 30) return (int)hipErrorInvalidValue;
+    if (most * 64 * ROWS_KW >> 32) return (int)hipErrorInvalidValue;
     hipLaunchKernelGGL((k_mxfp4_rows<OUT, A, GROUPED>), dim3((unsigned)(most + 7) / 8 * 8), dim3(64 * ROWS_KW), 0, st, KERNEL_ARGS);
     return (int)hipGetLastError();
 }

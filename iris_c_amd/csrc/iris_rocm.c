@@ -555,7 +555,7 @@ static int grouped_args(const char *what, const int *first_row, int groups, int 
         if (!y || !x || !W) { fail(-1, what, "y, x or W is missing"); return; }                                 \
         if (!need_ready(what)) return;                                                                          \
         g_last_kernel = name;                                                                                   \
-        LAUNCH(what, launcher(g_stream, linear_part(), y, x, W, first_row, groups, rows, in, out));                            \
+        LAUNCH(what, launcher(g_stream, linear_part(), y, x, W, first_row, groups, rows, in, out));             \
     } while (0)
 
 void iris_dev_linear_f32_grouped(float *y, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int rows, int in, int out) {

@@ -187,7 +187,7 @@ template <typename T, bool STREAM>
 int launch_to(void *stream, uint8_t *codes, uint8_t *scales, const T *src, int ld, int rows, int cols) {
     const uint32_t per_row = 4u * (((uint32_t)cols + 31) / 32);
     const size_t groups = (size_t)rows * per_row, blocks = (groups + THREADS * UNROLL - 1) / (THREADS * UNROLL);
-    if (blocks >> 31) return (int)hipErrorInvalidValue;
+    if (blocks * THREADS >> 32) return (int)hipErrorInvalidValue;       /* a launch has fewer than 2^32 threads */
     hipLaunchKernelGGL((k_to_mxfp4<T, STREAM>), dim3((unsigned)blocks), dim3(THREADS), 0, (hipStream_t)stream, reinterpret_cast<uint32_t *>(codes), scales, src, ld,
                        cols, per_row, groups);
     return (int)hipGetLastError();
@@ -196,7 +196,7 @@ template <typename T, bool STREAM>
 int launch_from(void *stream, T *dst, int ld, const uint8_t *codes, const uint8_t *scales, int rows, int cols) {
     const uint32_t per_row = 4u * (((uint32_t)cols + 31) / 32);
     const size_t groups = (size_t)rows * per_row, blocks = (groups + THREADS * UNROLL - 1) / (THREADS * UNROLL);
-    if (blocks >> 31) return (int)hipErrorInvalidValue;
+    if (blocks * THREADS >> 32) return (int)hipErrorInvalidValue;       /* a launch has fewer than 2^32 threads */
     hipLaunchKernelGGL((k_mxfp4_to<T, STREAM>), dim3((unsigned)blocks), dim3(THREADS), 0, (hipStream_t)stream, dst, ld, reinterpret_cast<const uint32_t *>(codes), scales,
                        cols, per_row, groups);
     return (int)hipGetLastError();
