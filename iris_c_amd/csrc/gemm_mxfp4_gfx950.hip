@@ -44,29 +44,29 @@ __device__ __forceinline__ void store4(uint16_t *p, f32x4 v, int n_left) {
     if (n_left >= 4 && ((uintptr_t)p & 7) == 0) { *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])); return; }
     for (int r = 0; r < 4 && r < n_left; r++) p[r] = (uint16_t)(pack_bf16(v[r], 0.0f) & 0xffffu);
 }
-/* 16 bytes of results at p, of which the row has `left` values: as one store whatever the alignment, through the L2s or with the streaming hint */
-typedef i32x4 i32x4_at2 __attribute__((aligned(2)));
-typedef i32x4 i32x4_at4 __attribute__((aligned(4)));
-template <bool STREAM>
-__device__ __forceinline__ void store16(uint16_t *p, i32x4 v, int left) {
-    if (left >= 8) {
-        if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<i32x4_at2 *>(p));
-        else store_through(p, v);
+/* 16 bytes of results at p, of which the row has `left` values. Where all rows are aligned, and so none ends inside 16 bytes, through the L2s or with the
+ * streaming hint; otherwise plainly (parts of lines are better put together in the L2s: 777 x 1000 -> 1111 5.2 us, 6.3 through them) or with the hint,
+ * as one store whatever the alignment, and single values at the end of a row. */
+enum Store { THROUGH, STREAMING, PLAIN_ANY, STREAMING_ANY };
+typedef i32x4 i32x4_at2 __attribute__((aligned(2)));           /* at an address that suits one value */
+template <Store KIND> using Kind = std::integral_constant<Store, KIND>;
+template <Store KIND, typename OUT>
+__device__ __forceinline__ void store16(OUT *p, i32x4 v, int left) {
+    constexpr int VALUES = 16 / (int)sizeof(OUT);
+    if constexpr (KIND == THROUGH) {
+        store_through(p, v);
+    } else if constexpr (KIND == STREAMING) {
+        __builtin_nontemporal_store(v, reinterpret_cast<i32x4 *>(p));
+    } else if (left >= VALUES) {
+        if constexpr (KIND == STREAMING_ANY) __builtin_nontemporal_store(v, reinterpret_cast<i32x4_at2 *>(p));
+        else *reinterpret_cast<i32x4_at2 *>(p) = v;
     } else {
 #pragma unroll
-        for (int i = 0; i < 7; i++)
-            if (i < left) p[i] = (uint16_t)((uint32_t)v[i / 2] >> (16 * (i & 1)));
-    }
-}
-template <bool STREAM>
-__device__ __forceinline__ void store16(float *p, i32x4 v, int left) {
-    if (left >= 4) {
-        if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<i32x4_at4 *>(p));
-        else store_through(p, v);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 3; i++)
-            if (i < left) p[i] = __int_as_float(v[i]);
+        for (int i = 0; i < VALUES - 1; i++)
+            if (i < left) {
+                if constexpr (VALUES == 8) p[i] = (OUT)((uint32_t)v[i / 2] >> (16 * (i & 1)));
+                else p[i] = __int_as_float(v[i]);
+            }
     }
 }
 /* scales: byte A_BYTE / B_BYTE of sa / sb; four bits an element on both sides */
@@ -194,7 +194,7 @@ k_mxfp4_rows(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
 
 /* ---- tiles of 256 rows x 256 or 192 columns ----
  *
- * For whole k tiles of 256 (in a multiple of 256): a k tile is 128 B of codes and 8 scales of every row. Eight waves, two per
+ * For k tiles of 256: 128 B of codes and 8 scales of every row. Eight waves, two per
  * SIMD, 4 (rows of 64) x 2 (columns of 16 NA): a wave owns 64 rows x 16 NA columns = NA x 4 accumulator blocks. A k tile is two
  * k-steps of v_mfma_scale_f32_16x16x128: in k-step ks lane group g of the four holds block 2 g + ks of its row, so that its two scales are
  * neighbouring bytes. (32x32x64 products draw more power: on random codes the chip keeps up 6090 TFLOP/s of them and 6880 of these.)
@@ -211,8 +211,12 @@ k_mxfp4_rows(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
  * products. Requests past the end of K are issued all the same (a branch around each costs more, and the waits count them), but all lanes ask for
  * one 16 B of the last tile, into a stage that nobody reads.
  *
- * Any number of columns: of an unaligned row the pieces are stored as they lie (4608 x 4096 -> 9001, 112 us; with tiles of 128 x 128, 165). One k tile
- * is taken too (2327 x 256 -> 16384, 24 us; 95). */
+ * Any number of columns: of an unaligned row the pieces are stored as they lie (4608 x 4096 -> 9001 98 us; with tiles of 128 x 128 165). One k tile
+ * is taken too (2327 x 256 -> 16384 24 us; 95).
+ *
+ * Rows that are no whole k tiles long, or whose scales are not 8-byte aligned: k_mxfp4_scales copies the scales into rows of 8 bytes a k tile. The last k
+ * tile then is the last 8 blocks of a row, with scales 0 for those that the one before it has had: 2^-254 a product, nothing in f32, whatever the codes. us,
+ * with it / tiles of 128 x 128: 2930 x 3793 -> 6325 57 / 97, 1158 x 896 -> 10821 18 / 48, 512 x 2500 -> 19457 26 / 51. */
 template <int NA>
 struct Wide {
     static constexpr int TM = 256, TN = 32 * NA, WP = (2 * NA + 7) / 8;                  /* WP: 8-row pieces of half of W per wave */
@@ -252,12 +256,13 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
     const int band = work / (BAND * tiles_n), in_band = work - band * (BAND * tiles_n), band_rows = min(tiles_m - band * BAND, BAND);
     const int tm = band * BAND + in_band % band_rows, n0 = in_band / band_rows * TN;
     RowTile rows = {tm * TM, M, 0};
+    const int nk = (nb + 7) / 8, ns = 8 * nk;                  /* k tiles, scales a row */
     if constexpr (GROUPED) {
         rows = all.tile(tm);
         W += (size_t)rows.group * N * nb * 16;
-        Ws += (size_t)rows.group * N * nb;
+        Ws += (size_t)rows.group * N * ns;
     }
-    const int m0 = rows.m0, m_end = rows.end, nk = nb / 8;
+    const int m0 = rows.m0, m_end = rows.end;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4, wm = wave & 3, wn = wave >> 2;
@@ -280,13 +285,14 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
         }
     }
     const int srow = min(64 * wave, TM + TN - 64);             /* of [x | W] */
-    uint32_t soff = (uint32_t)(64 * wave < TM ? min(m0 + srow + lane, m_end - 1) - m0 : min(n0 + srow - TM + lane, N - 1) - n0) * (uint32_t)nb;
+    uint32_t soff = (uint32_t)(64 * wave < TM ? min(m0 + srow + lane, m_end - 1) - m0 : min(n0 + srow - TM + lane, N - 1) - n0) * (uint32_t)ns;
     const uint8_t *x_tile = x + (size_t)m0 * nb * 16, *w_tile = W + (size_t)n0 * nb * 16;
+    const int last = (nb - 8) * 16;                            /* codes of the last k tile */
     /* With one k tile a row has 8 scales, and the next row's come with them; behind the very last row there is none, it comes with the row in
      * front. (Offsets are not negative: the base is 8 bytes lower.) */
     const int one = nk == 1 ? 8 : 0, x_last = m_end == M ? M - 1 : INT_MAX, w_last = !GROUPED || rows.group == groups - 1 ? N - 1 : INT_MAX;
     const int s_most = nk == 1 ? 0 : nk - 2;
-    const uint8_t *s_tile = (64 * wave < TM ? xs + (size_t)m0 * nb : Ws + (size_t)n0 * nb) - one;
+    const uint8_t *s_tile = (64 * wave < TM ? xs + (size_t)m0 * ns : Ws + (size_t)n0 * ns) - one;
     soff += (64 * wave < TM ? m0 + srow + lane >= x_last : n0 + srow - TM + lane >= w_last) ? 0 : one;
     const uint32_t lds0 = lds_address(lds);
     uint32_t lanes = ~0u;                                      /* 0 in the last two tiles, see above */
@@ -294,9 +300,9 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
         off &= lanes;
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds0 + to), "v"(off), "s"(from) : "memory", "m0");
     };
-    auto request_x = [&](int j, int kt, int stage) { load_lds(stage * T::XS + (4 * wave + j) * 1024, x_tile + (size_t)min(kt, nk - 1) * 128, xoff[j]); };
+    auto request_x = [&](int j, int kt, int stage) { load_lds(stage * T::XS + (4 * wave + j) * 1024, x_tile + min(kt * 128, last), xoff[j]); };
     auto request_w = [&](int half, int j, int kt, int slot) {
-        load_lds(T::W0 + slot * T::WH + wpiece[j] * 1024, w_tile + (size_t)min(kt, nk - 1) * 128, woff[half][j]);
+        load_lds(T::W0 + slot * T::WH + wpiece[j] * 1024, w_tile + min(kt * 128, last), woff[half][j]);
     };
     /* scales of k tiles 2 p and 2 p + 1, or of the last two */
     auto request_s = [&](int p) { load_lds(T::S0 + (p & 1) * T::SC + srow * 16, s_tile + (size_t)min(2 * p, s_most) * 8, soff); };
@@ -400,6 +406,7 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
      * that a store instruction covers whole row segments. */
     constexpr int PER16 = 16 / (int)sizeof(OUT);               /* outputs per 16 B */
     const int mw = m0 + 64 * wm, nw = n0 + 16 * NA * wn;
+    const bool aligned = N % PER16 == 0 && ((uintptr_t)y & 15) == 0;
     uint8_t *mine = lds + wave * 16384;
     if constexpr (sizeof(OUT) == 4) {
         float *buf = reinterpret_cast<float *>(mine);          /* 32 rows x 128 f32 at a time, chunk c of row r in slot (c & 16) | ((c ^ r) & 15) */
@@ -412,12 +419,16 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
                     const int chunk = 4 * a + lg;
                     *reinterpret_cast<f32x4 *>(&buf[(16 * b + li) * 128 + 4 * ((chunk & 16) | ((chunk ^ li) & 15))]) = acc[a][2 * half + b];
                 }
+            auto store = [&](auto kind) {
 #pragma unroll
-            for (int it = 0; it < 16; it++) {
-                const int row = 2 * it + (lane >> 5), c = lane & 31, m = mw + 32 * half + row, n = nw + PER16 * c;
-                const i32x4 v = *reinterpret_cast<const i32x4 *>(&buf[row * 128 + 4 * ((c & 16) | ((c ^ row) & 15))]);
-                if (c < 4 * NA && m < m_end && n < N) store16<STREAM>(y + (size_t)m * N + n, v, N - n);
-            }
+                for (int it = 0; it < 16; it++) {
+                    const int row = 2 * it + (lane >> 5), c = lane & 31, m = mw + 32 * half + row, n = nw + PER16 * c;
+                    const i32x4 v = *reinterpret_cast<const i32x4 *>(&buf[row * 128 + 4 * ((c & 16) | ((c ^ row) & 15))]);
+                    if (c < 4 * NA && m < m_end && n < N) store16<decltype(kind)::value>(y + (size_t)m * N + n, v, N - n);
+                }
+            };
+            if (aligned) store(Kind<STREAM ? STREAMING : THROUGH>{});
+            else store(Kind<STREAM ? STREAMING_ANY : PLAIN_ANY>{});
         }
     } else {
         uint16_t *buf = reinterpret_cast<uint16_t *>(mine);    /* 64 rows x 128 bf16, chunk c of row r in slot c ^ (r % 16) */
@@ -429,12 +440,16 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
                 *reinterpret_cast<uint2 *>(&buf[(16 * b + li) * 128 + 8 * (chunk ^ li) + 4 * (lg & 1)]) =
                     make_uint2(pack_bf16(acc[a][b][0], acc[a][b][1]), pack_bf16(acc[a][b][2], acc[a][b][3]));
             }
+        auto store = [&](auto kind) {
 #pragma unroll
-        for (int it = 0; it < 16; it++) {
-            const int row = 4 * it + (lane >> 4), c = lane & 15, m = mw + row, n = nw + PER16 * c;
-            const i32x4 v = *reinterpret_cast<const i32x4 *>(&buf[row * 128 + 8 * (c ^ (row & 15))]);
-            if (c < 2 * NA && m < m_end && n < N) store16<STREAM>(y + (size_t)m * N + n, v, N - n);
-        }
+            for (int it = 0; it < 16; it++) {
+                const int row = 4 * it + (lane >> 4), c = lane & 15, m = mw + row, n = nw + PER16 * c;
+                const i32x4 v = *reinterpret_cast<const i32x4 *>(&buf[row * 128 + 8 * (c ^ (row & 15))]);
+                if (c < 2 * NA && m < m_end && n < N) store16<decltype(kind)::value>(y + (size_t)m * N + n, v, N - n);
+            }
+        };
+        if (aligned) store(Kind<STREAM ? STREAMING : THROUGH>{});
+        else store(Kind<STREAM ? STREAMING_ANY : PLAIN_ANY>{});
     }
 }
 
@@ -659,20 +674,40 @@ k_mxfp4_tiles(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t 
         return v;
     };
     constexpr int CHUNKS = sizeof(OUT) == 4 ? 1 : 2, ACROSS = TN / 4 / CHUNKS;        /* chunks of four a thread stores at a time */
+    const bool aligned = N % (4 * CHUNKS) == 0 && ((uintptr_t)y & 15) == 0;
+    auto store = [&](auto kind) {
 #pragma unroll 4
-    for (int i = tid; i < TM * ACROSS; i += T::THREADS) {
-        const int row = i / ACROSS, c = i % ACROSS * CHUNKS, m = m0 + row, n = n0 + 4 * c;
-        if (m >= m_end || n >= N) continue;
-        const f32x4 v = sum(row, c);
-        if constexpr (CHUNKS == 1) {
-            store16<false>(y + (size_t)m * N + n, __builtin_bit_cast(i32x4, v), N - n);
-        } else {
-            const f32x4 w = sum(row, c + 1);
-            store16<false>(y + (size_t)m * N + n, i32x4{(int)pack_bf16(v[0], v[1]), (int)pack_bf16(v[2], v[3]), (int)pack_bf16(w[0], w[1]), (int)pack_bf16(w[2], w[3])}, N - n);
+        for (int i = tid; i < TM * ACROSS; i += T::THREADS) {
+            const int row = i / ACROSS, c = i % ACROSS * CHUNKS, m = m0 + row, n = n0 + 4 * c;
+            if (m >= m_end || n >= N) continue;
+            const f32x4 v = sum(row, c);
+            i32x4 r = __builtin_bit_cast(i32x4, v);
+            if constexpr (CHUNKS == 2) {
+                const f32x4 w = sum(row, c + 1);
+                r = i32x4{(int)pack_bf16(v[0], v[1]), (int)pack_bf16(v[2], v[3]), (int)pack_bf16(w[0], w[1]), (int)pack_bf16(w[2], w[3])};
+            }
+            store16<decltype(kind)::value>(y + (size_t)m * N + n, r, N - n);
         }
-    }
+    };
+    if (aligned) store(Kind<THROUGH>{});
+    else store(Kind<PLAIN_ANY>{});
 }
 #pragma clang diagnostic pop
+
+/* rows of nb scales to rows of 8 bytes a k tile: M of xs, behind them those of Ws, `rows` in all; see k_mxfp4_wide */
+__global__ void __launch_bounds__(256)
+k_mxfp4_scales(uint64_t *__restrict__ to, const uint8_t *__restrict__ xs, const uint8_t *__restrict__ Ws, int M, size_t rows, int nb) {
+    const int nk = (nb + 7) / 8, over = 8 * nk - nb;
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, row = i / nk;
+    if (row >= rows) return;
+    const int kt = (int)(i - row * nk), skip = kt == nk - 1 ? over : 0;
+    const uint8_t *from = (row < (size_t)M ? xs + row * nb : Ws + (row - M) * nb) + (kt == nk - 1 ? nb - 8 : 8 * kt);
+    uint64_t v = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        if (j >= skip) v |= (uint64_t)from[j] << (8 * j);
+    to[i] = v;
+}
 
 /* the arguments of every kernel here */
 #define KERNEL_ARGS y, x, xs, W, Ws, M, N, nb, first_row, groups
@@ -690,10 +725,11 @@ long tiles_at_most(int M, int N, int groups, int tm, int tn) {
  * 121.8 / 122.6, -> 8192 107.7 / 110.7. Kernels of their own: of a test in front of two stores to one place the compiler keeps one, the plain one. */
 constexpr size_t STREAM_BYTES = (size_t)100 << 20;
 
+/* part: room for the copy of the scales, NULL where they can be read as they are */
 template <typename OUT, int NA, bool GROUPED, bool STREAM = false>
-int launch_wide(hipStream_t st, KERNEL_PARAMS) {
+int launch_wide(hipStream_t st, void *part, KERNEL_PARAMS) {
     if constexpr (!STREAM)
-        if ((size_t)M * N * sizeof(OUT) >= STREAM_BYTES) return launch_wide<OUT, NA, GROUPED, true>(st, KERNEL_ARGS);
+        if ((size_t)M * N * sizeof(OUT) >= STREAM_BYTES) return launch_wide<OUT, NA, GROUPED, true>(st, part, KERNEL_ARGS);
     using T = Wide<NA>;
     static bool configured = false;
     if (!configured) {
@@ -703,6 +739,14 @@ int launch_wide(hipStream_t st, KERNEL_PARAMS) {
     }
     const long most = tiles_at_most<GROUPED>(M, N, groups, T::TM, T::TN);
     if (most * 512 >> 32) return (int)hipErrorInvalidValue;     /* a launch has fewer than 2^32 threads */
+    if (part) {
+        const size_t all = (size_t)M + (size_t)groups * N, nk = (size_t)(nb + 7) / 8;
+        hipLaunchKernelGGL(k_mxfp4_scales, dim3((unsigned)((all * nk + 255) / 256)), dim3(256), 0, st, (uint64_t *)part, xs, Ws, M, all, nb);
+        hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return (int)e;
+        xs = (const uint8_t *)part;
+        Ws = xs + M * nk * 8;
+    }
     hipLaunchKernelGGL((k_mxfp4_wide<OUT, NA, STREAM, GROUPED>), dim3((unsigned)(most + 7) / 8 * 8), dim3(512), T::LDS, st, KERNEL_ARGS);
     return (int)hipGetLastError();
 }
@@ -742,10 +786,13 @@ constexpr Shape SHAPES[] = {{32, 32, 4, 3.36f, 0.129f, 0.098f, 1.6f},   {64, 64,
 constexpr int NSHAPES = sizeof(SHAPES) / sizeof(SHAPES[0]), FIRST_WIDE = 4;
 
 /* -1 and -2: k_mxfp4_rows with that many blocks of columns, 0 - 3: k_mxfp4_tiles, 4 and 5: k_mxfp4_wide, in the order of SHAPES. whole: rows of whole k tiles
- * and aligned scales; otherwise, and with one k tile, k_mxfp4_tiles runs in its form for rows of any length, whose k tiles take a third and whose
- * further rounds twice as long. */
-int plan_mxfp4(int groups, int M, int N, int nb, bool whole) {
-    const bool tail = !whole || nb < 16, wide = whole && M >= 256 && N >= 192;
+ * and aligned scales; otherwise k_mxfp4_wide needs part_bytes of workspace for a copy of the scales and 4 us more, and, as with one k tile, k_mxfp4_tiles runs
+ * in its form for rows of any length, whose k tiles take a third and whose further rounds twice as long. */
+int plan_mxfp4(int groups, int M, int N, int nb, bool whole, size_t part_bytes) {
+    const bool tail = !whole || nb < 16;
+    const size_t copy = ((size_t)M + (size_t)groups * N) * ((nb + 7) / 8 * 8);
+    const bool wide = M >= 256 && N >= 192 && nb >= 8 && (whole || copy <= part_bytes);
+    const float first = whole ? 0.0f : 4.0f + 2.0f * (float)copy / 2.5e6f;
     const long some = groups < M ? groups : M;
     auto row_tiles = [&](int tm) { return groups == 1 ? ((long)M + tm - 1) / tm : row_tiles_about(M, groups, tm); };
     const float weights = 17.0f * (float)nb * (float)N, fresh = (float)some * weights / 5.0e6f;    /* HBM's 5 TB/s */
@@ -764,6 +811,7 @@ int plan_mxfp4(int groups, int M, int N, int nb, bool whole) {
         const bool slower = tail && i < FIRST_WIDE;
         float us = s.fixed + (float)((nb + 7) / 8) * step * (slower ? 1.3f : 1.0f) + (float)(rounds - 1) * s.again * (slower ? 2.0f : 1.0f);
         if (us < s.fixed + fresh) us = s.fixed + fresh;
+        if (i >= FIRST_WIDE) us += first;
         if (us < best) { best = us; plan = i; }
     }
     return plan;
@@ -781,21 +829,22 @@ int launch_shape(int shape, hipStream_t st, KERNEL_PARAMS) {
 }
 
 template <typename OUT, bool GROUPED>
-int linear(hipStream_t st, KERNEL_PARAMS) {
+int linear(hipStream_t st, void *part, KERNEL_PARAMS) {
     const bool whole = nb % 8 == 0 && (((uintptr_t)xs | (uintptr_t)Ws) & 7) == 0;
-    const int plan = plan_mxfp4(GROUPED ? groups : 1, M, N, nb, whole);
+    const int plan = plan_mxfp4(groups, M, N, nb, whole, part ? IRIS_LINEAR_PART_BYTES : 0);
     if (plan == -1) return launch_rows<OUT, 1, GROUPED>(st, KERNEL_ARGS);
     if (plan == -2) return launch_rows<OUT, 2, GROUPED>(st, KERNEL_ARGS);
-    if (plan == 5) return launch_wide<OUT, 8, GROUPED>(st, KERNEL_ARGS);
-    if (plan == 4) return launch_wide<OUT, 6, GROUPED>(st, KERNEL_ARGS);
+    if (whole) part = nullptr;
+    if (plan == 5) return launch_wide<OUT, 8, GROUPED>(st, part, KERNEL_ARGS);
+    if (plan == 4) return launch_wide<OUT, 6, GROUPED>(st, part, KERNEL_ARGS);
     return !whole || nb < 16 ? launch_shape<OUT, true, GROUPED>(plan, st, KERNEL_ARGS) : launch_shape<OUT, false, GROUPED>(plan, st, KERNEL_ARGS);
 }
 
 template <typename OUT>
-int linear(void *stream, OUT *y, const uint8_t *x, const uint8_t *xs, const uint8_t *W, const uint8_t *Ws, const int *first_row, int groups, int rows, int in, int out) {
+int linear(void *stream, void *part, OUT *y, const uint8_t *x, const uint8_t *xs, const uint8_t *W, const uint8_t *Ws, const int *first_row, int groups, int rows, int in, int out) {
     const int nb = (int)(((long)in + 31) / 32);
-    return first_row ? linear<OUT, true>((hipStream_t)stream, y, x, xs, W, Ws, rows, out, nb, first_row, groups)
-                     : linear<OUT, false>((hipStream_t)stream, y, x, xs, W, Ws, rows, out, nb, nullptr, 1);
+    return first_row ? linear<OUT, true>((hipStream_t)stream, part, y, x, xs, W, Ws, rows, out, nb, first_row, groups)
+                     : linear<OUT, false>((hipStream_t)stream, part, y, x, xs, W, Ws, rows, out, nb, nullptr, 1);
 }
 
 }  // namespace
@@ -805,16 +854,16 @@ extern "C" {
 /* The kernel a layer of these sizes takes with aligned operands, as plan_mxfp4 numbers them. No GPU needed. */
 int iris_hip_linear_mxfp4_plan(int groups, int rows, int in, int out) {
     const int nb = (int)(((long)in + 31) / 32);
-    return plan_mxfp4(groups, rows, out, nb, nb % 8 == 0);
+    return plan_mxfp4(groups, rows, out, nb, nb % 8 == 0, IRIS_LINEAR_PART_BYTES);
 }
 
-int iris_hip_linear_mxfp4_f32(void *stream, float *y, const uint8_t *x, const uint8_t *xs, const uint8_t *W, const uint8_t *Ws, const int *first_row, int groups,
-                              int rows, int in, int out) {
-    return linear(stream, y, x, xs, W, Ws, first_row, groups, rows, in, out);
+int iris_hip_linear_mxfp4_f32(void *stream, float *part, float *y, const uint8_t *x, const uint8_t *xs, const uint8_t *W, const uint8_t *Ws, const int *first_row,
+                              int groups, int rows, int in, int out) {
+    return linear(stream, part, y, x, xs, W, Ws, first_row, groups, rows, in, out);
 }
-int iris_hip_linear_mxfp4_bf16(void *stream, uint16_t *y, const uint8_t *x, const uint8_t *xs, const uint8_t *W, const uint8_t *Ws, const int *first_row, int groups,
+int iris_hip_linear_mxfp4_bf16(void *stream, float *part, uint16_t *y, const uint8_t *x, const uint8_t *xs, const uint8_t *W, const uint8_t *Ws, const int *first_row, int groups,
                                int rows, int in, int out) {
-    return linear(stream, y, x, xs, W, Ws, first_row, groups, rows, in, out);
+    return linear(stream, part, y, x, xs, W, Ws, first_row, groups, rows, in, out);
 }
 
 }  // extern "C"

@@ -177,10 +177,11 @@ int iris_hip_mxfp4_to_f32(void *stream, float *dst, int ld, const uint8_t *codes
 int iris_hip_mxfp4_to_bf16(void *stream, uint16_t *dst, int ld, const uint8_t *codes, const uint8_t *scales, int rows, int cols);
 /* Which kernel a layer takes, host arithmetic only: -1, -2 k_mxfp4_rows, 0 - 3 k_mxfp4_tiles, 4, 5 k_mxfp4_wide */
 int iris_hip_linear_mxfp4_plan(int groups, int rows, int in, int out);
-/* y[rows, out] = x W^T, x and W as codes (16-byte aligned) and scales; first_row NULL: one W for all rows, otherwise as above */
-int iris_hip_linear_mxfp4_f32(void *stream, float *y, const uint8_t *x, const uint8_t *xs, const uint8_t *W, const uint8_t *Ws, const int *first_row, int groups,
-                              int rows, int in, int out);
-int iris_hip_linear_mxfp4_bf16(void *stream, uint16_t *y, const uint8_t *x, const uint8_t *xs, const uint8_t *W, const uint8_t *Ws, const int *first_row,
+/* y[rows, out] = x W^T, x and W as codes (16-byte aligned) and scales; first_row NULL: one W for all rows, otherwise as above.
+ * part: as for the bf16 layers, here for a copy of the scales; NULL: none */
+int iris_hip_linear_mxfp4_f32(void *stream, float *part, float *y, const uint8_t *x, const uint8_t *xs, const uint8_t *W, const uint8_t *Ws, const int *first_row,
+                              int groups, int rows, int in, int out);
+int iris_hip_linear_mxfp4_bf16(void *stream, float *part, uint16_t *y, const uint8_t *x, const uint8_t *xs, const uint8_t *W, const uint8_t *Ws, const int *first_row,
                                int groups, int rows, int in, int out);
 
 /* 1: the tiles normalise themselves, 0: the norm kernel runs behind the layer, -1: not taken; host arithmetic only */

@@ -606,13 +606,13 @@ static int linear_mxfp4_args(const char *what, const void *y, const uint8_t *x, 
 void iris_dev_linear_mxfp4_f32(float *y, const uint8_t *x, const uint8_t *x_scales, const uint8_t *W, const uint8_t *W_scales, int rows, int in, int out) {
     if (!linear_mxfp4_args("linear_mxfp4", y, x, x_scales, W, W_scales, rows, in, out)) return;
     g_last_kernel = "linear_mxfp4";
-    LAUNCH("linear_mxfp4", iris_hip_linear_mxfp4_f32(g_stream, y, x, x_scales, W, W_scales, NULL, 1, rows, in, out));
+    LAUNCH("linear_mxfp4", iris_hip_linear_mxfp4_f32(g_stream, linear_part(), y, x, x_scales, W, W_scales, NULL, 1, rows, in, out));
 }
 
 void iris_dev_linear_mxfp4_bf16(uint16_t *y, const uint8_t *x, const uint8_t *x_scales, const uint8_t *W, const uint8_t *W_scales, int rows, int in, int out) {
     if (!linear_mxfp4_args("linear_mxfp4", y, x, x_scales, W, W_scales, rows, in, out)) return;
     g_last_kernel = "linear_mxfp4";
-    LAUNCH("linear_mxfp4", iris_hip_linear_mxfp4_bf16(g_stream, y, x, x_scales, W, W_scales, NULL, 1, rows, in, out));
+    LAUNCH("linear_mxfp4", iris_hip_linear_mxfp4_bf16(g_stream, linear_part(), y, x, x_scales, W, W_scales, NULL, 1, rows, in, out));
 }
 
 void iris_dev_linear_mxfp4_f32_grouped(float *y, const uint8_t *x, const uint8_t *x_scales, const uint8_t *W, const uint8_t *W_scales, const int *first_row,
@@ -621,7 +621,7 @@ void iris_dev_linear_mxfp4_f32_grouped(float *y, const uint8_t *x, const uint8_t
         !linear_mxfp4_args("linear_mxfp4_grouped", y, x, x_scales, W, W_scales, rows, in, out))
         return;
     g_last_kernel = "linear_mxfp4_grouped";
-    LAUNCH("linear_mxfp4_grouped", iris_hip_linear_mxfp4_f32(g_stream, y, x, x_scales, W, W_scales, first_row, groups, rows, in, out));
+    LAUNCH("linear_mxfp4_grouped", iris_hip_linear_mxfp4_f32(g_stream, linear_part(), y, x, x_scales, W, W_scales, first_row, groups, rows, in, out));
 }
 
 void iris_dev_linear_mxfp4_bf16_grouped(uint16_t *y, const uint8_t *x, const uint8_t *x_scales, const uint8_t *W, const uint8_t *W_scales, const int *first_row,
@@ -630,7 +630,7 @@ void iris_dev_linear_mxfp4_bf16_grouped(uint16_t *y, const uint8_t *x, const uin
         !linear_mxfp4_args("linear_mxfp4_grouped", y, x, x_scales, W, W_scales, rows, in, out))
         return;
     g_last_kernel = "linear_mxfp4_grouped";
-    LAUNCH("linear_mxfp4_grouped", iris_hip_linear_mxfp4_bf16(g_stream, y, x, x_scales, W, W_scales, first_row, groups, rows, in, out));
+    LAUNCH("linear_mxfp4_grouped", iris_hip_linear_mxfp4_bf16(g_stream, linear_part(), y, x, x_scales, W, W_scales, first_row, groups, rows, in, out));
 }
 
 void iris_dev_layer_norm_mod(uint16_t *out, const float *x, const float *shift, const float *scale,

@@ -299,6 +299,53 @@ def test_wide_tiles_at_any_width(dev, sizes, k, n, out):
     check_exact(got, np.concatenate([x[first[g]:first[g + 1]] @ w[g].T for g in range(groups)]), out)
 
 
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("k", [257, 290, 480, 897, 1504, 3793])
+@pytest.mark.parametrize("sizes", [[1301], [700, 0, 601], [1, 1300]])
+def test_wide_tiles_of_rows_of_any_length(dev, sizes, k, out):
+    """The last k tile is the last eight blocks of a row, of which some have been multiplied before: a NaN among those stays in its row, and values of
+    large and small scales are added once"""
+    rows, groups, n = sum(sizes), len(sizes), 4007
+    assert plan_of(groups, rows, k, n, out) >= 4
+    rng = np.random.default_rng(k)
+    cx, sx = exact_inputs(rng, rows, k)
+    cw, sw = exact_inputs(rng, groups * n, k)
+    first = np.concatenate([[0], np.cumsum(sizes)])
+    nb = sx.size // rows
+    sx = sx.reshape(rows, nb).copy()
+    sx[3, nb - 8] = 255                                            # blocks that the last k tile holds for a second time
+    sx[4] += 100
+    sx[5] -= 60
+    got = run_layer(dev, cx, sx, cw, sw, rows, k, n, out, first if groups > 1 else None)
+    sx[3, nb - 8] = 127
+    x, w = mx.decode(cx, sx, k), mx.decode(cw, sw, k).reshape(groups, n, k)
+    want = np.concatenate([x[first[g]:first[g + 1]] @ w[g].T for g in range(groups)])
+    assert np.isnan(got[3]).all()
+    keep = np.arange(rows) != 3
+    check_exact(got[keep], want[keep], out)
+
+
+@pytest.mark.parametrize("off", [1, 2, 4])
+@pytest.mark.parametrize("k", [256, 288, 1024])
+def test_wide_tiles_with_scales_that_start_anywhere(dev, k, off):
+    rows, n = 1301, 4007
+    rng = np.random.default_rng(off)
+    cx, sx = exact_inputs(rng, rows, k)
+    cw, sw = exact_inputs(rng, n, k)
+
+    def shifted(a):
+        d = dev.alloc(a.nbytes + 16)
+        dev.lib.iris_dev_upload(ptr_add(d, off), a.ctypes.data, a.nbytes)
+        return ptr_add(d, off)
+
+    y = dev.put(np.full(rows * n, 7.0, np.float32))
+    dev.lib.iris_dev_linear_mxfp4_f32(y, dev.put(cx), shifted(sx), dev.put(cw), shifted(sw), rows, k, n)
+    dev.check()
+    got = dev.get(y, (rows, n), np.float32)
+    dev.free_all()
+    check_exact(got, mx.decode(cx, sx, k) @ mx.decode(cw, sw, k).T, "f32")
+
+
 @pytest.mark.parametrize("rows,k,n", [(3, 1024, 64), (70, 1024, 512), (300, 768, 512), (500, 512, 16384)])
 @pytest.mark.parametrize("off", [1, 2, 3, 4, 8])
 def test_scales_and_results_that_start_anywhere(dev, rows, k, n, off):
