@@ -176,3 +176,41 @@ def test_layers_of_the_two_kinds_read_the_same_rows(dev):
     dev.check()
     assert np.array_equal(dev.get(y1, (rows, n), np.float32), dev.get(y2, (rows, n), np.float32))
     dev.free_all()
+
+
+def test_captured_layer_beside_eager_ones_that_copy_scales_into_the_workspace(dev):
+    """Rows that are no whole k tiles long: eager, the layer copies its scales into the workspace of the linear layers; captured it must not"""
+    import iris_c_amd
+    rows, n, layers = 1000, 5001, []
+    lib = dev.lib
+    for k in (900, 1300):
+        assert iris_c_amd.load().iris_hip_linear_mxfp4_plan(1, rows, k, n) >= 4
+        rng = np.random.default_rng(k)
+        cx, sx = mx.random_codes(rng, rows, k, 126, 128)
+        cw, sw = mx.random_codes(rng, n, k, 126, 128)
+        layers.append((dev.put(cx), dev.put(sx), dev.put(cw), dev.put(sw), k, (mx.decode(cx, sx, k) @ mx.decode(cw, sw, k).T).astype(np.float32)))
+    y1, y2 = dev.alloc(rows * n * 4), dev.alloc(rows * n * 4)
+    call = lambda y, layer: lib.iris_dev_linear_mxfp4_f32(y, *layer[:4], rows, layer[4], n)  # noqa: E731
+    for layer in layers:                                              # one behind the other through one workspace
+        call(y1, layer)
+        call(y2, layers[0])
+        dev.check()
+        assert np.array_equal(dev.get(y1, (rows, n), np.float32), layer[5]) and np.array_equal(dev.get(y2, (rows, n), np.float32), layers[0][5])
+    g = Graphs()
+    other = _vp()
+    assert g.rt.hipStreamCreate(C.byref(other)) == 0
+    run = g.capture(_vp(lib.iris_dev_stream()), lambda: call(y1, layers[0]))
+    for _ in range(4):
+        for y in (y1, y2):
+            junk = np.full(rows * n, 3.0, np.float32)
+            lib.iris_dev_upload(y, junk.ctypes.data, junk.nbytes)
+        assert g.rt.hipGraphLaunch(run, other) == 0
+        for _ in range(3):
+            call(y2, layers[1])
+        assert g.rt.hipStreamSynchronize(other) == 0
+        lib.iris_dev_sync()
+        dev.check()
+        assert np.array_equal(dev.get(y1, (rows, n), np.float32), layers[0][5]) and np.array_equal(dev.get(y2, (rows, n), np.float32), layers[1][5])
+    g.rt.hipGraphExecDestroy(run)
+    g.rt.hipStreamDestroy(other)
+    dev.free_all()
