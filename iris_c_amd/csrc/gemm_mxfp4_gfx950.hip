@@ -44,10 +44,10 @@ __device__ __forceinline__ void store4(uint16_t *p, f32x4 v, int n_left) {
     if (n_left >= 4 && ((uintptr_t)p & 7) == 0) { *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])); return; }
     for (int r = 0; r < 4 && r < n_left; r++) p[r] = (uint16_t)(pack_bf16(v[r], 0.0f) & 0xffffu);
 }
-/* 16 bytes of results at p, of which the row has `left` values. Where all rows are aligned, and so none ends inside 16 bytes, through the L2s or with the
- * streaming hint; otherwise plainly (parts of lines are better put together in the L2s: 777 x 1000 -> 1111 5.2 us, 6.3 through them) or with the hint,
- * as one store whatever the alignment, and single values at the end of a row. */
-enum Store { THROUGH, STREAMING, PLAIN_ANY, STREAMING_ANY };
+/* 16 bytes of results at p, of which the row has `left` values. THROUGH the L2s or STREAMING where all rows are aligned, and so none ends inside 16 bytes. ANY:
+ * one plain store whatever the alignment (parts of lines are better put together in the L2s: 777 x 1000 -> 1111 5.2 us, 6.3 through them), single values
+ * at the end of a row. */
+enum Store { THROUGH, STREAMING, ANY };
 typedef i32x4 i32x4_at2 __attribute__((aligned(2)));           /* at an address that suits one value */
 template <Store KIND> using Kind = std::integral_constant<Store, KIND>;
 template <Store KIND, typename OUT>
@@ -58,8 +58,7 @@ __device__ __forceinline__ void store16(OUT *p, i32x4 v, int left) {
     } else if constexpr (KIND == STREAMING) {
         __builtin_nontemporal_store(v, reinterpret_cast<i32x4 *>(p));
     } else if (left >= VALUES) {
-        if constexpr (KIND == STREAMING_ANY) __builtin_nontemporal_store(v, reinterpret_cast<i32x4_at2 *>(p));
-        else *reinterpret_cast<i32x4_at2 *>(p) = v;
+        *reinterpret_cast<i32x4_at2 *>(p) = v;
     } else {
 #pragma unroll
         for (int i = 0; i < VALUES - 1; i++)
@@ -427,8 +426,9 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
                     if (c < 4 * NA && m < m_end && n < N) store16<decltype(kind)::value>(y + (size_t)m * N + n, v, N - n);
                 }
             };
-            if (aligned) store(Kind<STREAM ? STREAMING : THROUGH>{});
-            else store(Kind<STREAM ? STREAMING_ANY : PLAIN_ANY>{});
+            if constexpr (STREAM) store(Kind<STREAMING>{});
+            else if (aligned) store(Kind<THROUGH>{});
+            else store(Kind<ANY>{});
         }
     } else {
         uint16_t *buf = reinterpret_cast<uint16_t *>(mine);    /* 64 rows x 128 bf16, chunk c of row r in slot c ^ (r % 16) */
@@ -448,8 +448,9 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
                 if (c < 2 * NA && m < m_end && n < N) store16<decltype(kind)::value>(y + (size_t)m * N + n, v, N - n);
             }
         };
-        if (aligned) store(Kind<STREAM ? STREAMING : THROUGH>{});
-        else store(Kind<STREAM ? STREAMING_ANY : PLAIN_ANY>{});
+        if constexpr (STREAM) store(Kind<STREAMING>{});
+        else if (aligned) store(Kind<THROUGH>{});
+        else store(Kind<ANY>{});
     }
 }
 
@@ -690,7 +691,7 @@ k_mxfp4_tiles(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t 
         }
     };
     if (aligned) store(Kind<THROUGH>{});
-    else store(Kind<PLAIN_ANY>{});
+    else store(Kind<ANY>{});
 }
 #pragma clang diagnostic pop
 
@@ -722,14 +723,14 @@ long tiles_at_most(int M, int N, int groups, int tm, int tn) {
  * keeps the operands. us, plain / through, and with the conversion of the result to MXFP4 behind: 512 x 2560 -> 19456 19.0 / 18.2 and 25.2 / 24.6,
  * 2115 x 4096 -> 4096 25.2 / 24.4 and 30.8 / 29.9, 1000 x 1024 -> 9216 11.7 / 10.4 and 17.6 / 16.9, 300 x 512 -> 4096 6.0 / 6.0 and 10.4 / 10.2. Plain / streaming:
  * 4608 x 4096 -> 36864 (340 MB) 360 / 341 and 427 / 419, -> 12288 (113 MB) 147 / 122 and 171.5 / 170.7, -> 10240 (94 MB) with the conversion
- * 121.8 / 122.6, -> 8192 107.7 / 110.7. Kernels of their own: of a test in front of two stores to one place the compiler keeps one, the plain one. */
+ * 121.8 / 122.6, -> 8192 107.7 / 110.7; unaligned rows not: 4608 x 2560 -> 16001 130 / 142. Kernels of their own: of a test in front of two stores to one place the compiler keeps one, the plain one. */
 constexpr size_t STREAM_BYTES = (size_t)100 << 20;
 
 /* part: room for the copy of the scales, NULL where they can be read as they are */
 template <typename OUT, int NA, bool GROUPED, bool STREAM = false>
 int launch_wide(hipStream_t st, void *part, KERNEL_PARAMS) {
     if constexpr (!STREAM)
-        if ((size_t)M * N * sizeof(OUT) >= STREAM_BYTES) return launch_wide<OUT, NA, GROUPED, true>(st, part, KERNEL_ARGS);
+        if ((size_t)M * N * sizeof(OUT) >= STREAM_BYTES && N % (16 / sizeof(OUT)) == 0 && ((uintptr_t)y & 15) == 0) return launch_wide<OUT, NA, GROUPED, true>(st, part, KERNEL_ARGS);
     using T = Wide<NA>;
     static bool configured = false;
     if (!configured) {
