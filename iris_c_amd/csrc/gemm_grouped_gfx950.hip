@@ -151,8 +151,11 @@ k_grouped_any(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_
  * multiplied; in the last step of a row that is no multiple of 32 U long, chunks past the end are zeros.
  *
  * Rows of an odd K start in the middle of 4 bytes every second time, and 16-byte loads from there take four times as long. HALVES: whole 4 bytes are loaded
- * instead, from those in which a run of values starts (half: 1 if in their middle) to those in which it ends, and shifted in registers. us, groups of 3, 4 and 1 rows, 8001 -> 1001, in 16-byte loads from anywhere 34.8, shifted 15.6 (8002 -> 1001 14.0); of 70 and 81 rows, 2817 -> 2661,
- * two blocks of columns, 104 / 42. (k_grouped_any loses by it: 2 x 1000 rows, 2561 -> 2561 88 / 101.) */
+ * instead, from those in which a run of values starts (half: 1 if in their middle) to those in which it ends, and shifted in registers. us,
+ * groups of 3, 4 and 1 rows, 8001 -> 1001, in 16-byte loads from anywhere 34.8, shifted 15.6 (8002 -> 1001 14.0); of 70 and 81 rows, 2817 -> 2661,
+ * two blocks of columns, 104 / 42. (k_grouped_any loses by it: 2 x 1000 rows, 2561 -> 2561 88 / 101.)
+ *
+ * Bound by HBM: 16 rows over 128 groups, 2560 -> 1536 (126 MB) 26 us. */
 __device__ __forceinline__ int half(const uint16_t *p) { return (int)((uintptr_t)p >> 1 & 1); }
 __device__ __forceinline__ u32x4 load_run(const uint16_t *p, int half) { return *reinterpret_cast<const u32x4_at4 *>(p - half); }
 __device__ __forceinline__ uint32_t load_end(const uint16_t *end, int half) { return *reinterpret_cast<const uint32_t *>(end - 2 + half); }
