@@ -16,6 +16,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "half_words.h"
 #include "iris_kernels_hip.h"
 #include "row_groups.h"
 
@@ -151,14 +152,14 @@ k_grouped_any(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_
  * multiplied; in the last step of a row that is no multiple of 32 U long, chunks past the end are zeros.
  *
  * Rows of an odd K start in the middle of 4 bytes every second time, and 16-byte loads from there take four times as long. HALVES: whole 4 bytes are loaded
- * instead, from those in which a run of values starts (half: 1 if in their middle) to those in which it ends, and shifted in registers. us,
+ * instead, from those in which a run of values starts (half: 1 if in their middle) to those in which it ends, and shifted in registers, but for the steps
+ * whose words would reach past the matrices (half_words.h), which are loaded as the last step is. us,
  * groups of 3, 4 and 1 rows, 8001 -> 1001, in 16-byte loads from anywhere 34.8, shifted 15.6 (8002 -> 1001 14.0); of 70 and 81 rows, 2817 -> 2661,
  * two blocks of columns, 104 / 42. (k_grouped_any loses by it: 2 x 1000 rows, 2561 -> 2561 88 / 101.)
  *
  * Bound by HBM: 16 rows over 128 groups, 2560 -> 1536 (126 MB) 26 us. */
-__device__ __forceinline__ int half(const uint16_t *p) { return (int)((uintptr_t)p >> 1 & 1); }
-__device__ __forceinline__ u32x4 load_run(const uint16_t *p, int half) { return *reinterpret_cast<const u32x4_at4 *>(p - half); }
-__device__ __forceinline__ uint32_t load_end(const uint16_t *end, int half) { return *reinterpret_cast<const uint32_t *>(end - 2 + half); }
+__device__ __forceinline__ u32x4 load_run(const uint16_t *p, int half) { return *reinterpret_cast<const u32x4_at4 *>(run_start(p, half)); }
+__device__ __forceinline__ uint32_t load_end(const uint16_t *end, int half) { return *reinterpret_cast<const uint32_t *>(run_last(end, half)); }
 __device__ __forceinline__ u32x4 shifted(u32x4 v, uint32_t behind, int bits) {
     return u32x4{__builtin_amdgcn_alignbit(v[1], v[0], bits), __builtin_amdgcn_alignbit(v[2], v[1], bits), __builtin_amdgcn_alignbit(v[3], v[2], bits),
                  __builtin_amdgcn_alignbit(behind, v[3], bits)};
@@ -227,10 +228,16 @@ k_grouped_rows(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16
             for (int i = 0; i < A; i++)
                 acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, s.a[u][i]), __builtin_bit_cast(bf16x8, s.b[u]), acc[i], 0, 0, 0);
     };
-    const int steps = (K + 32 * U - 1) / (32 * U), whole = K / (32 * U);
-    const int from = (int)((long)steps * kw / KW), to = (int)((long)steps * (kw + 1) / KW), full = min(to, whole);
+    const HalfSteps inside = HALVES ? half_steps(x, W, K, 32 * U) : HalfSteps{0, K / (32 * U)};
+    const int steps = (K + 32 * U - 1) / (32 * U);
+    const int from = (int)((long)steps * kw / KW), to = (int)((long)steps * (kw + 1) / KW), full = min(to, inside.upto);
     Step s0, s1;
     int at = from;
+    if (HALVES && at < min(inside.first, to)) {
+        fetch_last(s0, at * 32 * U);
+        multiply(s0);
+        at++;
+    }
     if (at < full) {
         fetch(s0, at * 32 * U);
         while (true) {
