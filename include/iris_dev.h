@@ -222,7 +222,8 @@ void iris_dev_linear_bf16_qknorm(uint16_t *y, const uint16_t *x, const uint16_t 
  * that they go to. x [rows, in], y [rows, out], W [groups, out, in], all contiguous; first_row: device int [groups + 1], not
  * decreasing, read when the layer runs. Groups may be empty. Rows of y in front of first_row[0] and from first_row[groups] on stay as
  * they were. A value of first_row below one before it counts as that one, values are limited to 0 .. rows: no call reads or writes
- * outside its matrices. Any sizes and alignment. groups 0 does nothing.
+ * outside its matrices. Any sizes and alignment, but for those that no launch holds (2^32 threads; a thread computes up to 64 results, fewer where groups end
+ * inside tiles), which are reported. groups 0 does nothing.
  * The f32 sums of a row are taken in an order that may differ from the plain layer's; a call gives the same bits every time. */
 void iris_dev_linear_f32_grouped(float *y, const uint16_t *x, const uint16_t *W, const int *first_row,
                                  int groups, int rows, int in, int out);
@@ -245,7 +246,8 @@ void iris_dev_mxfp4_to_f32(float *dst, int ldd, const uint8_t *codes, const uint
 void iris_dev_mxfp4_to_bf16(uint16_t *dst, int ldd, const uint8_t *codes, const uint8_t *scales, int rows, int cols);
 
 /* iris_dev_linear_f32 / _bf16 on rows and weights held in MXFP4: y[rows, out] = x[rows, in] @ W[out, in]^T, f32 accumulation. A last block
- * that `in` ends inside is multiplied as a whole: its zeros are for the caller to keep, as the conversions above do. */
+ * that `in` ends inside is multiplied as a whole: its zeros are for the caller to keep, as the conversions above do. Sizes that no launch holds are
+ * reported, as above. */
 void iris_dev_linear_mxfp4_f32(float *y, const uint8_t *x, const uint8_t *x_scales, const uint8_t *W, const uint8_t *W_scales,
                                int rows, int in, int out);
 void iris_dev_linear_mxfp4_bf16(uint16_t *y, const uint8_t *x, const uint8_t *x_scales, const uint8_t *W, const uint8_t *W_scales,

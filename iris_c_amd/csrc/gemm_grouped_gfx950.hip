@@ -14,6 +14,8 @@
  * LDS where they are many (4000 rows, 4097 -> 4097: 309 us, 435 TFLOP/s; tiles of 64 take 414).
  */
 #include <hip/hip_runtime.h>
+
+#include <cfloat>
 #include <stdint.h>
 
 #include "half_words.h"
@@ -276,7 +278,7 @@ bool halves(const uint16_t *x, const uint16_t *W, int in) { return (in & 1) || (
 template <typename OUT, int A, int U, int KW>
 int launch_rows(hipStream_t st, OUT *y, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int rows, int in, int out) {
     const long wgs = row_tiles_at_most(rows, groups, 16) * ((out + 16L * A - 1) / (16 * A));
-    if (wgs * 64 * KW >> 32) return (int)hipErrorInvalidValue;  /* a launch has fewer than 2^32 threads */
+    if (!launch_fits(wgs, 64 * KW)) return (int)hipErrorInvalidValue;
     const dim3 grid((unsigned)(wgs + 7) / 8 * 8), block(64 * KW);
     if (halves(x, W, in)) hipLaunchKernelGGL((k_grouped_rows<OUT, A, U, KW, true>), grid, block, 0, st, y, x, W, rows, out, in, first_row, groups);
     else hipLaunchKernelGGL((k_grouped_rows<OUT, A, U, KW, false>), grid, block, 0, st, y, x, W, rows, out, in, first_row, groups);
@@ -286,7 +288,7 @@ int launch_rows(hipStream_t st, OUT *y, const uint16_t *x, const uint16_t *W, co
 template <typename OUT, int B>
 int launch_any(hipStream_t st, OUT *y, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int rows, int in, int out) {
     const long wgs = row_tiles_at_most(rows, groups, 32 * B) * ((out + 32L * B - 1) / (32 * B));
-    if (wgs * 256 >> 32) return (int)hipErrorInvalidValue;
+    if (!launch_fits(wgs, 256)) return (int)hipErrorInvalidValue;
     hipLaunchKernelGGL((k_grouped_any<OUT, B>), dim3((unsigned)wgs), dim3(256), 0, st, y, x, W, rows, out, in, first_row, groups);
     return (int)hipGetLastError();
 }
@@ -297,14 +299,17 @@ int launch_any(hipStream_t st, OUT *y, const uint16_t *x, const uint16_t *W, con
  * where they come from a cache (its loads are 16 rows of 64 bytes each) and 5 TB/s from HBM, the tiles at 4.7 from HBM. us, k_grouped_rows / the
  * best tiles: 16 groups of 8 rows, 2560 -> 2560 43.5 / 48.5, of 16 49.6 / 47.7, of 17 74.9 / 48.8, of 64 139 / 50; 4 groups of 1024 -> 1024, 1 row each 3.9 / 8.8,
  * 30 5.8 / 8.8, 64 8.6 / 10.0; 2 groups of 2560 -> 6144, 16 rows 16 / 17.5, 32 22.8 / 17.8. Two blocks of columns a wave halve the reads of x where there are
- * enough workgroups: the 16 groups 57.8 / 46.0 at 12 rows, but 1 row in each of 4 3.9 / 4.7. */
+ * enough workgroups: the 16 groups 57.8 / 46.0 at 12 rows, but 1 row in each of 4 3.9 / 4.7. Kernels whose grid could pass the limit of a launch are left
+ * out: k_grouped_rows has a thread for every 8 - 16 results, and k_grouped_any for every 16 - 64. (The tiles' operands fill the memory before theirs could.) */
 struct Plan { int kernel, shape, splits; };
 Plan plan_grouped(int groups, int rows, int in, int out, int out_size, bool aligned16, bool halves, size_t part_bytes) {
     const long some = groups < rows ? groups : rows, few_tiles = row_tiles_about(rows, groups, 16);
     const float weights = (float)out * (float)in * 2.0f, every = (float)some * weights;
     const float cached = (float)few_tiles * weights / (halves ? 4.2e6f : 6.0e6f), fresh = every / 5.0e6f;
+    auto fits = [&](int tm, int tn) { return launch_fits(row_tiles_at_most(rows, groups, tm) * ((out + tn - 1L) / tn), 256); };
     float best = 3.0f + (cached > fresh ? cached : fresh);
     Plan plan = {1, few_tiles * ((out + 31L) / 32) >= 512 ? 2 : 1, 1};
+    if (!fits(16, 16 * plan.shape)) { best = FLT_MAX; plan = {0, 4, 1}; }
     const float least = 4.0f + every / 4.7e6f;                 /* of the tiles */
     if (aligned16) {
         int shape = 0, splits = 1;
@@ -319,7 +324,7 @@ Plan plan_grouped(int groups, int rows, int in, int out, int out_size, bool alig
         const float alone = blocks == 2 ? 0.62f : 1.1f, share = blocks == 2 ? 0.42f : 1.08f;
         const long wgs = row_tiles_about(rows, groups, tile) * ((out + tile - 1L) / tile);
         const float each = share * (float)((wgs + 255) / 256), us = 5.0f + (float)((in + 63) / 64) * (each > alone ? each : alone);
-        if (us < best) { best = us; plan = {0, blocks, 1}; }
+        if (us < best && fits(tile, tile)) { best = us; plan = {0, blocks, 1}; }
     }
     return plan;
 }

@@ -15,6 +15,7 @@
  */
 #include <hip/hip_runtime.h>
 
+#include <cfloat>
 #include <climits>
 #include <stdint.h>
 #include <type_traits>
@@ -745,7 +746,7 @@ int launch_wide(hipStream_t st, void *part, KERNEL_PARAMS) {
         configured = true;
     }
     const long most = tiles_at_most<GROUPED>(M, N, groups, T::TM, T::TN);
-    if (most * 512 >> 32) return (int)hipErrorInvalidValue;     /* a launch has fewer than 2^32 threads */
+    if (!launch_fits(most, 512)) return (int)hipErrorInvalidValue;
     if (part) {
         const size_t all = (size_t)M + (size_t)groups * N, nk = (size_t)(nb + 7) / 8;
         hipLaunchKernelGGL(k_mxfp4_scales, dim3((unsigned)((all * nk + 255) / 256)), dim3(256), 0, st, (uint64_t *)part, xs, Ws, M, all, nb);
@@ -769,7 +770,7 @@ int launch_tiles(hipStream_t st, KERNEL_PARAMS) {
         configured = true;
     }
     const long most = tiles_at_most<GROUPED>(M, N, groups, T::TM, T::TN);
-    if (most * T::THREADS >> 32) return (int)hipErrorInvalidValue;
+    if (!launch_fits(most, T::THREADS)) return (int)hipErrorInvalidValue;
     hipLaunchKernelGGL((k_mxfp4_tiles<OUT, NB, NA, WM, WN, KG, STAGES, TAIL, GROUPED>), dim3((unsigned)(most + 7) / 8 * 8), dim3(T::THREADS), T::LDS, st, KERNEL_ARGS);
     return (int)hipGetLastError();
 }
@@ -777,7 +778,7 @@ int launch_tiles(hipStream_t st, KERNEL_PARAMS) {
 template <typename OUT, int A, bool GROUPED>
 int launch_rows(hipStream_t st, KERNEL_PARAMS) {
     const long most = tiles_at_most<GROUPED>(M, N, groups, 16, 16 * A);
-    if (most * 64 * ROWS_KW >> 32) return (int)hipErrorInvalidValue;
+    if (!launch_fits(most, 64 * ROWS_KW)) return (int)hipErrorInvalidValue;
     hipLaunchKernelGGL((k_mxfp4_rows<OUT, A, GROUPED>), dim3((unsigned)(most + 7) / 8 * 8), dim3(64 * ROWS_KW), 0, st, KERNEL_ARGS);
     return (int)hipGetLastError();
 }
@@ -787,9 +788,9 @@ int launch_rows(hipStream_t st, KERNEL_PARAMS) {
  * 190 sizes (1 - 4608 rows, 512 -> 512 to 16384 -> 1024 and 2560 -> 19456): what is chosen takes 1.7 % longer on average than the best of 17 tiles,
  * 20 % at worst. us, best others / chosen: 512 x 9728 -> 2560 (64 x 128) 23.2 / 18.3, 64 x 9728 -> 2560 (32 x 32) 11.2 / 8.8, 512 x 4096 ->
  * 12288 (256 x 192) 30.8 / 23.2, 2115 x 4096 -> 12288 (256 x 256) 73.4 / 61.6. */
-struct Shape { int tm, tn, resident; float fixed, step, share, again; };
-constexpr Shape SHAPES[] = {{32, 32, 4, 3.36f, 0.129f, 0.098f, 1.6f},   {64, 64, 2, 3.87f, 0.257f, 0.214f, 2.5f},  {64, 128, 1, 4.16f, 0.344f, 0.354f, 3.2f},
-                            {128, 128, 1, 4.85f, 0.205f, 0.455f, 5.5f}, {256, 192, 1, 5.0f, 0.326f, 0.973f, 6.0f}, {256, 256, 1, 5.16f, 0.635f, 1.22f, 6.0f}};
+struct Shape { int tm, tn, threads, resident; float fixed, step, share, again; };
+constexpr Shape SHAPES[] = {{32, 32, 256, 4, 3.36f, 0.129f, 0.098f, 1.6f},   {64, 64, 256, 2, 3.87f, 0.257f, 0.214f, 2.5f},  {64, 128, 256, 1, 4.16f, 0.344f, 0.354f, 3.2f},
+                            {128, 128, 512, 1, 4.85f, 0.205f, 0.455f, 5.5f}, {256, 192, 512, 1, 5.0f, 0.326f, 0.973f, 6.0f}, {256, 256, 512, 1, 5.16f, 0.635f, 1.22f, 6.0f}};
 constexpr int NSHAPES = sizeof(SHAPES) / sizeof(SHAPES[0]), FIRST_WIDE = 4;
 
 /* -1 and -2: k_mxfp4_rows with that many blocks of columns, 0 - 3: k_mxfp4_tiles, 4 and 5: k_mxfp4_wide, in the order of SHAPES. whole: rows of whole k tiles
@@ -810,6 +811,9 @@ int plan_mxfp4(int groups, int M, int N, int nb, bool whole, size_t part_bytes) 
     if (best < 2.2f + fresh) best = 2.2f + fresh;
     /* two blocks of columns: 40 rows over 64 weight matrices of 2560 -> 1536 13.9 us with one, 12.7 with two; 1 row, 4096 -> 4096 3.7 / 4.9 */
     int plan = row_tiles(16) * ((N + 31L) / 32) >= 512 ? -2 : -1;
+    /* kernels whose grid could pass the limit of a launch are left out */
+    auto fits = [&](int tm, int tn, int threads) { return launch_fits(row_tiles_at_most(M, groups, tm) * ((N + tn - 1L) / tn), threads); };
+    if (!fits(16, -16 * plan, 64 * ROWS_KW)) best = FLT_MAX;
     /* the tiles' offsets inside a tile of rows have 32 bits */
     for (int i = 0; i < (nb >> 20 ? 0 : wide ? NSHAPES : FIRST_WIDE); i++) {
         const Shape &s = SHAPES[i];
@@ -819,7 +823,7 @@ int plan_mxfp4(int groups, int M, int N, int nb, bool whole, size_t part_bytes) 
         float us = s.fixed + (float)((nb + 7) / 8) * step * (slower ? 1.3f : 1.0f) + (float)(rounds - 1) * s.again * (slower ? 2.0f : 1.0f);
         if (us < s.fixed + fresh) us = s.fixed + fresh;
         if (i >= FIRST_WIDE) us += first;
-        if (us < best) { best = us; plan = i; }
+        if (us < best && fits(s.tm, s.tn, s.threads)) { best = us; plan = i; }
     }
     return plan;
 }

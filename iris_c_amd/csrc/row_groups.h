@@ -93,4 +93,7 @@ static inline long row_tiles_about(int rows, int groups, int height) {
     return filled > some ? filled : some;
 }
 
+/* a launch has fewer than 2^32 threads: whether `wgs` workgroups, rounded up to as many for every XCD, can be one */
+static inline bool launch_fits(long wgs, int threads) { return (wgs + 7) / 8 * 8 <= ((1L << 32) - 1) / threads; }
+
 #endif
