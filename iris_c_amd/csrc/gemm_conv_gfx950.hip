@@ -468,7 +468,7 @@ struct Wide {
 template <typename OUT, int NA, bool QKN, bool GROUPED>
 __global__ void __launch_bounds__(512, 2)
 k_gemm_wide(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t *__restrict__ W, int M, int N, int K,
-            int tiles_m, int total, int per_xcd, int turns, QkNorm qn, const float *__restrict__ bias, int streaming_out, RowGroupsArg grouped) {
+            int tiles_m, int total, int per_xcd, int turns, QkNorm qn, const float *__restrict__ bias, RowGroupsArg grouped) {
     using T = Wide<NA>;
     constexpr int TM = T::TM, TN = T::TN, XS = T::XS, WS = T::WS, WP = T::WP, H0 = (NA + 1) / 2, H1 = NA / 2;
     static_assert(WP <= 4 && H1 >= 2, "");
@@ -682,9 +682,7 @@ k_gemm_wide(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t 
                 f32x4 v = *reinterpret_cast<const f32x4 *>(&buf[row * 128 + 4 * ((c & 16) | ((c ^ row) & 15))]);
                 if (c < 4 * NA && m < m_end && n < N) {
                     if (bias) v += *reinterpret_cast<const f32x4 *>(bias + n);
-                    f32x4 *dst = reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(y) + (size_t)m * N + n);
-                    if (streaming_out) __builtin_nontemporal_store(v, dst);
-                    else *dst = v;
+                    *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(y) + (size_t)m * N + n) = v;
                 }
             }
         }
@@ -702,11 +700,7 @@ k_gemm_wide(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t 
         for (int it = 0; it < 16; it++) {
             const int row = 4 * it + (lane >> 4), c = lane & 15, m = mw + row, n = nw + PER16 * c;
             const u32x4 v = *reinterpret_cast<const u32x4 *>(&buf[row * 128 + 8 * (c ^ (row & 15))]);
-            if (c < 2 * NA && m < m_end && n < N) {
-                u32x4 *dst = reinterpret_cast<u32x4 *>(reinterpret_cast<uint16_t *>(y) + (size_t)m * N + n);
-                if (streaming_out) __builtin_nontemporal_store(v, dst);
-                else *dst = v;
-            }
+            if (c < 2 * NA && m < m_end && n < N) *reinterpret_cast<u32x4 *>(reinterpret_cast<uint16_t *>(y) + (size_t)m * N + n) = v;
         }
     }
 }
@@ -762,13 +756,8 @@ int launch_gemm_wide(hipStream_t st, OUT *y, const uint16_t *x, const uint16_t *
     const int tiles_m = GROUPED ? (int)row_tiles_at_most(M, grouped.groups, DT) : (M + DT - 1) / DT, tiles_n = (N + 32 * NA - 1) / (32 * NA),
               total = tiles_m * tiles_n;
     const int per_xcd = (total + 7) / 8;
-    /* An output of 192 MB or more cannot stay in the 256 MB Infinity Cache next to the operands: stored with the
-     * streaming hint it does not push the weights out on its way (4608 x 3072 -> 27648: f32 output 671 -> 626 us, bf16
-     * 594 -> 585 when it was introduced; smaller outputs are within 1 % either way and keep the plain stores, which leave
-     * them cached for the operator that reads them next). */
-    const int streaming_out = (size_t)M * N * sizeof(OUT) >= ((size_t)192 << 20);
     hipLaunchKernelGGL((k_gemm_wide<OUT, NA, QKN, GROUPED>), dim3((unsigned)per_xcd * 8), dim3(512), Wide<NA>::LDS, st, y, x, W, M, N, K,
-                       tiles_m, total, per_xcd, in_order ? 0 : iris_hip_gemm_turns(wide_wgs(M, N, 8), (size_t)N * K * 2), qn, bias, streaming_out, grouped);
+                       tiles_m, total, per_xcd, in_order ? 0 : iris_hip_gemm_turns(wide_wgs(M, N, 8), (size_t)N * K * 2), qn, bias, grouped);
     return (int)hipGetLastError();
 }
 
