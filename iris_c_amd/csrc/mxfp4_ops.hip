@@ -179,9 +179,11 @@ k_mxfp4_to(T *__restrict__ dst, int ld, const uint32_t *__restrict__ codes, cons
     }
 }
 
-/* Values of 64 MB and more are read, of 100 MB and more written, with the streaming hint, past the Infinity Cache (256 MB): they do not all stay there, and the
- * codes, which are read next, do. There and back, us, plain / streaming: 4608 x 16384 bf16 74.1 / 61.8 (6.2 TB/s with the codes),
- * 4608 x 8192 40.3 / 34.6, f32 there and bf16 back 48.9 / 48.7; with both hints 4608 x 4096 18.8 / 19.7. */
+/* Values of 2 bytes: 64 MB and more are read, 100 MB and more written, with the streaming hint, past the Infinity Cache (256 MB): they do not all stay there, and
+ * the codes, which are read next, do. There and back, us, plain / streaming: 4608 x 16384 bf16 74.1 / 61.8 (6.2 TB/s with the codes), 4608 x 8192 40.3 / 34.6; with
+ * both hints 4608 x 4096 18.8 / 19.7. Not f32, where a thread's 8 values are two accesses of 16 bytes, 32 bytes apart in neighbouring lanes, and with the hint the halves
+ * of a line go their own ways. To codes, 1024 x 16384 12.4 / 15.4, 4608 x 16384 61.8 / 64.8 (and 2304 x 16384 with bf16 back 48.9 / 49.0); from codes, 1600 x 16384
+ * 28.5 / 39.9, 4608 x 16384 78.0 / 121 (4.4 TB/s with the codes), 3001 x 16381 62 / 78. */
 constexpr size_t STREAM_READ = (size_t)64 << 20, STREAM_WRITE = (size_t)100 << 20;
 
 template <typename T, bool STREAM>
@@ -205,13 +207,15 @@ int launch_from(void *stream, T *dst, int ld, const uint8_t *codes, const uint8_
 
 template <typename T>
 int to_mxfp4(void *stream, uint8_t *codes, uint8_t *scales, const T *src, int ld, int rows, int cols) {
-    return (size_t)rows * cols * sizeof(T) >= STREAM_READ ? launch_to<T, true>(stream, codes, scales, src, ld, rows, cols)
-                                                          : launch_to<T, false>(stream, codes, scales, src, ld, rows, cols);
+    if constexpr (sizeof(T) == 2)
+        if ((size_t)rows * cols * sizeof(T) >= STREAM_READ) return launch_to<T, true>(stream, codes, scales, src, ld, rows, cols);
+    return launch_to<T, false>(stream, codes, scales, src, ld, rows, cols);
 }
 template <typename T>
 int mxfp4_to(void *stream, T *dst, int ld, const uint8_t *codes, const uint8_t *scales, int rows, int cols) {
-    return (size_t)rows * cols * sizeof(T) >= STREAM_WRITE ? launch_from<T, true>(stream, dst, ld, codes, scales, rows, cols)
-                                                           : launch_from<T, false>(stream, dst, ld, codes, scales, rows, cols);
+    if constexpr (sizeof(T) == 2)
+        if ((size_t)rows * cols * sizeof(T) >= STREAM_WRITE) return launch_from<T, true>(stream, dst, ld, codes, scales, rows, cols);
+    return launch_from<T, false>(stream, dst, ld, codes, scales, rows, cols);
 }
 
 }  // namespace
