@@ -154,8 +154,8 @@ k_grouped_any(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_
  * multiplied; in the last step of a row that is no multiple of 32 U long, chunks past the end are zeros.
  *
  * Rows of an odd K start in the middle of 4 bytes every second time, and 16-byte loads from there take four times as long. HALVES: whole 4 bytes are loaded
- * instead, from those in which a run of values starts (half: 1 if in their middle) to those in which it ends, and shifted in registers, but for the steps
- * whose words would reach past the matrices (half_words.h), which are loaded as the last step is. us,
+ * instead, from those in which a run of values starts (half: 1 if in their middle) to those in which it ends, and shifted in registers. INSIDE: x or W starts in the middle of
+ * 4 bytes itself; the steps whose words would reach past the matrices (half_words.h) are loaded as the last step is. A kernel of its own: in one for both the others took 5 % longer. us,
  * groups of 3, 4 and 1 rows, 8001 -> 1001, in 16-byte loads from anywhere 34.8, shifted 15.6 (8002 -> 1001 14.0); of 70 and 81 rows, 2817 -> 2661,
  * two blocks of columns, 104 / 42. (k_grouped_any loses by it: 2 x 1000 rows, 2561 -> 2561 88 / 101.)
  *
@@ -167,10 +167,14 @@ __device__ __forceinline__ u32x4 shifted(u32x4 v, uint32_t behind, int bits) {
                  __builtin_amdgcn_alignbit(behind, v[3], bits)};
 }
 
-template <typename OUT, int A, int U, int KW, bool HALVES>
+/* all rows start at 4 bytes; the matrices do, but rows are odd; x or W does not */
+enum Starts { WORDS, HALVES, INSIDE };
+
+template <typename OUT, int A, int U, int KW, Starts STARTS>
 __global__ void __launch_bounds__(64 * KW)
 k_grouped_rows(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_t *__restrict__ W, int M, int N, int K, const int *__restrict__ first_row, int groups) {
     constexpr int TM = 16, TN = 16 * A;
+    constexpr bool SHIFTED = STARTS != WORDS;
     __shared__ __align__(16) f32x4 sums[KW][A][64];
     const int tiles_n = (N + TN - 1) / TN;
     RowGroups<TM> all;
@@ -191,10 +195,10 @@ k_grouped_rows(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16
         for (int u = 0; u < U; u++) {
             const int k = k0 + 8 * (U * lg + u);
 #pragma unroll
-            for (int i = 0; i < A; i++) s.a[u][i] = load_run(wrow[i] + k, HALVES ? half(wrow[i]) : 0);
-            s.b[u] = load_run(xrow + k, HALVES ? half(xrow) : 0);
+            for (int i = 0; i < A; i++) s.a[u][i] = load_run(wrow[i] + k, SHIFTED ? half(wrow[i]) : 0);
+            s.b[u] = load_run(xrow + k, SHIFTED ? half(xrow) : 0);
         }
-        if constexpr (HALVES) {
+        if constexpr (SHIFTED) {
             const int end = k0 + 8 * U * (lg + 1);
 #pragma unroll
             for (int i = 0; i < A; i++) s.a_end[i] = load_end(wrow[i] + end, half(wrow[i]));
@@ -202,7 +206,7 @@ k_grouped_rows(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16
         }
     };
     auto shift = [&](Step &s) {
-        if constexpr (HALVES) {
+        if constexpr (SHIFTED) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
 #pragma unroll
@@ -230,12 +234,12 @@ k_grouped_rows(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16
             for (int i = 0; i < A; i++)
                 acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, s.a[u][i]), __builtin_bit_cast(bf16x8, s.b[u]), acc[i], 0, 0, 0);
     };
-    const HalfSteps inside = HALVES ? half_steps(x, W, K, 32 * U) : HalfSteps{0, K / (32 * U)};
+    const HalfSteps inside = STARTS == INSIDE ? half_steps(x, W, K, 32 * U) : HalfSteps{0, K / (32 * U)};
     const int steps = (K + 32 * U - 1) / (32 * U);
     const int from = (int)((long)steps * kw / KW), to = (int)((long)steps * (kw + 1) / KW), full = min(to, inside.upto);
     Step s0, s1;
     int at = from;
-    if (HALVES && at < min(inside.first, to)) {
+    if (STARTS == INSIDE && at < min(inside.first, to)) {
         fetch_last(s0, at * 32 * U);
         multiply(s0);
         at++;
@@ -273,15 +277,18 @@ k_grouped_rows(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16
     }
 }
 
-bool halves(const uint16_t *x, const uint16_t *W, int in) { return (in & 1) || (((uintptr_t)x | (uintptr_t)W) & 2); }
+bool halves(const uint16_t *x, const uint16_t *W, int in) { return (in & 1) || half(x) || half(W); }
 
 template <typename OUT, int A, int U, int KW>
 int launch_rows(hipStream_t st, OUT *y, const uint16_t *x, const uint16_t *W, const int *first_row, int groups, int rows, int in, int out) {
     const long wgs = row_tiles_at_most(rows, groups, 16) * ((out + 16L * A - 1) / (16 * A));
     if (!launch_fits(wgs, 64 * KW)) return (int)hipErrorInvalidValue;
     const dim3 grid((unsigned)(wgs + 7) / 8 * 8), block(64 * KW);
-    if (halves(x, W, in)) hipLaunchKernelGGL((k_grouped_rows<OUT, A, U, KW, true>), grid, block, 0, st, y, x, W, rows, out, in, first_row, groups);
-    else hipLaunchKernelGGL((k_grouped_rows<OUT, A, U, KW, false>), grid, block, 0, st, y, x, W, rows, out, in, first_row, groups);
+#define ROWS(STARTS) hipLaunchKernelGGL((k_grouped_rows<OUT, A, U, KW, STARTS>), grid, block, 0, st, y, x, W, rows, out, in, first_row, groups)
+    if (half(x) || half(W)) ROWS(INSIDE);
+    else if (in & 1) ROWS(HALVES);
+    else ROWS(WORDS);
+#undef ROWS
     return (int)hipGetLastError();
 }
 
