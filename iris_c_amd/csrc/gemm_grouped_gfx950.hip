@@ -4,14 +4,15 @@
  *   y[m, :] = x[m, :] W[g]^T for the rows m of group g      bf16 inputs, f32 accumulation, f32 or bf16 output
  *
  * Groups of many rows run on the tiles of the plain layers (k_gemm_wide of gemm_conv_gfx950.hip, k_gemm_tiles of gemm_tiles_gfx950.hip, which take
- * their tile's rows and weights from row_groups.h), groups of a few rows on k_grouped_rows below.
+ * their tile's rows and weights from row_groups.h), where rows are a multiple of 64 long, results a multiple of 8 and matrices 16-byte aligned; groups of a
+ * few rows on k_grouped_rows below.
  *
  * k_grouped_any takes every size and alignment: tiles of 64 x 64 or 128 x 128 on 2 x 2 waves, K in steps of 64, two LDS stages of
  * [W tile | x tile] with rows padded to 160 B (the 16 lanes that the LDS serves together on a 128-bit read then fall in distinct bank
  * windows). The next step is put into one stage while the other is multiplied, and the one after it is on its way to registers. Its loads are 16
  * bytes wide at any alignment; where a row of K ends inside one, in the last step, single values are read and zeros stand behind them. Latency bounds it where
  * tiles are few (3556 rows, 1355 -> 256: 18.5 us in tiles of 64, 29.3 of 128, and 65 with one stage and a test at each load), the loads and the
- * LDS where they are many (4000 rows, 4097 -> 4097: 309 us, 435 TFLOP/s; tiles of 64 take 414).
+ * LDS where they are many (4000 rows, 4097 -> 4097: 300 us, 448 TFLOP/s; tiles of 64 take 414).
  */
 #include <hip/hip_runtime.h>
 
@@ -155,11 +156,11 @@ k_grouped_any(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_
  *
  * Rows of an odd K start in the middle of 4 bytes every second time, and 16-byte loads from there take four times as long. HALVES: whole 4 bytes are loaded
  * instead, from those in which a run of values starts (half: 1 if in their middle) to those in which it ends, and shifted in registers. INSIDE: x or W starts in the middle of
- * 4 bytes itself; the steps whose words would reach past the matrices (half_words.h) are loaded as the last step is. A kernel of its own: in one for both the others took 5 % longer. us,
- * groups of 3, 4 and 1 rows, 8001 -> 1001, in 16-byte loads from anywhere 34.8, shifted 15.6 (8002 -> 1001 14.0); of 70 and 81 rows, 2817 -> 2661,
+ * 4 bytes itself; the steps whose words would reach past the matrices (half_words.h) are loaded as the last step is. A kernel of its own: in one for both the others took 5 % longer. us:
+ * groups of 3, 4 and 1 rows, 8001 -> 1001, in 16-byte loads from anywhere 34.8, shifted 16.1 (8002 -> 1001 14.0); of 70 and 81 rows, 2817 -> 2661,
  * two blocks of columns, 104 / 42. (k_grouped_any loses by it: 2 x 1000 rows, 2561 -> 2561 88 / 101.)
  *
- * Bound by HBM: 16 rows over 128 groups, 2560 -> 1536 (126 MB) 26 us. */
+ * Bound by HBM: 16 rows over 128 groups, 2560 -> 1536 (126 MB) 27 us. */
 __device__ __forceinline__ u32x4 load_run(const uint16_t *p, int half) { return *reinterpret_cast<const u32x4_at4 *>(run_start(p, half)); }
 __device__ __forceinline__ uint32_t load_end(const uint16_t *end, int half) { return *reinterpret_cast<const uint32_t *>(run_last(end, half)); }
 __device__ __forceinline__ u32x4 shifted(u32x4 v, uint32_t behind, int bits) {

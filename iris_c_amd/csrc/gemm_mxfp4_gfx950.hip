@@ -10,8 +10,8 @@
  * are neighbouring bytes. As in the bf16 layers the product is issued transposed (A = W rows, B = x rows), so that a lane holds
  * four consecutive n of one output row.
  *
- * Three kernels: k_mxfp4_rows for a few rows (bound by the reading of the weights), k_mxfp4_tiles in four tiles, k_mxfp4_wide in tiles of 256 rows
- * (bound by the chip's power: on random codes its matrix cores alone keep up 6880 TFLOP/s). plan_mxfp4 chooses.
+ * Three kernels: k_mxfp4_rows for a few rows (bound by the reading of the weights), k_mxfp4_tiles in four tiles, k_mxfp4_wide in tiles of 256 rows.
+ * plan_mxfp4 chooses. Times are medians; "from HBM": the weights of more layers in turn than the Infinity Cache (256 MB) holds, otherwise they may be in it.
  */
 #include <hip/hip_runtime.h>
 
@@ -87,8 +87,8 @@ __device__ __forceinline__ f32x16 mfma32(i32x4 a, i32x4 b, f32x16 c, int sa, int
  * A workgroup owns 16 rows x 16 A columns; its KW waves walk a range of K each and add their sums through the LDS, in order. A step is 16 blocks of
  * 32: lane group g of the four holds blocks 4 g .. 4 g + 3, 64 contiguous bytes of its row, four products follow each other, and the
  * scales are the bytes of one register. The operands of the next step are on their way while this one is multiplied. In the last step of a row
- * that is no multiple of 16 blocks long, blocks past the end are zeros with scale 1. Any sizes. Bound by HBM: 1 row, 4096 -> 24576 (54 MB) 10.2 us,
- * 40 rows over 64 groups, 2560 -> 1536 (48 MB) 12.8. */
+ * that is no multiple of 16 blocks long, blocks past the end are zeros with scale 1. Any sizes. Bound by the reading of the weights: 1 row, 4096 -> 24576 (54 MB) 11.6 us
+ * from HBM (4.6 TB/s), 10.4 from the Infinity Cache; 40 rows over 64 groups, 2560 -> 1536 (48 MB) 14.2 and 13.1. */
 constexpr int ROWS_KW = 4;
 typedef uint32_t uint32_at1 __attribute__((aligned(1)));
 
@@ -198,7 +198,7 @@ k_mxfp4_rows(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
  * For k tiles of 256: 128 B of codes and 8 scales of every row. Eight waves, two per
  * SIMD, 4 (rows of 64) x 2 (columns of 16 NA): a wave owns 64 rows x 16 NA columns = NA x 4 accumulator blocks. A k tile is two
  * k-steps of v_mfma_scale_f32_16x16x128: in k-step ks lane group g of the four holds block 2 g + ks of its row, so that its two scales are
- * neighbouring bytes. (32x32x64 products draw more power: on random codes the chip keeps up 6090 TFLOP/s of them and 6880 of these.)
+ * neighbouring bytes. (32x32x64 products draw more power: of registers with random codes the chip keeps up 6600 TFLOP/s of them and 7100 - 7400 of these.)
  *
  * Everything comes from memory straight into the LDS (160 KB at 256 columns): two stages of x, two and a half of W (a ring of five half tiles,
  * the columns of one wave column each), two of scales, which are fetched for two k tiles at a time (16 B a row). 16 B chunk c of row r sits
@@ -212,15 +212,16 @@ k_mxfp4_rows(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
  * products. Requests past the end of K are issued all the same (a branch around each costs more, and the waits count them), but all lanes ask for
  * one 16 B of the last tile, into a stage that nobody reads.
  *
- * Bound by the chip's power, and by the 6 - 7 us of first loads and stores of every round of tiles: 4608 x 4096 -> 36864 335 - 345 us (4.1 PFLOP/s; the matrix cores
- * are busy for half of the cycles, at 1.96 GHz), 512 + 4096 rows in groups -> 12288 122 - 126, 512 x 2560 -> 19456 17.5 - 18.1.
+ * A k tile takes 1.68 us (256 tiles, K 4096 and 12288), its products at the rate above 1.16 - 1.21, and the first loads and the stores of a round of tiles 5.5 more, when nothing
+ * else runs on a CU. 4608 x 4096 -> 36864 357 us (3.9 PFLOP/s; 2592 tiles are 10.1 rounds and take 11; the matrix cores are busy for half of the cycles, at 1.96 of
+ * 2.4 GHz), 512 + 4096 rows in groups -> 12288 128 (from HBM 149), 512 x 2560 -> 19456 18.9 (21.1). f32 results, 4608 x 4096 -> 36864 395.
  *
- * Any number of columns: of an unaligned row the pieces are stored as they lie (4608 x 4096 -> 9001 98 us; with tiles of 128 x 128 165). One k tile
- * is taken too (2327 x 256 -> 16384 24 us; 95).
+ * Any number of columns: of an unaligned row the pieces are stored as they lie (bf16 results, 4608 x 4096 -> 9001 102 us; with tiles of 128 x 128 165). One k tile
+ * is taken too (2327 x 256 -> 16384 25 us; 95).
  *
  * Rows that are no whole k tiles long, or whose scales are not 8-byte aligned: k_mxfp4_scales copies the scales into rows of 8 bytes a k tile. The last k
  * tile then is the last 8 blocks of a row, with scales 0 for those that the one before it has had: 2^-254 a product, nothing in f32, whatever the codes. us,
- * with it / tiles of 128 x 128: 2930 x 3793 -> 6325 57 / 97, 1158 x 896 -> 10821 18 / 48, 512 x 2500 -> 19457 26 / 51. */
+ * bf16 results, with it / tiles of 128 x 128: 2930 x 3793 -> 6325 60 / 97, 1158 x 896 -> 10821 19 / 48, 512 x 2500 -> 19457 26 / 51. */
 template <int NA>
 struct Wide {
     static constexpr int TM = 256, TN = 32 * NA, WP = (2 * NA + 7) / 8;                  /* WP: 8-row pieces of half of W per wave */
@@ -470,7 +471,7 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
  * lines as its codes. Part p of a row (two k tiles) sits in slot p ^ ((r >> 2) & 3). One barrier a k tile, in front of the last
  * step: behind it the tile's stage is free and is requested again, STAGES tiles ahead.
  *
- * Bound by latency, k tile after k tile: 777 x 1000 -> 1111 4.9 - 5.5 us, 512 x 9728 -> 2560 18.
+ * Bound by latency, k tile after k tile: 777 x 1000 -> 1111 5.3 us, 512 x 9728 -> 2560 18 (from HBM 23).
  *
  * TAIL: any number of blocks, and scales at any address. Codes past the end of a row come from a line of zeros; scales go through
  * registers, 1 for blocks past the end. */
@@ -728,9 +729,9 @@ long tiles_at_most(int M, int N, int groups, int tm, int tn) {
 
 /* Results leave the L2s as they are stored (write_through.h), those of 100 MB and more past the Infinity Cache (256 MB) too, with the streaming hint: it then
  * keeps the operands. us, plain / through, and with the conversion of the result to MXFP4 behind: 512 x 2560 -> 19456 19.0 / 18.2 and 25.2 / 24.6,
- * 2115 x 4096 -> 4096 25.2 / 24.4 and 30.8 / 29.9, 1000 x 1024 -> 9216 11.7 / 10.4 and 17.6 / 16.9, 300 x 512 -> 4096 6.0 / 6.0 and 10.4 / 10.2. Plain / streaming:
- * 4608 x 4096 -> 36864 (340 MB) 360 / 341 and 427 / 419, -> 12288 (113 MB) 147 / 122 and 171.5 / 170.7, -> 10240 (94 MB) with the conversion
- * 121.8 / 122.6, -> 8192 107.7 / 110.7; unaligned rows not: 4608 x 2560 -> 16001 130 / 142. Kernels of their own: of a test in front of two stores to one place the compiler keeps one, the plain one. */
+ * 2115 x 4096 -> 4096 25.2 / 24.4 and 30.8 / 29.9, 1000 x 1024 -> 9216 11.7 / 10.4 and 17.6 / 16.9, 300 x 512 -> 4096 6.0 / 6.0 and 10.4 / 10.2. Through / streaming:
+ * 4608 x 4096 -> 36864 (340 MB) 387 / 363 (weights from HBM 380 / 366) and 446 / 440, -> 12288 (113 MB) 133 / 129 (131 / 131) and 154 / 155, in two groups 150 / 130 (150 / 149); f32
+ * 36864 450 / 413, 9000 x 1024 -> 4096 (147 MB) 51.4 / 49.0; unaligned rows not: 4608 x 2560 -> 16001 130 / 142. Kernels of their own: of a test in front of two stores to one place the compiler keeps one, the plain one. */
 constexpr size_t STREAM_BYTES = (size_t)100 << 20;
 
 /* part: room for the copy of the scales, NULL where they can be read as they are */
@@ -786,7 +787,8 @@ int launch_rows(hipStream_t st, KERNEL_PARAMS) {
 /* Estimated times in us. A workgroup's k tile takes `step` where workgroups have a CU to themselves and `share` for each of those on its CU where they
  * are more; `fixed` is the launch, the first tiles and the end, `again` what a further round of the resident ones takes more. Fitted to
  * 190 sizes (1 - 4608 rows, 512 -> 512 to 16384 -> 1024 and 2560 -> 19456): what is chosen takes 1.7 % longer on average than the best of 17 tiles,
- * 20 % at worst. us, best others / chosen: 512 x 9728 -> 2560 (64 x 128) 23.2 / 18.3, 64 x 9728 -> 2560 (32 x 32) 11.2 / 8.8, 512 x 4096 ->
+ * 20 % at worst, with operands from the caches. The times are there to be compared: as the clock falls with the work, large layers take longer (4608 x 4096 -> 36864
+ * 280, measured 357; 512 + 4096 rows -> 12288 101, 128). us, best others / chosen: 512 x 9728 -> 2560 (64 x 128) 23.2 / 18.3, 64 x 9728 -> 2560 (32 x 32) 11.2 / 8.8, 512 x 4096 ->
  * 12288 (256 x 192) 30.8 / 23.2, 2115 x 4096 -> 12288 (256 x 256) 73.4 / 61.6. */
 struct Shape { int tm, tn, threads, resident; float fixed, step, share, again; };
 constexpr Shape SHAPES[] = {{32, 32, 256, 4, 3.36f, 0.129f, 0.098f, 1.6f},   {64, 64, 256, 2, 3.87f, 0.257f, 0.214f, 2.5f},  {64, 128, 256, 1, 4.16f, 0.344f, 0.354f, 3.2f},
@@ -804,7 +806,7 @@ int plan_mxfp4(int groups, int M, int N, int nb, bool whole, size_t part_bytes) 
     const long some = groups < M ? groups : M;
     auto row_tiles = [&](int tm) { return groups == 1 ? ((long)M + tm - 1) / tm : row_tiles_about(M, groups, tm); };
     const float weights = 17.0f * (float)nb * (float)N, fresh = (float)some * weights / 5.0e6f;    /* HBM's 5 TB/s */
-    /* k_mxfp4_rows: a step of a wave 1 us, W once for every 16 rows at 5.5 TB/s, a workgroup 1.15 ns */
+    /* k_mxfp4_rows: a step of a wave 1 us, W once for every 16 rows at 5.5 TB/s (from the Infinity Cache), a workgroup 1.15 ns */
     const float steps = (float)(((nb + 15) / 16 + ROWS_KW - 1) / ROWS_KW), read = (float)row_tiles(16) * weights / 5.5e6f;
     const float starts = 1.15e-3f * (float)row_tiles(16) * (float)((N + 15L) / 16), most = steps > read ? steps : read;
     float best = 2.2f + (most > starts ? most : starts);
