@@ -11,7 +11,7 @@
  * four consecutive n of one output row.
  *
  * Three kernels: k_mxfp4_rows for a few rows (bound by the reading of the weights), k_mxfp4_tiles in four tiles, k_mxfp4_wide in tiles of 256 rows.
- * plan_mxfp4 chooses. Times are medians; "from HBM": the weights of more layers in turn than the Infinity Cache (256 MB) holds, otherwise they may be in it.
+ * plan_mxfp4 chooses. Times are medians, of several runs from the least to the largest; "from HBM": the weights of more layers in turn than the Infinity Cache (256 MB) holds, otherwise they may be in it.
  */
 #include <hip/hip_runtime.h>
 
@@ -87,8 +87,8 @@ __device__ __forceinline__ f32x16 mfma32(i32x4 a, i32x4 b, f32x16 c, int sa, int
  * A workgroup owns 16 rows x 16 A columns; its KW waves walk a range of K each and add their sums through the LDS, in order. A step is 16 blocks of
  * 32: lane group g of the four holds blocks 4 g .. 4 g + 3, 64 contiguous bytes of its row, four products follow each other, and the
  * scales are the bytes of one register. The operands of the next step are on their way while this one is multiplied. In the last step of a row
- * that is no multiple of 16 blocks long, blocks past the end are zeros with scale 1. Any sizes. Bound by the reading of the weights: 1 row, 4096 -> 24576 (54 MB) 11.6 us
- * from HBM (4.6 TB/s), 10.4 from the Infinity Cache; 40 rows over 64 groups, 2560 -> 1536 (48 MB) 14.2 and 13.1. */
+ * that is no multiple of 16 blocks long, blocks past the end are zeros with scale 1. Any sizes. Bound by the reading of the weights: 1 row, 4096 -> 24576 (54 MB) 11.6 - 12.0 us
+ * from HBM (4.5 TB/s), 10.4 - 10.8 from the Infinity Cache; 40 rows over 64 groups, 2560 -> 1536 (48 MB) 14.2 and 13.1. */
 constexpr int ROWS_KW = 4;
 typedef uint32_t uint32_at1 __attribute__((aligned(1)));
 
@@ -212,9 +212,9 @@ k_mxfp4_rows(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
  * products. Requests past the end of K are issued all the same (a branch around each costs more, and the waits count them), but all lanes ask for
  * one 16 B of the last tile, into a stage that nobody reads.
  *
- * A k tile takes 1.68 us (256 tiles, K 4096 and 12288), its products at the rate above 1.16 - 1.21, and the first loads and the stores of a round of tiles 5.5 more, when nothing
- * else runs on a CU. 4608 x 4096 -> 36864 357 us (3.9 PFLOP/s; 2592 tiles are 10.1 rounds and take 11; the matrix cores are busy for half of the cycles, at 1.96 of
- * 2.4 GHz), 512 + 4096 rows in groups -> 12288 128 (from HBM 149), 512 x 2560 -> 19456 18.9 (21.1). f32 results, 4608 x 4096 -> 36864 395.
+ * A k tile takes 1.7 us (256 tiles, K 4096 and 12288), its products at the rate above 1.16 - 1.21, and the first loads and the stores of a round of tiles 5.5 more, when nothing
+ * else runs on a CU. 4608 x 4096 -> 36864 355 - 366 us (3.8 - 3.9 PFLOP/s; 2592 tiles are 10.1 rounds and take 11; the matrix cores are busy for half of the cycles, at 1.85 - 1.96 of
+ * 2.4 GHz), 512 + 4096 rows in groups -> 12288 128 - 132 (from HBM 148), 512 x 2560 -> 19456 18.8 - 19.6 (21.0 - 21.4). f32 results, 4608 x 4096 -> 36864 395.
  *
  * Any number of columns: of an unaligned row the pieces are stored as they lie (bf16 results, 4608 x 4096 -> 9001 102 us; with tiles of 128 x 128 165). One k tile
  * is taken too (2327 x 256 -> 16384 25 us; 95).
@@ -471,7 +471,7 @@ k_mxfp4_wide(OUT *__restrict__ y, const uint8_t *__restrict__ x, const uint8_t *
  * lines as its codes. Part p of a row (two k tiles) sits in slot p ^ ((r >> 2) & 3). One barrier a k tile, in front of the last
  * step: behind it the tile's stage is free and is requested again, STAGES tiles ahead.
  *
- * Bound by latency, k tile after k tile: 777 x 1000 -> 1111 5.3 us, 512 x 9728 -> 2560 18 (from HBM 23).
+ * Bound by latency, k tile after k tile: 777 x 1000 -> 1111 5.0 - 5.4 us, 512 x 9728 -> 2560 18 (from HBM 23).
  *
  * TAIL: any number of blocks, and scales at any address. Codes past the end of a row come from a line of zeros; scales go through
  * registers, 1 for blocks past the end. */
@@ -788,7 +788,7 @@ int launch_rows(hipStream_t st, KERNEL_PARAMS) {
  * are more; `fixed` is the launch, the first tiles and the end, `again` what a further round of the resident ones takes more. Fitted to
  * 190 sizes (1 - 4608 rows, 512 -> 512 to 16384 -> 1024 and 2560 -> 19456): what is chosen takes 1.7 % longer on average than the best of 17 tiles,
  * 20 % at worst, with operands from the caches. The times are there to be compared: as the clock falls with the work, large layers take longer (4608 x 4096 -> 36864
- * 280, measured 357; 512 + 4096 rows -> 12288 101, 128). us, best others / chosen: 512 x 9728 -> 2560 (64 x 128) 23.2 / 18.3, 64 x 9728 -> 2560 (32 x 32) 11.2 / 8.8, 512 x 4096 ->
+ * 280, measured 359; 512 + 4096 rows -> 12288 101, 130). us, best others / chosen: 512 x 9728 -> 2560 (64 x 128) 23.2 / 18.3, 64 x 9728 -> 2560 (32 x 32) 11.2 / 8.8, 512 x 4096 ->
  * 12288 (256 x 192) 30.8 / 23.2, 2115 x 4096 -> 12288 (256 x 256) 73.4 / 61.6. */
 struct Shape { int tm, tn, threads, resident; float fixed, step, share, again; };
 constexpr Shape SHAPES[] = {{32, 32, 256, 4, 3.36f, 0.129f, 0.098f, 1.6f},   {64, 64, 256, 2, 3.87f, 0.257f, 0.214f, 2.5f},  {64, 128, 256, 1, 4.16f, 0.344f, 0.354f, 3.2f},

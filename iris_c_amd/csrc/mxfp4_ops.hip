@@ -12,7 +12,7 @@
  * A thread takes 8 values: four lanes hold a block and find its largest magnitude with two DPP exchanges, each stores 4 bytes of
  * codes, so that a wave's stores are 256 contiguous bytes, and the first lane of the four the scale. Rows may start anywhere: the
  * loads are 16 bytes wide whatever their alignment, single values only where a row ends. Bound by memory: 4608 x 16384 bf16 there
- * 35 us and back 27.6 (5.5 and 6.9 TB/s with the codes), f32 62 and 77 (5.5 and 4.4); a row is a launch of 2 us.
+ * 36 us and back 28 (5.4 and 6.9 TB/s with the codes), f32 62 and 77 (5.5 and 4.4); a row is a launch of 2 us.
  */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
