@@ -7,7 +7,7 @@ import pytest
 
 import iris_c_amd
 import mxfp4_reference as mx
-from gpu_harness import Dev
+from gpu_harness import Dev, ptr_add
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +94,30 @@ def test_every_kernel_and_tile(dev, groups, rows, k, n, route, kind, out):
     if (groups, rows) == (64, 4096) and kind != "uneven":
         pytest.skip("250 million weights: once")
     layer(dev, groups, rows, k, n, FIRST[kind](np.random.default_rng(groups + rows), rows, groups), out)
+
+
+# rows of each group, n: a block of columns a wave, and two
+@pytest.mark.parametrize("sizes,n", [([3, 0, 1], 37), ([5] * 16, 2560)])
+@pytest.mark.parametrize("k", [1, 2, 63, 64, 65, 127, 128, 129, 191, 192, 256, 511, 512, 640, 1025])
+@pytest.mark.parametrize("x_off,w_off", [(1, 0), (0, 1), (1, 1), (3, 2), (0, 0)])
+def test_few_rows_of_matrices_that_start_in_the_middle_of_four_bytes(dev, sizes, n, k, x_off, w_off):
+    """x and W apart, in front of and behind them values that are not numbers; every number of steps up to several a wave"""
+    groups, rows = len(sizes), sum(sizes) + 1
+    first = np.concatenate([[0], np.cumsum(sizes)])
+    rng = np.random.default_rng(k)
+    x, w = rng.integers(0, 17, (rows, k), dtype=np.uint8), rng.integers(0, 17, (groups, n, k), dtype=np.uint8)
+
+    def put(a, off):
+        host = np.full(a.size + 32, 0x7fff, np.uint16)
+        host[16 + off:16 + off + a.size] = BITS[a].reshape(-1)
+        return ptr_add(dev.put(host), 2 * (16 + off))
+
+    dy = dev.put(np.full((rows, n), 7.0, np.float32))
+    dev.lib.iris_dev_linear_f32_grouped(dy, put(x, x_off), put(w, w_off), dev.put(first.astype(np.int32)), groups, rows, k, n)
+    dev.check()
+    got = dev.get(dy, (rows, n), np.float32)
+    dev.free_all()
+    want = np.full((rows, n), 7.0, np.float32)
+    for g in range(groups):
+        want[first[g]:first[g + 1]] = VALUES[x[first[g]:first[g + 1]]] @ VALUES[w[g]].T
+    assert np.array_equal(got, want)
