@@ -80,7 +80,7 @@ k_grouped_any(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16_
         src[0][c] = W + (size_t)min(n0 + srow + 32 * c, N - 1) * K + scol;
         src[1][c] = x + (size_t)min(t.m0 + srow + 32 * c, t.end - 1) * K + scol;
     }
-    const int steps = (K + TK - 1) / TK, whole = K / TK;
+    const int steps = (K - 1) / TK + 1, whole = K / TK;
     struct Step { u32x4 v[2][B]; };
     auto fetch = [&](Step &s, int step) {
         if (step < whole) {
@@ -236,7 +236,7 @@ k_grouped_rows(OUT *__restrict__ y, const uint16_t *__restrict__ x, const uint16
                 acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, s.a[u][i]), __builtin_bit_cast(bf16x8, s.b[u]), acc[i], 0, 0, 0);
     };
     const HalfSteps inside = STARTS == INSIDE ? half_steps(x, W, K, 32 * U) : HalfSteps{0, K / (32 * U)};
-    const int steps = (K + 32 * U - 1) / (32 * U);
+    const int steps = (K - 1) / (32 * U) + 1;
     const int from = (int)((long)steps * kw / KW), to = (int)((long)steps * (kw + 1) / KW), full = min(to, inside.upto);
     Step s0, s1;
     int at = from;
@@ -331,7 +331,7 @@ Plan plan_grouped(int groups, int rows, int in, int out, int out_size, bool alig
         const int tile = 32 * blocks;
         const float alone = blocks == 2 ? 0.62f : 1.1f, share = blocks == 2 ? 0.42f : 1.08f;
         const long wgs = row_tiles_about(rows, groups, tile) * ((out + tile - 1L) / tile);
-        const float each = share * (float)((wgs + 255) / 256), us = 5.0f + (float)((in + 63) / 64) * (each > alone ? each : alone);
+        const float each = share * (float)((wgs + 255) / 256), us = 5.0f + (float)((in + 63L) / 64) * (each > alone ? each : alone);
         if (us < best && fits(tile, tile)) { best = us; plan = {0, blocks, 1}; }
     }
     return plan;

@@ -70,3 +70,28 @@ def test_grouped_mxfp4_layer_of_two_million_columns(dev):
         else:
             want = mx.bf16_round((w[g:g + 4096] @ x[m] + 0.0).astype(np.float32))
             assert np.array_equal(got[m], np.tile(want, turns)[:n]), m
+
+
+@pytest.mark.parametrize("k", [2 ** 31 - 1, 2 ** 31 - 64])
+def test_the_longest_rows(dev, k):
+    """Rows of up to 2^31 - 1 values (4 GB), zeros but for some, the last ones among them"""
+    rng = np.random.default_rng(0)
+    at = np.unique(np.concatenate([rng.integers(0, k, 60), [0, 1, 127, 128, k // 2, k - 129, k - 65, k - 2, k - 1]]))
+    values = rng.integers(1, 9, (2, at.size)).astype(np.float32)
+    zeros = np.zeros(1 << 27, np.uint16)
+    d = []
+    for v in values:
+        p = dev.alloc(k * 2)
+        for start in range(0, k, zeros.size):
+            dev.lib.iris_dev_upload(ptr_add(p, 2 * start), zeros.ctypes.data, 2 * min(zeros.size, k - start))
+        bits = mx.bf16_round(v)
+        for i, b in zip(at, bits):
+            one = np.array([b], np.uint16)
+            dev.lib.iris_dev_upload(ptr_add(p, 2 * int(i)), one.ctypes.data, 2)
+        d.append(p)
+    dy = dev.put(np.full(2, 7.0, np.float32))
+    dev.lib.iris_dev_linear_f32_grouped(dy, d[0], d[1], dev.put(np.array([0, 1], np.int32)), 1, 1, k, 1)
+    dev.check()
+    got = dev.get(dy, (2,), np.float32)
+    dev.free_all()
+    assert got.tolist() == [float((values[0] * values[1]).sum()), 7.0]
