@@ -258,6 +258,69 @@ void iris_dev_linear_mxfp4_f32_grouped(float *y, const uint8_t *x, const uint8_t
 void iris_dev_linear_mxfp4_bf16_grouped(uint16_t *y, const uint8_t *x, const uint8_t *x_scales, const uint8_t *W, const uint8_t *W_scales,
                                         const int *first_row, int groups, int rows, int in, int out);
 
+/* ---- packed sequences, and a key-value cache in pages ----
+ * Rows of several sequences lie one behind the other: sequence g has the rows first_row[g] <= m < first_row[g + 1]; first_row: device int
+ * [sequences + 1], not decreasing, read when the call runs. Sequences may be empty. Whatever the arrays hold, no call reads or writes
+ * outside its rows: a value below one before it counts as that one, values are limited to 0 .. rows. Rows of an output in front of the
+ * first sequence and behind the last one stay as they were. sequences 0 or rows 0 does nothing. */
+
+/* iris_dev_attention within every sequence, as one launch: the prompts of a batch without their padding, pictures of several sizes.
+ * q, out: rows of heads * head_dim; k, v: rows of kv_heads * head_dim, both of stride ldkv; query head h takes kv head
+ * h / (heads / kv_heads). first_key NULL: the keys of a sequence are its own rows (keys == rows). Otherwise its keys are the rows
+ * first_key[g] <= j < first_key[g + 1] of k and v (limited to 0 .. keys): a prompt that goes on from rows in a cache (iris_dev_cache_read_*).
+ * causal: the last row of a sequence sees all of its keys, each row in front of it one key less: row i of n sees the keys
+ * j <= i + (m - n) of m. A row that sees no key gives zeros. What it does not see has no part in its result, infinities and NaN included.
+ * head_dim 128 on rows that are 16-byte aligned (out: 8) and scale > 0 run on the matrix cores, everything else on a scalar kernel. P is
+ * rounded to bf16 for the P V product and the row sums are those of the rounded values, as in iris_dev_attention.
+ * Needs rows * heads < 2^31; larger calls, and those that no launch holds, are reported. */
+void iris_dev_attention_sequences(uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k, const uint16_t *v, int ldkv,
+                                  const int *first_row, const int *first_key, int sequences, int rows, int keys,
+                                  int heads, int kv_heads, int head_dim, float scale, int causal);
+
+/* The cache. `pages` pages of page_size tokens (a power of two), for K and for V: [pages, kv_heads, page_size, head_dim], in bf16 or in 8
+ * bits (e4m3: sign, four bits of exponent, three of fraction, largest 448) with a scale byte s, 2^(s - 127), 255 for NaN, for each token's
+ * row of a head: [pages, kv_heads, page_size]. page_table: device int [sequences, table_ld], position p of sequence g is place
+ * p % page_size of page page_table[g * table_ld + p / page_size]; lengths: device int [sequences], the tokens of each sequence, those
+ * that the call brings included. Both are read when the call runs. A page number outside 0 .. pages - 1 is a page that is not there: its
+ * positions are not written, not read, and no keys. Lengths count as limited to 0 .. table_ld * page_size. Sequences may share pages. */
+
+/* The rows of the sequences (k and v: rows of kv_heads * head_dim, stride ld) into their pages: of a sequence with n rows, row i goes to
+ * position lengths[g] - n + i; positions below 0, and those that the table does not reach, are left out. first_row NULL: row g is the one
+ * row of sequence g (rows == sequences), the newest token of each. No two rows of a call may go to the same place.
+ * Quantised, the scale of a row is the smallest power of two (at least 2^-127) that its largest magnitude is at most 448 times of, its
+ * codes the nearest ones to value / scale, ties to the even code; a row with an infinity or a NaN in it becomes NaN as a whole. */
+void iris_dev_cache_write_bf16(uint16_t *k_pages, uint16_t *v_pages, int pages, int page_size, const int *page_table, int table_ld,
+                               const int *lengths, const uint16_t *k, const uint16_t *v, int ld, const int *first_row, int sequences,
+                               int rows, int kv_heads, int head_dim);
+void iris_dev_cache_write_fp8(uint8_t *k_pages, uint8_t *v_pages, uint8_t *k_scales, uint8_t *v_scales, int pages, int page_size,
+                              const int *page_table, int table_ld, const int *lengths, const uint16_t *k, const uint16_t *v, int ld,
+                              const int *first_row, int sequences, int rows, int kv_heads, int head_dim);
+/* Back, the last n positions of each sequence into its n rows; rows whose position is not there stay as they were. Exact, but for values
+ * that bf16 rounds. */
+void iris_dev_cache_read_bf16(uint16_t *k, uint16_t *v, int ld, const uint16_t *k_pages, const uint16_t *v_pages, int pages, int page_size,
+                              const int *page_table, int table_ld, const int *lengths, const int *first_row, int sequences, int rows,
+                              int kv_heads, int head_dim);
+void iris_dev_cache_read_fp8(uint16_t *k, uint16_t *v, int ld, const uint8_t *k_pages, const uint8_t *v_pages, const uint8_t *k_scales,
+                             const uint8_t *v_scales, int pages, int page_size, const int *page_table, int table_ld, const int *lengths,
+                             const int *first_row, int sequences, int rows, int kv_heads, int head_dim);
+
+/* Attention of one row a sequence, its newest token, over the lengths[g] tokens that the cache holds of it: out[g] = softmax(scale q[g]
+ * K^T) V; q and out: rows of heads * head_dim. A sequence without keys gives zeros. What lies in the pages behind a sequence's last
+ * token has no part in its result, whatever it is. head_dim 128 on 16-byte aligned rows and pages and scale > 0 run on the matrix cores,
+ * everything else on a scalar kernel.
+ * The keys are cut into ranges whose partial results pass through `workspace`, at least iris_dev_attention_paged_workspace() bytes of
+ * device memory, 16-byte aligned, that nothing else uses meanwhile; NULL: the library's own, which the library's stream orders. Captured
+ * calls that may be replayed beside others therefore take workspaces of their own. The ranges, and with them the order of the f32 sums,
+ * depend on the lengths of all sequences of the call; a call gives the same bits every time. */
+size_t iris_dev_attention_paged_workspace(void);
+void iris_dev_attention_paged_bf16(uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k_pages, const uint16_t *v_pages,
+                                   int pages, int page_size, const int *page_table, int table_ld, const int *lengths, int sequences,
+                                   int heads, int kv_heads, int head_dim, float scale, void *workspace);
+void iris_dev_attention_paged_fp8(uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint8_t *k_pages, const uint8_t *v_pages,
+                                  const uint8_t *k_scales, const uint8_t *v_scales, int pages, int page_size, const int *page_table,
+                                  int table_ld, const int *lengths, int sequences, int heads, int kv_heads, int head_dim, float scale,
+                                  void *workspace);
+
 /* The library's stream as a hipStream_t, for callers that time kernels with
  * HIP events or order their own work after the library's. */
 void *iris_dev_stream(void);

@@ -61,6 +61,14 @@ ABI = {
     "iris_dev_linear_mxfp4_bf16": (None, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i]),
     "iris_dev_linear_mxfp4_f32_grouped": (None, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i]),
     "iris_dev_linear_mxfp4_bf16_grouped": (None, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i]),
+    "iris_dev_attention_sequences": (None, [_vp, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i]),
+    "iris_dev_cache_write_bf16": (None, [_vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i]),
+    "iris_dev_cache_write_fp8": (None, [_vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i]),
+    "iris_dev_cache_read_bf16": (None, [_vp, _vp, _i, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i]),
+    "iris_dev_cache_read_fp8": (None, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i]),
+    "iris_dev_attention_paged_workspace": (_sz, []),
+    "iris_dev_attention_paged_bf16": (None, [_vp, _i, _vp, _i, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _i, _i, _i, _f, _vp]),
+    "iris_dev_attention_paged_fp8": (None, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _i, _i, _i, _f, _vp]),
     "iris_dev_stream": (_vp, []),
     "iris_dev_last_error": (_i, []),
     "iris_dev_last_kernel": (C.c_char_p, []),

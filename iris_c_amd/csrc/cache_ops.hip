@@ -1,0 +1,184 @@
+/*
+ * Rows of K and V into the pages of a cache (paged_cache.h) and back, as bf16 or as e4m3 codes with a scale for each row of a head.
+ *
+ * Quantising a row x of head_dim values: 2^e is the smallest power of two with max |x| <= 448 * 2^e (448 is the largest e4m3 value), at
+ * least 2^-127; the codes are x / 2^e rounded to the nearest code, ties to the even one. Dividing by a power of two is exact, so that
+ * one rounding is the only one, at most half a step, 2^-4 of the value (2^-10 of 2^e below 2^-6 of it), and no value saturates. From
+ * the bits of the largest magnitude, sign off: e = exponent - 8, one more where its fraction is above .75. A row with an infinity or a
+ * NaN in it becomes NaN as a whole (scale byte 255, codes 0).
+ *
+ * The rows of a call are the last ones of their sequences: row i of n is position length - n + i. A workgroup takes ROWS rows of one
+ * sequence, of K or of V. Bound by memory: each value is read and written once.
+ */
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "iris_kernels_hip.h"
+#include "paged_cache.h"
+#include "sequences.h"
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+namespace {
+
+constexpr int ROWS = 16, THREADS = 256;
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const f32x2 p = {lo, hi};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(p, bf16x2));
+}
+
+/* the scale byte of a row whose largest magnitude has these bf16 bits (sign off), and what its values are multiplied by */
+__device__ __forceinline__ unsigned scale_byte(unsigned top, float *factor) {
+    const int exponent = (int)(top >> 7), e = max(exponent - 135 + ((top & 0x7f) > 0x60), -127);
+    *factor = e == -127 ? __uint_as_float(0x7f000000u) : __uint_as_float((unsigned)(127 - e) << 23);
+    return exponent == 255 ? 255 : (unsigned)(e + 127);
+}
+
+/* position of row `row` of the sequence, or -1 where the cache has no place for it */
+__device__ __forceinline__ int position(const PagedArg &c, const SequenceTile &s, int row) {
+    const int pos = max(c.lengths[s.g], 0) - s.n + row;
+    return pos >= 0 && pos < ((long)c.ld << c.shift) ? pos : -1;
+}
+
+struct Pair { void *k, *v; };
+struct ConstPair { const void *k, *v; };
+
+/* head_dim = 8 LANES, rows 16-byte aligned: 16 bytes of bf16 to a lane, LANES lanes to a row of a head */
+template <int LANES, bool FP8, bool WRITE>
+__global__ void __launch_bounds__(THREADS)
+k_cache_rows(Pair pages, Pair scales, ConstPair rows, Pair out, int ld, PagedArg cache, SequencesArg seqs) {
+    SequenceTiles tiles;
+    const int count = tiles.count(seqs, ROWS), t = blockIdx.x >> 1;
+    if (t >= count) return;
+    const bool second = blockIdx.x & 1;
+    const SequenceTile s = tiles.tile(t);
+    const int n = min(ROWS, s.n - s.c0), units = n * cache.kv_heads * LANES;
+    uint8_t *codes = (uint8_t *)(second ? pages.v : pages.k), *bytes = (uint8_t *)(second ? scales.v : scales.k);
+    uint16_t *plain = (uint16_t *)(second ? pages.v : pages.k);
+    const uint16_t *from = (const uint16_t *)(second ? rows.v : rows.k);
+    uint16_t *to = (uint16_t *)(second ? out.v : out.k);
+    for (int u = threadIdx.x; u < units; u += THREADS) {
+        const int lane = u % LANES, head = u / LANES % cache.kv_heads, row = s.c0 + u / LANES / cache.kv_heads;
+        const int pos = position(cache, s, row);
+        const long place = pos < 0 ? -1 : paged_row(cache, s.g, pos, head);
+        if (place < 0) continue;                                     /* the same for the LANES lanes of a row */
+        const size_t at = (size_t)(s.row0 + row) * ld + (size_t)head * (8 * LANES) + 8 * lane, in_pages = (size_t)place * (8 * LANES) + 8 * lane;
+        if constexpr (!FP8) {
+            if (WRITE) *reinterpret_cast<uint4 *>(plain + in_pages) = *reinterpret_cast<const uint4 *>(from + at);
+            else *reinterpret_cast<uint4 *>(to + at) = *reinterpret_cast<const uint4 *>(plain + in_pages);
+        } else if constexpr (WRITE) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(from + at);
+            const unsigned w[4] = {x.x, x.y, x.z, x.w};
+            unsigned top = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) top = max(top, max(w[i] & 0x7fff, (w[i] >> 16) & 0x7fff));
+#pragma unroll
+            for (int d = 1; d < LANES; d <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, d, 64));
+            float factor;
+            const unsigned byte = scale_byte(top, &factor);
+            int c[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float lo = __uint_as_float(w[i] << 16) * factor, hi = __uint_as_float(w[i] & 0xffff0000u) * factor;
+                c[i / 2] = i % 2 ? __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, c[i / 2], true) : __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, c[i / 2], false);
+            }
+            *reinterpret_cast<int2 *>(codes + in_pages) = byte == 255 ? make_int2(0, 0) : make_int2(c[0], c[1]);
+            if (lane == 0) bytes[place] = (uint8_t)byte;
+        } else {
+            const int2 c = *reinterpret_cast<const int2 *>(codes + in_pages);
+            const float scale = paged_scale(bytes[place]);
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int word = i < 2 ? c.x : c.y;
+                const f32x2 f = i % 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(word, true) : __builtin_amdgcn_cvt_pk_f32_fp8(word, false);
+                w[i] = pack_bf16(f[0] * scale, f[1] * scale);
+            }
+            *reinterpret_cast<uint4 *>(to + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+/* any head_dim, stride and alignment: a wave to a row of a head */
+template <bool FP8, bool WRITE>
+__global__ void __launch_bounds__(THREADS)
+k_cache_rows_any(Pair pages, Pair scales, ConstPair rows, Pair out, int ld, PagedArg cache, SequencesArg seqs) {
+    SequenceTiles tiles;
+    const int count = tiles.count(seqs, ROWS), t = blockIdx.x >> 1, hd = cache.head_dim;
+    if (t >= count) return;
+    const bool second = blockIdx.x & 1;
+    const SequenceTile s = tiles.tile(t);
+    const int units = min(ROWS, s.n - s.c0) * cache.kv_heads, lane = threadIdx.x & 63;
+    uint8_t *codes = (uint8_t *)(second ? pages.v : pages.k), *bytes = (uint8_t *)(second ? scales.v : scales.k);
+    uint16_t *plain = (uint16_t *)(second ? pages.v : pages.k);
+    const uint16_t *from = (const uint16_t *)(second ? rows.v : rows.k);
+    uint16_t *to = (uint16_t *)(second ? out.v : out.k);
+    for (int u = threadIdx.x >> 6; u < units; u += THREADS / 64) {
+        const int head = u % cache.kv_heads, row = s.c0 + u / cache.kv_heads;
+        const int pos = position(cache, s, row);
+        const long place = pos < 0 ? -1 : paged_row(cache, s.g, pos, head);
+        if (place < 0) continue;
+        const size_t at = (size_t)(s.row0 + row) * ld + (size_t)head * hd, in_pages = (size_t)place * hd;
+        if constexpr (!FP8) {
+            for (int d = lane; d < hd; d += 64)
+                if (WRITE) plain[in_pages + d] = from[at + d];
+                else to[at + d] = plain[in_pages + d];
+        } else if constexpr (WRITE) {
+            unsigned top = 0;
+            for (int d = lane; d < hd; d += 64) top = max(top, (unsigned)(from[at + d] & 0x7fff));
+            for (int d = 1; d < 64; d <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, d, 64));
+            float factor;
+            const unsigned byte = scale_byte(top, &factor);
+            for (int d = lane; d < hd; d += 64) {
+                const int c = __builtin_amdgcn_cvt_pk_fp8_f32(__uint_as_float((uint32_t)from[at + d] << 16) * factor, 0.0f, 0, false);
+                codes[in_pages + d] = byte == 255 ? (uint8_t)0 : (uint8_t)c;
+            }
+            if (lane == 0) bytes[place] = (uint8_t)byte;
+        } else {
+            const float scale = paged_scale(bytes[place]);
+            for (int d = lane; d < hd; d += 64)
+                to[at + d] = (uint16_t)pack_bf16(__builtin_amdgcn_cvt_f32_fp8(codes[in_pages + d], 0) * scale, 0.0f);
+        }
+    }
+}
+
+bool aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+
+template <bool FP8, bool WRITE>
+int launch(hipStream_t stream, Pair pages, Pair scales, ConstPair rows, Pair out, int ld, const PagedArg &c, const SequencesArg &seqs) {
+    const long wgs = 2 * sequence_tiles_at_most(seqs, ROWS);
+    if (!wgs) return 0;
+    if (wgs > ((1L << 32) - 1) / THREADS) return (int)hipErrorInvalidValue;
+    const bool wide = ld % 8 == 0 && aligned(WRITE ? rows.k : out.k, 16) && aligned(WRITE ? rows.v : out.v, 16) && aligned(pages.k, FP8 ? 8 : 16) &&
+                      aligned(pages.v, FP8 ? 8 : 16);
+    const dim3 grid((unsigned)wgs), block(THREADS);
+    if (wide && c.head_dim == 128) hipLaunchKernelGGL((k_cache_rows<16, FP8, WRITE>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs);
+    else if (wide && c.head_dim == 64) hipLaunchKernelGGL((k_cache_rows<8, FP8, WRITE>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs);
+    else if (wide && c.head_dim == 256) hipLaunchKernelGGL((k_cache_rows<32, FP8, WRITE>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs);
+    else hipLaunchKernelGGL((k_cache_rows_any<FP8, WRITE>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs);
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+
+extern "C" int iris_hip_cache_write(void *stream, void *k_pages, void *v_pages, uint8_t *k_scales, uint8_t *v_scales, int pages, int page_shift,
+                                    const int *table, int table_ld, const int *lengths, const uint16_t *k, const uint16_t *v, int ld,
+                                    const int *first_row, int n, int rows, int kv_heads, int head_dim) {
+    const PagedArg c = {table, lengths, table_ld, pages, page_shift, kv_heads, head_dim};
+    const SequencesArg s = {first_row, nullptr, n, rows, 0, 1};
+    const Pair scales = {k_scales, v_scales}, none = {nullptr, nullptr};
+    return k_scales ? launch<true, true>((hipStream_t)stream, {k_pages, v_pages}, scales, {k, v}, none, ld, c, s)
+                    : launch<false, true>((hipStream_t)stream, {k_pages, v_pages}, scales, {k, v}, none, ld, c, s);
+}
+
+extern "C" int iris_hip_cache_read(void *stream, uint16_t *k, uint16_t *v, int ld, const void *k_pages, const void *v_pages,
+                                   const uint8_t *k_scales, const uint8_t *v_scales, int pages, int page_shift, const int *table, int table_ld,
+                                   const int *lengths, const int *first_row, int n, int rows, int kv_heads, int head_dim) {
+    const PagedArg c = {table, lengths, table_ld, pages, page_shift, kv_heads, head_dim};
+    const SequencesArg s = {first_row, nullptr, n, rows, 0, 1};
+    const Pair at = {const_cast<void *>(k_pages), const_cast<void *>(v_pages)}, scales = {const_cast<uint8_t *>(k_scales), const_cast<uint8_t *>(v_scales)};
+    return k_scales ? launch<true, false>((hipStream_t)stream, at, scales, {nullptr, nullptr}, {k, v}, ld, c, s)
+                    : launch<false, false>((hipStream_t)stream, at, scales, {nullptr, nullptr}, {k, v}, ld, c, s);
+}

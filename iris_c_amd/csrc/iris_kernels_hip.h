@@ -218,6 +218,24 @@ int iris_lt_linear(void *stream, void *y, int out_bf16, const uint16_t *x, const
 int iris_lt_available(void);
 void iris_lt_release(void);
 
+/* ---- packed sequences and the paged cache (attn_sequences.hip, cache_ops.hip) ----
+ * n sequences: rows [first_row[g], first_row[g + 1]) of `rows` (first_row NULL: row g), keys [first_key[g], ...) of `keys` (first_key NULL:
+ * the rows' own); any values in the arrays. Requires rows * heads < 2^31, heads % kv_heads == 0. */
+int iris_hip_sequences_any(void *stream, uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k, const uint16_t *v, int ldkv,
+                           const int *first_row, const int *first_key, int n, int rows, int keys, int heads, int kv_heads, int head_dim,
+                           float scale, int causal);
+/* One row a sequence over the pages; ks, vs NULL: bf16, otherwise e4m3 codes and scale bytes. Pages of 2^page_shift rows. */
+int iris_hip_paged_any(void *stream, uint16_t *out, int ldo, const uint16_t *q, int ldq, const void *k, const void *v, const uint8_t *ks,
+                       const uint8_t *vs, int pages, int page_shift, const int *table, int table_ld, const int *lengths, int n, int heads,
+                       int kv_heads, int head_dim, float scale);
+/* The last rows of every sequence into the pages and back; scales NULL: bf16 */
+int iris_hip_cache_write(void *stream, void *k_pages, void *v_pages, uint8_t *k_scales, uint8_t *v_scales, int pages, int page_shift,
+                         const int *table, int table_ld, const int *lengths, const uint16_t *k, const uint16_t *v, int ld,
+                         const int *first_row, int n, int rows, int kv_heads, int head_dim);
+int iris_hip_cache_read(void *stream, uint16_t *k, uint16_t *v, int ld, const void *k_pages, const void *v_pages, const uint8_t *k_scales,
+                        const uint8_t *v_scales, int pages, int page_shift, const int *table, int table_ld, const int *lengths,
+                        const int *first_row, int n, int rows, int kv_heads, int head_dim);
+
 /* Rotary tables [seq, half] gathered from a dictionary of (axis, position) rows: entry
  * (s, col) with columns[col] = (axis a, column j inside the axis, columns n of the axis, unused) is
  * values[index[s * naxes + a] + j] for the cosine and ... + n + j for the sine. All pointers

@@ -633,6 +633,144 @@ void iris_dev_linear_mxfp4_bf16_grouped(uint16_t *y, const uint8_t *x, const uin
     LAUNCH("linear_mxfp4_grouped", iris_hip_linear_mxfp4_bf16(g_stream, linear_part(), y, x, x_scales, W, W_scales, first_row, groups, rows, in, out));
 }
 
+/* ---- packed sequences, and the key-value cache in pages ---- */
+
+void iris_dev_attention_sequences(uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k, const uint16_t *v, int ldkv,
+                                  const int *first_row, const int *first_key, int sequences, int rows, int keys,
+                                  int heads, int kv_heads, int head_dim, float scale, int causal) {
+    static const char what[] = "attention_sequences";
+    if (rows <= 0 || heads <= 0 || !sequences) return;
+    if (kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0 || sequences < 0 || keys < 0) {
+        fail(-1, what, "need heads % kv_heads == 0, head_dim > 0, sequences >= 0, keys >= 0");
+        return;
+    }
+    if (!first_row || !out || !q || (keys && (!k || !v))) { fail(-1, what, "first_row, out, q, k or v is missing"); return; }
+    if (!first_key && keys != rows) { fail(-1, what, "without first_key the keys are the rows: need keys == rows"); return; }
+    if ((long long)rows * heads > INT32_MAX || (long long)heads * head_dim > INT32_MAX || ldo < heads * head_dim || ldq < heads * head_dim ||
+        (keys && ldkv < kv_heads * head_dim)) {
+        fail(-1, what, "need rows * heads < 2^31, ldo and ldq >= heads * head_dim, ldkv >= kv_heads * head_dim");
+        return;
+    }
+    if (!need_ready(what)) return;
+    g_last_kernel = "attention_sequences_generic";
+    LAUNCH("attention_sequences", iris_hip_sequences_any(g_stream, out, ldo, q, ldq, k, v, ldkv, first_row, first_key, sequences, rows, keys, heads,
+                                                          kv_heads, head_dim, scale, causal != 0));
+}
+
+/* 1 and the logarithm of page_size, or 0 after reporting what is wrong; also where there is nothing to do. `fp8`: there have to be scales */
+static int cache_args(const char *what, const void *k_pages, const void *v_pages, const uint8_t *k_scales, const uint8_t *v_scales, int fp8,
+                      int pages, int page_size, const int *page_table, int table_ld, const int *lengths, int sequences, int kv_heads,
+                      int head_dim, int *shift) {
+    if (sequences < 0 || kv_heads <= 0 || head_dim <= 0 || (long long)kv_heads * head_dim > INT32_MAX) {
+        fail(-1, what, "need sequences >= 0, kv_heads > 0, head_dim > 0");
+        return 0;
+    }
+    if (pages < 0 || table_ld < 0 || page_size <= 0 || (page_size & (page_size - 1))) {
+        fail(-1, what, "need pages >= 0, table_ld >= 0 and page_size a power of two");
+        return 0;
+    }
+    if (!k_pages || !v_pages || !page_table || !lengths || (fp8 && (!k_scales || !v_scales))) {
+        fail(-1, what, "pages, scales, page_table or lengths are missing");
+        return 0;
+    }
+    *shift = __builtin_ctz((unsigned)page_size);
+    return 1;
+}
+
+static int cache_rows_args(const char *what, const uint16_t *k, const uint16_t *v, int ld, const int *first_row, int sequences, int rows,
+                           int kv_heads, int head_dim) {
+    if (!k || !v) { fail(-1, what, "k or v is missing"); return 0; }
+    if (!first_row && rows != sequences) { fail(-1, what, "without first_row every sequence has one row: need rows == sequences"); return 0; }
+    if (ld < kv_heads * head_dim) { fail(-1, what, "need ld >= kv_heads * head_dim"); return 0; }
+    return 1;
+}
+
+static void cache_write(const char *what, void *k_pages, void *v_pages, uint8_t *k_scales, uint8_t *v_scales, int fp8, int pages, int page_size,
+                        const int *page_table, int table_ld, const int *lengths, const uint16_t *k, const uint16_t *v, int ld,
+                        const int *first_row, int sequences, int rows, int kv_heads, int head_dim) {
+    int shift;
+    if (rows <= 0 || !sequences ||
+        !cache_args(what, k_pages, v_pages, k_scales, v_scales, fp8, pages, page_size, page_table, table_ld, lengths, sequences, kv_heads, head_dim, &shift) ||
+        !cache_rows_args(what, k, v, ld, first_row, sequences, rows, kv_heads, head_dim))
+        return;
+    LAUNCH("cache_write", iris_hip_cache_write(g_stream, k_pages, v_pages, k_scales, v_scales, pages, shift, page_table, table_ld, lengths, k, v, ld,
+                                               first_row, sequences, rows, kv_heads, head_dim));
+}
+
+static void cache_read(const char *what, uint16_t *k, uint16_t *v, int ld, const void *k_pages, const void *v_pages, const uint8_t *k_scales,
+                       const uint8_t *v_scales, int fp8, int pages, int page_size, const int *page_table, int table_ld, const int *lengths,
+                       const int *first_row, int sequences, int rows, int kv_heads, int head_dim) {
+    int shift;
+    if (rows <= 0 || !sequences ||
+        !cache_args(what, k_pages, v_pages, k_scales, v_scales, fp8, pages, page_size, page_table, table_ld, lengths, sequences, kv_heads, head_dim, &shift) ||
+        !cache_rows_args(what, k, v, ld, first_row, sequences, rows, kv_heads, head_dim))
+        return;
+    LAUNCH("cache_read", iris_hip_cache_read(g_stream, k, v, ld, k_pages, v_pages, k_scales, v_scales, pages, shift, page_table, table_ld, lengths,
+                                             first_row, sequences, rows, kv_heads, head_dim));
+}
+
+void iris_dev_cache_write_bf16(uint16_t *k_pages, uint16_t *v_pages, int pages, int page_size, const int *page_table, int table_ld,
+                               const int *lengths, const uint16_t *k, const uint16_t *v, int ld, const int *first_row, int sequences,
+                               int rows, int kv_heads, int head_dim) {
+    cache_write("cache_write_bf16", k_pages, v_pages, NULL, NULL, 0, pages, page_size, page_table, table_ld, lengths, k, v, ld, first_row, sequences, rows,
+                kv_heads, head_dim);
+}
+
+void iris_dev_cache_write_fp8(uint8_t *k_pages, uint8_t *v_pages, uint8_t *k_scales, uint8_t *v_scales, int pages, int page_size,
+                              const int *page_table, int table_ld, const int *lengths, const uint16_t *k, const uint16_t *v, int ld,
+                              const int *first_row, int sequences, int rows, int kv_heads, int head_dim) {
+    cache_write("cache_write_fp8", k_pages, v_pages, k_scales, v_scales, 1, pages, page_size, page_table, table_ld, lengths, k, v, ld, first_row, sequences,
+                rows, kv_heads, head_dim);
+}
+
+void iris_dev_cache_read_bf16(uint16_t *k, uint16_t *v, int ld, const uint16_t *k_pages, const uint16_t *v_pages, int pages, int page_size,
+                              const int *page_table, int table_ld, const int *lengths, const int *first_row, int sequences, int rows,
+                              int kv_heads, int head_dim) {
+    cache_read("cache_read_bf16", k, v, ld, k_pages, v_pages, NULL, NULL, 0, pages, page_size, page_table, table_ld, lengths, first_row, sequences, rows,
+               kv_heads, head_dim);
+}
+
+void iris_dev_cache_read_fp8(uint16_t *k, uint16_t *v, int ld, const uint8_t *k_pages, const uint8_t *v_pages, const uint8_t *k_scales,
+                             const uint8_t *v_scales, int pages, int page_size, const int *page_table, int table_ld, const int *lengths,
+                             const int *first_row, int sequences, int rows, int kv_heads, int head_dim) {
+    cache_read("cache_read_fp8", k, v, ld, k_pages, v_pages, k_scales, v_scales, 1, pages, page_size, page_table, table_ld, lengths, first_row, sequences,
+               rows, kv_heads, head_dim);
+}
+
+size_t iris_dev_attention_paged_workspace(void) { return 0; }
+
+static void attention_paged(const char *what, uint16_t *out, int ldo, const uint16_t *q, int ldq, const void *k_pages, const void *v_pages,
+                            const uint8_t *k_scales, const uint8_t *v_scales, int fp8, int pages, int page_size, const int *page_table,
+                            int table_ld, const int *lengths, int sequences, int heads, int kv_heads, int head_dim, float scale, void *workspace) {
+    int shift;
+    if (!sequences || heads <= 0) return;
+    if (kv_heads <= 0 || heads % kv_heads != 0) { fail(-1, what, "need heads % kv_heads == 0"); return; }
+    if (!cache_args(what, k_pages, v_pages, k_scales, v_scales, fp8, pages, page_size, page_table, table_ld, lengths, sequences, kv_heads, head_dim, &shift)) return;
+    if (!out || !q || !aligned(workspace, 16)) { fail(-1, what, "out or q is missing, or the workspace is not 16-byte aligned"); return; }
+    if ((long long)heads * head_dim > INT32_MAX || ldo < heads * head_dim || ldq < heads * head_dim) {
+        fail(-1, what, "need ldo and ldq >= heads * head_dim");
+        return;
+    }
+    g_last_kernel = "attention_paged_generic";
+    LAUNCH("attention_paged", iris_hip_paged_any(g_stream, out, ldo, q, ldq, k_pages, v_pages, k_scales, v_scales, pages, shift, page_table, table_ld,
+                                                 lengths, sequences, heads, kv_heads, head_dim, scale));
+}
+
+void iris_dev_attention_paged_bf16(uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k_pages, const uint16_t *v_pages,
+                                   int pages, int page_size, const int *page_table, int table_ld, const int *lengths, int sequences,
+                                   int heads, int kv_heads, int head_dim, float scale, void *workspace) {
+    attention_paged("attention_paged_bf16", out, ldo, q, ldq, k_pages, v_pages, NULL, NULL, 0, pages, page_size, page_table, table_ld, lengths, sequences,
+                    heads, kv_heads, head_dim, scale, workspace);
+}
+
+void iris_dev_attention_paged_fp8(uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint8_t *k_pages, const uint8_t *v_pages,
+                                  const uint8_t *k_scales, const uint8_t *v_scales, int pages, int page_size, const int *page_table,
+                                  int table_ld, const int *lengths, int sequences, int heads, int kv_heads, int head_dim, float scale,
+                                  void *workspace) {
+    attention_paged("attention_paged_fp8", out, ldo, q, ldq, k_pages, v_pages, k_scales, v_scales, 1, pages, page_size, page_table, table_ld, lengths,
+                    sequences, heads, kv_heads, head_dim, scale, workspace);
+}
+
 void iris_dev_layer_norm_mod(uint16_t *out, const float *x, const float *shift, const float *scale,
                              int rows, int dim, float eps) {
     LAUNCH("layer_norm_mod", iris_hip_layer_norm_mod(g_stream, out, x, shift, scale, rows, dim, eps));
