@@ -228,6 +228,13 @@ int iris_hip_sequences_any(void *stream, uint16_t *out, int ldo, const uint16_t 
 int iris_hip_paged_any(void *stream, uint16_t *out, int ldo, const uint16_t *q, int ldq, const void *k, const void *v, const uint8_t *ks,
                        const uint8_t *vs, int pages, int page_shift, const int *table, int table_ld, const int *lengths, int n, int heads,
                        int kv_heads, int head_dim, float scale);
+/* The same on the matrix cores: head_dim 128, scale > 0, q 16-byte and out 8-byte aligned, ldq % 8 == 0, ldo % 4 == 0, pages 16-byte aligned;
+ * `takes`: whether the sizes are ones that it has numbers for. part: iris_hip_paged_workspace() bytes, 16-byte aligned. */
+size_t iris_hip_paged_workspace(void);
+int iris_hip_paged_hd128_takes(int pages, int page_shift, int table_ld, int n, int heads, int kv_heads);
+int iris_hip_paged_hd128(void *stream, float *part, uint16_t *out, int ldo, const uint16_t *q, int ldq, const void *k, const void *v,
+                         const uint8_t *ks, const uint8_t *vs, int pages, int page_shift, const int *table, int table_ld, const int *lengths,
+                         int n, int heads, int kv_heads, float scale);
 /* The last rows of every sequence into the pages and back; scales NULL: bf16 */
 int iris_hip_cache_write(void *stream, void *k_pages, void *v_pages, uint8_t *k_scales, uint8_t *v_scales, int pages, int page_shift,
                          const int *table, int table_ld, const int *lengths, const uint16_t *k, const uint16_t *v, int ld,

@@ -35,6 +35,8 @@ static uint16_t *g_conv_scratch = NULL;
 /* partial sums of linear layers and convolutions whose K is cut into ranges; allocated at initialisation, so that a linear layer never
  * allocates */
 static float *g_linear_part = NULL;
+/* partial results of attention over the paged cache, allocated at initialisation: no call allocates */
+static float *g_paged_part = NULL;
 /* group norm of up to 64 groups, which keeps counters there: allocated and cleared once, by iris_dev_init; and of more */
 static float *g_gn_scratch = NULL, *g_gn_more = NULL;
 static size_t g_gn_more_floats = 0;
@@ -106,6 +108,10 @@ int iris_dev_init(void) {
         (void)hipGetLastError();                             /* linear layers then leave K whole */
         g_linear_part = NULL;
     }
+    if (!g_paged_part && hipMalloc((void **)&g_paged_part, iris_hip_paged_workspace()) != hipSuccess) {
+        (void)hipGetLastError();                             /* calls without a workspace of their own then take the scalar kernel */
+        g_paged_part = NULL;
+    }
     if (hipStreamCreate(&g_stream) != hipSuccess) return 0;
     (void)gn_scratch_setup();
     /* address of the in-library scratch of iris_dev_group_norm_noalloc on this device; if the lookup
@@ -138,6 +144,8 @@ void iris_dev_cleanup(void) {
     if (g_conv_scratch) check(hipFree(g_conv_scratch), "free");
     if (g_linear_part) check(hipFree(g_linear_part), "free");
     g_linear_part = NULL;
+    if (g_paged_part) check(hipFree(g_paged_part), "free");
+    g_paged_part = NULL;
     if (g_gn_scratch) check(hipFree(g_gn_scratch), "free");
     if (g_gn_more) check(hipFree(g_gn_more), "free");
     if (g_rope_stage) check(hipFree(g_rope_stage), "free");
@@ -737,7 +745,7 @@ void iris_dev_cache_read_fp8(uint16_t *k, uint16_t *v, int ld, const uint8_t *k_
                rows, kv_heads, head_dim);
 }
 
-size_t iris_dev_attention_paged_workspace(void) { return 0; }
+size_t iris_dev_attention_paged_workspace(void) { return iris_hip_paged_workspace(); }
 
 static void attention_paged(const char *what, uint16_t *out, int ldo, const uint16_t *q, int ldq, const void *k_pages, const void *v_pages,
                             const uint8_t *k_scales, const uint8_t *v_scales, int fp8, int pages, int page_size, const int *page_table,
@@ -749,6 +757,14 @@ static void attention_paged(const char *what, uint16_t *out, int ldo, const uint
     if (!out || !q || !aligned(workspace, 16)) { fail(-1, what, "out or q is missing, or the workspace is not 16-byte aligned"); return; }
     if ((long long)heads * head_dim > INT32_MAX || ldo < heads * head_dim || ldq < heads * head_dim) {
         fail(-1, what, "need ldo and ldq >= heads * head_dim");
+        return;
+    }
+    if (!need_ready(what)) return;
+    if (head_dim == 128 && scale > 0.0f && ldq % 8 == 0 && ldo % 4 == 0 && aligned(q, 16) && aligned(out, 8) && aligned(k_pages, 16) && aligned(v_pages, 16) &&
+        (workspace || g_paged_part) && iris_hip_paged_hd128_takes(pages, shift, table_ld, sequences, heads, kv_heads)) {
+        g_last_kernel = "fa_paged_hd128";
+        LAUNCH("attention_paged", iris_hip_paged_hd128(g_stream, workspace ? workspace : g_paged_part, out, ldo, q, ldq, k_pages, v_pages, k_scales, v_scales,
+                                                       pages, shift, page_table, table_ld, lengths, sequences, heads, kv_heads, scale));
         return;
     }
     g_last_kernel = "attention_paged_generic";
