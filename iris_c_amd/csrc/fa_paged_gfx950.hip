@@ -360,12 +360,14 @@ k_paged_hd128(Args a) {
     }
 }
 
-/* Workgroup w joins the list entry that the end of range w cuts, if it is the first end in it. A wave takes every fourth part, for all
- * columns a pair of dims to a lane; the LDS joins the waves. */
-__global__ void __launch_bounds__(256)
+/* Workgroup w joins the list entry that the end of range w cuts, if it is the first end in it. 32 lanes take 4 dims each of a column and
+ * every so many-th part, eight at a time so that their loads are under way together; the LDS joins what several groups of 32 have. */
+constexpr int JOIN = 512;
+__global__ void __launch_bounds__(JOIN)
 k_paged_join(Args a, int keys) {
-    __shared__ float sums[4][HD], tops[4], dens[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = blockIdx.x, per = a.cache.kv_heads * a.blocks;
+    __shared__ f32x4 sums[JOIN];
+    __shared__ float tops[JOIN / 32], dens[JOIN / 32];
+    const int w = blockIdx.x, per = a.cache.kv_heads * a.blocks;
     Work work;
     const int total = work.count(a.cache, a.n, per, keys), waves = ranges(total, gridDim.x);
     if (w + 1 >= waves) return;
@@ -376,35 +378,55 @@ k_paged_join(Args a, int keys) {
     if (first == u || first < range_begin(total, w, waves)) return;
     const int last = range_of(total, first + tiles - 1, waves);
     const int kvh = entry / a.blocks, block = entry - kvh * a.blocks, cols = min(COLS, a.group - block * COLS);
-    for (int c = 0; c < cols; c++) {
-        float top = -INFINITY, den = 0.0f;
-        f32x2 sum = {0.0f, 0.0f};
-        for (int i = w + wave; i <= last; i += 4) {
-            const float *pp = a.part + (size_t)(2 * i + (i == w)) * PART;
-            const float t = pp[COLS * HD + c], d = pp[COLS * HD + COLS + c];
-            const f32x2 o = *reinterpret_cast<const f32x2 *>(pp + c * HD + 2 * lane);
-            const float now = fmaxf(top, t), base = now == -INFINITY ? 0.0f : now;
-            const float fa = __builtin_amdgcn_exp2f(top - base), fb = __builtin_amdgcn_exp2f(t - base);
-            sum[0] = sum[0] * fa + o[0] * fb;
-            sum[1] = sum[1] * fa + o[1] * fb;
-            den = den * fa + d * fb;
+    const int places = cols <= 1 ? 1 : cols <= 2 ? 2 : cols <= 4 ? 4 : cols <= 8 ? 8 : 16, groups = JOIN / 32 / places;     /* per column */
+    const int unit = threadIdx.x >> 5, c = unit & (places - 1), part = unit / places, at = threadIdx.x & 31;
+    float top = -INFINITY, den = 0.0f;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c < cols) {
+        for (int i0 = w + part; i0 <= last; i0 += 8 * groups) {
+            float t[8], d[8];
+            f32x4 o[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int i = min(i0 + j * groups, last);
+                const float *pp = a.part + (size_t)(2 * i + (i == w)) * PART;
+                t[j] = i0 + j * groups <= last ? pp[COLS * HD + c] : -INFINITY;
+                d[j] = pp[COLS * HD + COLS + c];
+                o[j] = *reinterpret_cast<const f32x4 *>(pp + c * HD + 4 * at);
+            }
+            float now = top;
+#pragma unroll
+            for (int j = 0; j < 8; j++) now = fmaxf(now, t[j]);
+            const float base = now == -INFINITY ? 0.0f : now, alpha = __builtin_amdgcn_exp2f(top - base);
+            sum *= alpha;
+            den *= alpha;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (i0 + j * groups > last) break;
+                const float f = __builtin_amdgcn_exp2f(t[j] - base);
+                sum += o[j] * f;
+                den += d[j] * f;
+            }
             top = now;
         }
-        __syncthreads();
-        sums[wave][2 * lane] = sum[0];
-        sums[wave][2 * lane + 1] = sum[1];
-        if (lane == 0) { tops[wave] = top; dens[wave] = den; }
-        __syncthreads();
-        if (wave == 0) {
-            const float now = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), base = now == -INFINITY ? 0.0f : now;
-            float d = 0.0f, x = 0.0f, y = 0.0f;
-            for (int i = 0; i < 4; i++) {
-                const float f = __builtin_amdgcn_exp2f(tops[i] - base);
-                d += dens[i] * f; x += sums[i][2 * lane] * f; y += sums[i][2 * lane + 1] * f;
-            }
-            const float inv = d > 0.0f ? 1.0f / d : 0.0f;
-            *reinterpret_cast<uint32_t *>(a.out + (size_t)g * a.ldo + (size_t)(kvh * a.group + block * COLS + c) * HD + 2 * lane) = pack_bf16(x * inv, y * inv);
+    }
+    sums[threadIdx.x] = sum;
+    if (at == 0) { tops[unit] = top; dens[unit] = den; }
+    __syncthreads();
+    if (part == 0 && c < cols) {
+        float now = top;
+        for (int j = 1; j < groups; j++) now = fmaxf(now, tops[c + j * places]);
+        const float base = now == -INFINITY ? 0.0f : now, alpha = __builtin_amdgcn_exp2f(top - base);
+        sum *= alpha;
+        den *= alpha;
+        for (int j = 1; j < groups; j++) {
+            const float f = __builtin_amdgcn_exp2f(tops[c + j * places] - base);
+            sum += sums[threadIdx.x + 32 * places * j] * f;
+            den += dens[c + j * places] * f;
         }
+        const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+        *reinterpret_cast<uint2 *>(a.out + (size_t)g * a.ldo + (size_t)(kvh * a.group + block * COLS + c) * HD + 4 * at) =
+            make_uint2(pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv));
     }
 }
 
@@ -429,6 +451,6 @@ extern "C" int iris_hip_paged_hd128(void *stream, float *part, uint16_t *out, in
     const int waves = tiles / 2 < 1 ? 1 : tiles / 2 < MOST_WAVES ? (int)(tiles / 2) : MOST_WAVES;
     if (ks) hipLaunchKernelGGL(k_paged_hd128<true>, dim3(waves), dim3(64), STAGES * Shape<true>::STAGE, (hipStream_t)stream, a);
     else hipLaunchKernelGGL(k_paged_hd128<false>, dim3(waves), dim3(64), STAGES * Shape<false>::STAGE, (hipStream_t)stream, a);
-    if (waves > 1) hipLaunchKernelGGL(k_paged_join, dim3(waves), dim3(256), 0, (hipStream_t)stream, a, keys);
+    if (waves > 1) hipLaunchKernelGGL(k_paged_join, dim3(waves), dim3(JOIN), 0, (hipStream_t)stream, a, keys);
     return (int)hipGetLastError();
 }
