@@ -288,7 +288,8 @@ void iris_dev_attention_sequences(uint16_t *out, int ldo, const uint16_t *q, int
  * position lengths[g] - n + i; positions below 0, and those that the table does not reach, are left out. first_row NULL: row g is the one
  * row of sequence g (rows == sequences), the newest token of each. No two rows of a call may go to the same place.
  * Quantised, the scale of a row is the smallest power of two (at least 2^-127) that its largest magnitude is at most 448 times of, its
- * codes the nearest ones to value / scale, ties to the even code; a row with an infinity or a NaN in it becomes NaN as a whole. */
+ * codes the nearest ones to value / scale, ties to the even code; a row with an infinity or a NaN in it becomes NaN as a whole
+ * (scale 255, codes 0x7f, which is NaN too). */
 void iris_dev_cache_write_bf16(uint16_t *k_pages, uint16_t *v_pages, int pages, int page_size, const int *page_table, int table_ld,
                                const int *lengths, const uint16_t *k, const uint16_t *v, int ld, const int *first_row, int sequences,
                                int rows, int kv_heads, int head_dim);

@@ -5,7 +5,7 @@
  * least 2^-127; the codes are x / 2^e rounded to the nearest code, ties to the even one. Dividing by a power of two is exact, so that
  * one rounding is the only one, at most half a step, 2^-4 of the value (2^-10 of 2^e below 2^-6 of it), and no value saturates. From
  * the bits of the largest magnitude, sign off: e = exponent - 8, one more where its fraction is above .75. A row with an infinity or a
- * NaN in it becomes NaN as a whole (scale byte 255, codes 0).
+ * NaN in it becomes NaN as a whole (scale byte 255, all codes 0x7f).
  *
  * The rows of a call are the last ones of their sequences: row i of n is position length - n + i. A workgroup takes ROWS rows of one
  * sequence, of K or of V. Bound by memory: each value is read and written once.
@@ -27,13 +27,6 @@ constexpr int ROWS = 16, THREADS = 256;
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const f32x2 p = {lo, hi};
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(p, bf16x2));
-}
-
-/* the scale byte of a row whose largest magnitude has these bf16 bits (sign off), and what its values are multiplied by */
-__device__ __forceinline__ unsigned scale_byte(unsigned top, float *factor) {
-    const int exponent = (int)(top >> 7), e = max(exponent - 135 + ((top & 0x7f) > 0x60), -127);
-    *factor = e == -127 ? __uint_as_float(0x7f000000u) : __uint_as_float((unsigned)(127 - e) << 23);
-    return exponent == 255 ? 255 : (unsigned)(e + 127);
 }
 
 /* position of row `row` of the sequence, or -1 where the cache has no place for it */
@@ -84,7 +77,7 @@ k_cache_rows(Pair pages, Pair scales, ConstPair rows, Pair out, int ld, PagedArg
                 const float lo = __uint_as_float(w[i] << 16) * factor, hi = __uint_as_float(w[i] & 0xffff0000u) * factor;
                 c[i / 2] = i % 2 ? __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, c[i / 2], true) : __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, c[i / 2], false);
             }
-            *reinterpret_cast<int2 *>(codes + in_pages) = byte == 255 ? make_int2(0, 0) : make_int2(c[0], c[1]);
+            *reinterpret_cast<int2 *>(codes + in_pages) = byte == 255 ? make_int2(0x7f7f7f7f, 0x7f7f7f7f) : make_int2(c[0], c[1]);
             if (lane == 0) bytes[place] = (uint8_t)byte;
         } else {
             const int2 c = *reinterpret_cast<const int2 *>(codes + in_pages);
@@ -133,7 +126,7 @@ k_cache_rows_any(Pair pages, Pair scales, ConstPair rows, Pair out, int ld, Page
             const unsigned byte = scale_byte(top, &factor);
             for (int d = lane; d < hd; d += 64) {
                 const int c = __builtin_amdgcn_cvt_pk_fp8_f32(__uint_as_float((uint32_t)from[at + d] << 16) * factor, 0.0f, 0, false);
-                codes[in_pages + d] = byte == 255 ? (uint8_t)0 : (uint8_t)c;
+                codes[in_pages + d] = byte == 255 ? (uint8_t)0x7f : (uint8_t)c;
             }
             if (lane == 0) bytes[place] = (uint8_t)byte;
         } else {

@@ -27,6 +27,7 @@
  */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "iris_kernels_hip.h"
 #include "paged_cache.h"
@@ -37,6 +38,8 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -71,38 +74,57 @@ template <class F> __device__ __forceinline__ float over_column(float v, F f) {
     return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-/* The list of tiles: sequence g has tiles(g) * per of them, per = kv_heads * blocks of 16 query heads */
+/* The list of tiles: sequence g has tiles(g) * per of them, per = kv_heads * blocks of 16 query heads. Looked at 256 sequences at a time,
+ * four to a lane, so that their lengths are one trip to memory. */
 struct Work {
     PagedArg cache;
     int n, per, keys;                            /* keys of a tile */
-    int lane_tiles, upto, total;                 /* this lane's sequence of the last 64 looked at */
+    int length[4], upto[4], total;               /* this lane's sequences of the last 256 looked at: tokens, and tiles with all in front */
 
     __device__ __forceinline__ void look(int base) {
-        const int g = base + (threadIdx.x & 63);
-        lane_tiles = g < n ? (int)(((long)paged_length(cache, g) + keys - 1) / keys) : 0;
-        upto = total + wave_sum_upto(lane_tiles * per);
-        total = __builtin_amdgcn_readlane(upto, 63);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int g = base + 64 * i + (threadIdx.x & 63);
+            length[i] = cache.lengths[min(g, n - 1)];
+        }
+        const long most = (long)cache.ld << cache.shift;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            length[i] = base + 64 * i + (int)(threadIdx.x & 63) < n ? (int)min((long)max(length[i], 0), most) : 0;
+            upto[i] = total + wave_sum_upto(tiles(length[i]) * per);
+            total = __builtin_amdgcn_readlane(upto[i], 63);
+        }
     }
+    __device__ __forceinline__ int tiles(int tokens) const { return (tokens + keys - 1) / keys; }
     __device__ __forceinline__ int count(const PagedArg &c, int sequences, int per_tile, int tile_keys) {
         cache = c; n = sequences; per = per_tile; keys = tile_keys; total = 0;
-        for (int base = 0; base < n; base += 64) look(base);
+        for (int base = 0; base < n; base += 256) look(base);
         return total;
     }
-    /* the sequence of tile u < count(): its number, tiles, and the tiles in front of it */
-    __device__ __forceinline__ void find(int u, int *g, int *tiles, int *before) {
+    /* the sequence of tile u < count(): its number, tokens, the tiles of a list entry, and those in front of it */
+    __device__ __forceinline__ void find(int u, int *g, int *tokens, int *entry, int *before) {
         int base = 0;
-        if (n > 64) {
+        if (n > 256) {
             total = 0;
-            for (; base < n; base += 64) {
+            for (; base < n; base += 256) {
                 look(base);
                 if (u < total) break;
             }
         }
-        const unsigned long long past = __ballot(upto > u);
-        const int at = past ? __ffsll(past) - 1 : 0;
-        *g = base + at;
-        *tiles = __builtin_amdgcn_readlane(lane_tiles, at);
-        *before = __builtin_amdgcn_readlane(upto, at) - *tiles * per;
+        *g = *before = *tokens = 0; *entry = 1;
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const unsigned long long past = __ballot(upto[i] > u);
+            if (past && !found) {
+                const int at = __ffsll(past) - 1;
+                found = true;
+                *g = base + 64 * i + at;
+                *tokens = __builtin_amdgcn_readlane(length[i], at);
+                *entry = tiles(*tokens);
+                *before = __builtin_amdgcn_readlane(upto[i], at) - *entry * per;
+            }
+        }
     }
 };
 
@@ -131,56 +153,111 @@ __device__ __forceinline__ void load_16(uint32_t lds, const unsigned char *src) 
 __device__ __forceinline__ void load_byte(uint32_t lds, const unsigned char *src) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
 }
+/* a dword of each lane */
+__device__ __forceinline__ void load_word(uint32_t lds, const void *src) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
+}
 #pragma clang diagnostic pop
+/* Stores that are counted with the loads behind which they are issued; the compiler might make fewer of them */
+__device__ __forceinline__ void store_8(void *p, uint2 v) {
+    const u32x2 w = {v.x, v.y};
+    asm volatile("global_store_dwordx2 %0, %1, off" ::"v"(p), "v"(w) : "memory");
+}
+__device__ __forceinline__ void store_16(void *p, f32x4 v) {         /* the wait states in front of the next write of its registers */
+    asm volatile("global_store_dwordx4 %0, %1, off\n\ts_nop 1" ::"v"(p), "v"(v) : "memory");
+}
+constexpr int STORES = 8;                                            /* of a column's result, at least */
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-/* The sums of 16 columns over keys: O^T as dims 16 db + 4 lg + r of column li, its maximum, and this lane's part of the denominator */
-struct State { f32x4 o[8]; float top, sum; };
+/* A tile that has been asked for: the keys of it that count, and what it belongs to */
+struct Tile {
+    unsigned long long seen;
+    int g, head, cols;                           /* sequence, first query head, query heads (at most 16) */
+    bool begin, end, from_start, whole;          /* first and last of its list entry in this range; the entry began here; and ended here */
+};
 
-/* The keys [tile0, tile1) * KEYS of a sequence's kv head */
-template <bool FP8>
-__device__ __forceinline__ void walk(State &st, const Args &a, unsigned char *lds, int g, int kvh, int block, int tile0, int tile1) {
+template <bool FP8, int QROWS>
+__global__ void __launch_bounds__(64, 2)                              /* 256 registers: the products then leave their results in vector registers */
+k_paged_hd128(Args a) {
     typedef Shape<FP8> S;
-    const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
-    const int length = paged_length(a.cache, g), shift = a.cache.shift;
+    extern __shared__ __align__(16) unsigned char lds[];              /* two stages, Q of two list entries, pages of two runs of 64 */
+    constexpr int Q0 = STAGES * S::STAGE, Q_BYTES = QROWS * 2 * HD, P0 = Q0 + 2 * Q_BYTES;
+    const int lane = threadIdx.x, li = lane & 15, lg = lane >> 4, w = blockIdx.x, per = a.cache.kv_heads * a.blocks, shift = a.cache.shift;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)lds);
+    Work work;
+    const int total = work.count(a.cache, a.n, per, S::KEYS), waves = ranges(total, gridDim.x);
+    for (int g = w; g < a.n; g += gridDim.x)                         /* sequences without keys */
+        if (paged_length(a.cache, g) == 0)
+            for (int c = lane; c < a.group * a.cache.kv_heads * (HD / 4); c += 64)
+                *reinterpret_cast<uint2 *>(a.out + (size_t)g * a.ldo + 4 * (size_t)c) = make_uint2(0, 0);
+    if (w >= waves) return;
+    const int begin = range_begin(total, w, waves), end = range_begin(total, w + 1, waves);
+    if (begin == end) return;                                        /* no keys at all */
 
-    /* Q^T: lane (li, lg) holds 8 dims of column li for each of four steps of 32: dims 32 ks + 8 lg, and with rows of 8 bits, whose 16-byte
-     * reads carry two steps, 64 (ks / 2) + 16 lg + 8 (ks % 2) */
-    bf16x8 qb[4];
-    {
-        const int col = block * COLS + li;
-        const uint16_t *qp = a.q + (size_t)g * a.ldq + (size_t)(kvh * a.group + min(col, a.group - 1)) * HD;
-#pragma unroll
-        for (int ks = 0; ks < 4; ks++) {
-            u32x4 w = *reinterpret_cast<const u32x4 *>(qp + (FP8 ? 64 * (ks >> 1) + 16 * lg + 8 * (ks & 1) : 32 * ks + 8 * lg));
-            if (col >= a.group) w = u32x4{0, 0, 0, 0};
-            qb[ks] = __builtin_bit_cast(bf16x8, w);
-        }
-    }
+    /* the tile that is asked for next */
+    int u = begin, g, length, tiles, before, q_turn = 0;
+    work.find(u, &g, &length, &tiles, &before);
+    int entry = (u - before) / tiles, tile = u - before - entry * tiles, kvh = entry / a.blocks, block = entry - kvh * a.blocks;
+    bool from_start = false;
 
-    /* the pages of the next 64 page-fuls of tokens, one to a lane, from the one that the tile asked for begins in */
-    int page_base = (tile0 * S::KEYS) >> shift, page_id;
-    auto look_up = [&]() {
-        const int at = page_base + lane;
-        page_id = at < a.cache.ld ? a.cache.table[(size_t)g * a.cache.ld + at] : -1;
+    /* The pages of 64 page-fuls of tokens, from the one that a tile begins in. Those that the next tile needs are asked for in front of
+     * the loads of the tile before it: whoever waits for that tile has them. */
+    int run_g = g, run_page = tile * S::KEYS >> shift, run = 0;
+    auto ask_pages = [&]() {
+        const int at = run_page + lane;
+        load_word(lds0 + P0 + 256 * run, at < a.cache.ld ? (const void *)(a.cache.table + (size_t)run_g * a.cache.ld + at) : (const void *)zeros);
     };
-    look_up();
+    ask_pages();
+    wait_loads<0>();
 
-    unsigned long long seen[STAGES];                                 /* the keys of the tile in each stage that count */
-    auto request = [&](int tile, int stage) {
+    /* asks for tile u, steps to the next one; whether that one's pages have been asked for just now */
+    auto request = [&](Tile &t, int stage) -> bool {
         const int k0 = tile * S::KEYS;
-        if (((k0 + S::KEYS - 1) >> shift) - page_base >= 64) {
-            page_base = k0 >> shift;
-            look_up();
-        }
+        t.g = g;
+        t.head = kvh * a.group + block * COLS;
+        t.cols = min(COLS, a.group - block * COLS);
+        t.begin = u == begin || tile == 0;
+        if (t.begin) from_start = tile == 0;
+        t.from_start = from_start;
+        t.end = u + 1 == end || tile + 1 == tiles;
+        t.whole = from_start && tile + 1 == tiles;
+
         const int pos = k0 + (lane & (S::KEYS - 1));
-        const int page = __shfl(page_id, (pos >> shift) - page_base, 64);
-        const bool there = pos < length && (unsigned)page < (unsigned)a.cache.pages;
-        const unsigned row = there ? (((unsigned)page * (unsigned)a.cache.kv_heads + (unsigned)kvh) << shift) + ((unsigned)pos & ((1u << shift) - 1)) : NO_ROW;
+        const unsigned page = reinterpret_cast<const unsigned *>(lds + P0 + 256 * run)[(pos >> shift) - run_page];
+        const bool there = pos < length && page < (unsigned)a.cache.pages;
+        const unsigned row = there ? ((page * (unsigned)a.cache.kv_heads + (unsigned)kvh) << shift) + ((unsigned)pos & ((1u << shift) - 1)) : NO_ROW;
         const unsigned long long word = __ballot(there);
-        seen[stage] = S::KEYS == 64 ? word : word & 0xffffffffu;
+        t.seen = S::KEYS == 64 ? word : word & 0xffffffffu;
+
+        /* step, and ask for the next one's pages where they are not those that are here */
+        u++; tile++;
+        bool asked = false;
+        if (u < end) {
+            if (tile == tiles) {
+                tile = 0;
+                if (++block == a.blocks) { block = 0; kvh++; }
+                if (kvh == a.cache.kv_heads) {
+                    kvh = 0;
+                    work.find(u, &g, &length, &tiles, &before);
+                }
+            }
+            const int from = tile * S::KEYS >> shift, to = (tile * S::KEYS + S::KEYS - 1) >> shift;
+            if (g != run_g || from < run_page || to >= run_page + 64) {
+                run_g = g; run_page = from; run ^= 1;
+                ask_pages();
+                asked = true;
+            }
+        }
+        if (t.begin) {
+#pragma unroll
+            for (int j = 0; j < QROWS / 4; j++) {
+                const int r = 4 * j + (lane >> 4);
+                load_16(lds0 + Q0 + Q_BYTES * q_turn + 1024 * j,
+                        r < t.cols ? (const unsigned char *)(a.q + (size_t)t.g * a.ldq + (size_t)(t.head + r) * HD + 8 * (lane & 15)) : zeros);
+            }
+            q_turn ^= 1;
+        }
         const uint32_t dst = lds0 + stage * S::STAGE;
         constexpr int LANES = S::ROW / 16;                           /* to a row */
 #pragma unroll
@@ -196,12 +273,15 @@ __device__ __forceinline__ void walk(State &st, const Args &a, unsigned char *ld
             load_byte(dst + 2 * S::HALF, row == NO_ROW ? zeros : a.ks + row);
             load_byte(dst + 2 * S::HALF + 256, row == NO_ROW ? zeros : a.vs + row);
         }
+        return asked;
     };
 
-#pragma unroll
-    for (int db = 0; db < 8; db++) st.o[db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    st.top = -INFINITY; st.sum = 0.0f;
-    float base = 0.0f;                                               /* the maximum, 0 where it is -infinity */
+    /* O^T: dims 16 db + 4 lg + r of column li; the column's maximum, and this lane's part of the denominator */
+    f32x4 o[8];
+    float top = 0.0f, sum = 0.0f, base = 0.0f;                       /* base: the maximum, 0 where it is -infinity */
+    bf16x8 qb[4];                                                    /* Q^T in bf16, or in two parts of 8 bits and their scale */
+    i32x8 q_hi, q_lo;
+    int q_scale = 0, q_read = 0;
 
     /* where a lane reads, from the start of K or V in a stage */
     int k_rd[4], v_rd[8];
@@ -215,52 +295,84 @@ __device__ __forceinline__ void walk(State &st, const Args &a, unsigned char *ld
                                                      : 16 * ((2 * db + ((li & 3) >> 1)) ^ swizzle<FP8>(row)) + 8 * (li & 1));
     }
 
-    request(tile0, 0);
-    if (tile0 + 1 < tile1) request(tile0 + 1, 1);
-    for (int t = tile0; t < tile1; t++) {
-        const int stage = (t - tile0) & 1;
+    Tile now, next;
+    bool stored = false;
+    const bool asked = request(now, 0);
+    if (begin + 1 < end) {
+        if (asked) wait_loads<0>();
+        request(next, 1);
+    }
+    for (int t = begin, stage = 0; t < end; t++, stage ^= 1) {
         const unsigned char *cur = lds + stage * S::STAGE;
-        if (t + 1 < tile1) wait_loads<S::LOADS>();
-        else wait_loads<0>();
+        /* all but the next tile's, and the stores of the last result if there was one: this tile, its Q, the pages of the one after the next */
+        if (t + 1 == end) wait_loads<0>();
+        else if (stored) wait_loads<S::LOADS + STORES>();
+        else wait_loads<S::LOADS>();
+        stored = now.end;
+        if (now.begin) {
+            const unsigned char *qp = lds + Q0 + Q_BYTES * q_read + (li & (QROWS - 1)) * 2 * HD;
+            if constexpr (FP8) {
+                /* lane (li, lg) holds dims 16 lg .. + 15 and 64 + 16 lg .. + 15 of column li */
+                u32x4 x[4];
+                unsigned most = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    x[i] = *reinterpret_cast<const u32x4 *>(qp + 128 * (i >> 1) + 32 * lg + 16 * (i & 1));
+                    if (QROWS < COLS && li >= QROWS) x[i] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) most = max(most, max(x[i][j] & 0x7fff, (x[i][j] >> 16) & 0x7fff));
+                }
+                most = max(most, (unsigned)__shfl_xor((int)most, 16, 64));      /* one scale for the column: a lane's 32 values are of two blocks */
+                most = max(most, (unsigned)__shfl_xor((int)most, 32, 64));
+                float factor;
+                q_scale = (int)scale_byte(most, &factor);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    int hi = 0, lo = 0;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t word = x[i >> 1][2 * (i & 1) + h];
+                        const float c0 = __uint_as_float(word << 16) * factor, c1 = __uint_as_float(word & 0xffff0000u) * factor;
+                        hi = h ? __builtin_amdgcn_cvt_pk_fp8_f32(c0, c1, hi, true) : __builtin_amdgcn_cvt_pk_fp8_f32(c0, c1, hi, false);
+                        const f32x2 back = h ? __builtin_amdgcn_cvt_pk_f32_fp8(hi, true) : __builtin_amdgcn_cvt_pk_f32_fp8(hi, false);
+                        lo = h ? __builtin_amdgcn_cvt_pk_fp8_f32(c0 - back[0], c1 - back[1], lo, true) : __builtin_amdgcn_cvt_pk_fp8_f32(c0 - back[0], c1 - back[1], lo, false);
+                    }
+                    q_hi[i] = hi; q_lo[i] = lo;
+                }
+            } else {
+                /* lane (li, lg) holds dims 32 ks + 8 lg .. + 7 of column li */
+#pragma unroll
+                for (int ks = 0; ks < 4; ks++) {
+                    u32x4 x = *reinterpret_cast<const u32x4 *>(qp + 64 * ks + 16 * lg);
+                    if (QROWS < COLS && li >= QROWS) x = u32x4{0, 0, 0, 0};
+                    qb[ks] = __builtin_bit_cast(bf16x8, x);
+                }
+            }
+            q_read ^= 1;
+#pragma unroll
+            for (int db = 0; db < 8; db++) o[db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            top = -INFINITY; sum = 0.0f; base = 0.0f;
+        }
         constexpr int MB = S::KEYS / 16;
-        f32x4 s[MB];
+        f32x4 s[MB];                                                 /* key 16 mb + 4 lg + r against column li, in units of log2 */
 #pragma unroll
         for (int mb = 0; mb < MB; mb++) {
             f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
             if constexpr (FP8) {
-#pragma unroll
-                for (int p = 0; p < 2; p++) {
-                    const u32x4 w = *reinterpret_cast<const u32x4 *>(cur + (k_rd[p] ^ 16 * (mb & 1)) + 16 * mb * S::ROW);     /* swizzle(16 mb + li) */
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const bf16x2 c0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * e], 1.0f, false), c1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * e], 1.0f, true);
-                        const bf16x2 c2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * e + 1], 1.0f, false), c3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * e + 1], 1.0f, true);
-                        const bf16x8 ka = {c0[0], c0[1], c1[0], c1[1], c2[0], c2[1], c3[0], c3[1]};
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qb[2 * p + e], acc, 0, 0, 0);
-                    }
-                }
+                const u32x4 k0 = *reinterpret_cast<const u32x4 *>(cur + (k_rd[0] ^ 16 * (mb & 1)) + 16 * mb * S::ROW);        /* swizzle(16 mb + li) */
+                const u32x4 k1 = *reinterpret_cast<const u32x4 *>(cur + (k_rd[1] ^ 16 * (mb & 1)) + 16 * mb * S::ROW);
+                const i32x8 ka = __builtin_bit_cast(i32x8, __builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7));
+                const int scale = *reinterpret_cast<const int *>(cur + 2 * S::HALF + 4 * (16 * mb + li));
+                acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ka, q_lo, acc, 0, 0, 0, scale, 0, q_scale);
+                acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ka, q_hi, acc, 0, 0, 0, scale, 0, q_scale);
             } else {
 #pragma unroll
                 for (int ks = 0; ks < 4; ks++)
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8 *>(cur + k_rd[ks] + 16 * mb * S::ROW), qb[ks], acc, 0, 0, 0);
             }
-            s[mb] = acc;
+            s[mb] = acc * a.scale_log2;
         }
-        /* key 16 mb + 4 lg + r against column li, in units of log2 */
-        float high = -INFINITY, vscale[MB][4];
-#pragma unroll
-        for (int mb = 0; mb < MB; mb++) {
-            float f[4] = {a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2};
-            if constexpr (FP8) {
-                const u32x4 kb = *reinterpret_cast<const u32x4 *>(cur + 2 * S::HALF + 4 * (16 * mb + 4 * lg));
-                const u32x4 vb = *reinterpret_cast<const u32x4 *>(cur + 2 * S::HALF + 256 + 4 * (16 * mb + 4 * lg));
-#pragma unroll
-                for (int r = 0; r < 4; r++) { f[r] *= paged_scale(kb[r]); vscale[mb][r] = paged_scale(vb[r]); }
-            }
-#pragma unroll
-            for (int r = 0; r < 4; r++) s[mb][r] *= f[r];
-        }
-        const unsigned long long all = S::KEYS == 64 ? ~0ull : 0xffffffffull, mine = seen[stage];
+        const unsigned long long all = S::KEYS == 64 ? ~0ull : 0xffffffffull, mine = now.seen;
         if (mine != all) {
 #pragma unroll
             for (int mb = 0; mb < MB; mb++)
@@ -268,16 +380,17 @@ __device__ __forceinline__ void walk(State &st, const Args &a, unsigned char *ld
                 for (int r = 0; r < 4; r++)
                     if (!((mine >> (16 * mb + 4 * lg + r)) & 1ull)) s[mb][r] = -INFINITY;
         }
+        float high = -INFINITY;
 #pragma unroll
         for (int mb = 0; mb < MB; mb++) high = fmaxf(fmaxf(fmaxf(high, s[mb][0]), fmaxf(s[mb][1], s[mb][2])), s[mb][3]);
-        if (__any(high > st.top + RAISE)) {                          /* the first tile: -infinity + 8 */
-            const float now = fmaxf(st.top, over_column(high, [](float x, float y) { return fmaxf(x, y); }));
-            base = now == -INFINITY ? 0.0f : now;
-            const float alpha = __builtin_amdgcn_exp2f(st.top - base);
-            st.top = now;
-            st.sum *= alpha;
+        if (__any(high > top + RAISE)) {                          /* the first tile: -infinity + 8 */
+            const float peak = fmaxf(top, over_column(high, [](float x, float y) { return fmaxf(x, y); }));
+            base = peak == -INFINITY ? 0.0f : peak;
+            const float alpha = __builtin_amdgcn_exp2f(top - base);
+            top = peak;
+            sum *= alpha;
 #pragma unroll
-            for (int db = 0; db < 8; db++) st.o[db] *= alpha;
+            for (int db = 0; db < 8; db++) o[db] *= alpha;
         }
         u32x4 pw[MB / 2];
 #pragma unroll
@@ -288,10 +401,11 @@ __device__ __forceinline__ void walk(State &st, const Args &a, unsigned char *ld
                 p[r] = __builtin_amdgcn_exp2f(s[2 * kg][r] - base);
                 p[4 + r] = __builtin_amdgcn_exp2f(s[2 * kg + 1][r] - base);
             }
-            st.sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
             if constexpr (FP8) {
+                const u32x4 v0 = *reinterpret_cast<const u32x4 *>(cur + 2 * S::HALF + 256 + 4 * (32 * kg + 4 * lg)), v1 = *reinterpret_cast<const u32x4 *>(cur + 2 * S::HALF + 256 + 4 * (32 * kg + 16 + 4 * lg));
 #pragma unroll
-                for (int r = 0; r < 4; r++) { p[r] *= vscale[2 * kg][r]; p[4 + r] *= vscale[2 * kg + 1][r]; }
+                for (int r = 0; r < 4; r++) { p[r] = ldexpf(p[r], (int)v0[r] - 127); p[4 + r] = ldexpf(p[4 + r], (int)v1[r] - 127); }
             }
             pw[kg] = u32x4{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])};
         }
@@ -311,52 +425,28 @@ __device__ __forceinline__ void walk(State &st, const Args &a, unsigned char *ld
                     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(vp + 16 * S::ROW));
                     va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
                 }
-                st.o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, pw[kg]), st.o[db], 0, 0, 0);
+                o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, pw[kg]), o[db], 0, 0, 0);
             }
         wait_lds();                                                  /* this stage has been read */
-        if (t + 2 < tile1) request(t + 2, stage);
-    }
-    st.sum = over_column(st.sum, [](float x, float y) { return x + y; });
-}
-
-template <bool FP8>
-__global__ void __launch_bounds__(64, 1)
-k_paged_hd128(Args a) {
-    extern __shared__ __align__(16) unsigned char lds[];
-    const int lane = threadIdx.x, li = lane & 15, lg = lane >> 4, w = blockIdx.x, per = a.cache.kv_heads * a.blocks;
-    Work work;
-    const int total = work.count(a.cache, a.n, per, Shape<FP8>::KEYS), waves = ranges(total, gridDim.x);
-    for (int g = w; g < a.n; g += gridDim.x)                         /* sequences without keys */
-        if (paged_length(a.cache, g) == 0)
-            for (int c = lane; c < a.group * a.cache.kv_heads * (HD / 4); c += 64)
-                *reinterpret_cast<uint2 *>(a.out + (size_t)g * a.ldo + 4 * (size_t)c) = make_uint2(0, 0);
-    if (w >= waves) return;
-    int u = range_begin(total, w, waves);
-    const int end = range_begin(total, w + 1, waves);
-    while (u < end) {
-        int g, tiles, before;
-        work.find(u, &g, &tiles, &before);
-        do {                                                         /* the list entries of this sequence */
-            const int entry = (u - before) / tiles, tile0 = u - before - entry * tiles, tile1 = min(tiles, tile0 + end - u);
-            const int kvh = entry / a.blocks, block = entry - kvh * a.blocks, cols = min(COLS, a.group - block * COLS);
-            State st;
-            walk<FP8>(st, a, lds, g, kvh, block, tile0, tile1);
-            if (li < cols) {
-                if (tile1 - tile0 == tiles) {
-                    const float inv = st.sum > 0.0f ? 1.0f / st.sum : 0.0f;
-                    uint16_t *op = a.out + (size_t)g * a.ldo + (size_t)(kvh * a.group + block * COLS + li) * HD + 4 * lg;
+        const Tile done = now;
+        now = next;
+        if (t + 2 < end) request(next, stage);
+        if (!done.end) continue;
+        const float den = over_column(sum, [](float x, float y) { return x + y; });
+        if (li < done.cols && done.whole) {
+            const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+            uint16_t *op = a.out + (size_t)done.g * a.ldo + (size_t)(done.head + li) * HD + 4 * lg;
 #pragma unroll
-                    for (int db = 0; db < 8; db++)
-                        *reinterpret_cast<uint2 *>(op + 16 * db) = make_uint2(pack_bf16(st.o[db][0] * inv, st.o[db][1] * inv), pack_bf16(st.o[db][2] * inv, st.o[db][3] * inv));
-                } else {
-                    float *pp = a.part + (size_t)(2 * w + (tile0 == 0)) * PART;
+            for (int db = 0; db < 8; db++)
+                store_8(op + 16 * db, make_uint2(pack_bf16(o[db][0] * inv, o[db][1] * inv), pack_bf16(o[db][2] * inv, o[db][3] * inv)));
+        } else if (li < done.cols) {
+            float *pp = a.part + (size_t)(2 * w + done.from_start) * PART;
+            /* the products have left the matrix cores: the compiler places no wait states in front of an asm statement */
+            asm volatile("s_nop 15\n\ts_nop 3" : "+v"(o[0]), "+v"(o[1]), "+v"(o[2]), "+v"(o[3]), "+v"(o[4]), "+v"(o[5]), "+v"(o[6]), "+v"(o[7]));
 #pragma unroll
-                    for (int db = 0; db < 8; db++) *reinterpret_cast<f32x4 *>(pp + li * HD + 16 * db + 4 * lg) = st.o[db];
-                    if (lg == 0) { pp[COLS * HD + li] = st.top; pp[COLS * HD + COLS + li] = st.sum; }
-                }
-            }
-            u += tile1 - tile0;
-        } while (u < end && u - before < tiles * per);
+            for (int db = 0; db < 8; db++) store_16(pp + li * HD + 16 * db + 4 * lg, o[db]);
+            if (lg == 0) { pp[COLS * HD + li] = top; pp[COLS * HD + COLS + li] = den; }
+        }
     }
 }
 
@@ -372,8 +462,8 @@ k_paged_join(Args a, int keys) {
     const int total = work.count(a.cache, a.n, per, keys), waves = ranges(total, gridDim.x);
     if (w + 1 >= waves) return;
     const int u = range_begin(total, w + 1, waves);
-    int g, tiles, before;
-    work.find(u, &g, &tiles, &before);
+    int g, length, tiles, before;
+    work.find(u, &g, &length, &tiles, &before);
     const int entry = (u - before) / tiles, first = before + entry * tiles;
     if (first == u || first < range_begin(total, w, waves)) return;
     const int last = range_of(total, first + tiles - 1, waves);
@@ -448,9 +538,19 @@ extern "C" int iris_hip_paged_hd128(void *stream, float *part, uint16_t *out, in
     const Args a = {out, q, (const unsigned char *)k, (const unsigned char *)v, ks, vs, {table, lengths, table_ld, pages, page_shift, kv_heads, HD},
                     ldo, ldq, n, group, blocks, scale * 1.4426950408889634f, part};
     const long tiles = ((((long)table_ld << page_shift) + keys - 1) / keys) * n * kv_heads * blocks;
-    const int waves = tiles / 2 < 1 ? 1 : tiles / 2 < MOST_WAVES ? (int)(tiles / 2) : MOST_WAVES;
-    if (ks) hipLaunchKernelGGL(k_paged_hd128<true>, dim3(waves), dim3(64), STAGES * Shape<true>::STAGE, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(k_paged_hd128<false>, dim3(waves), dim3(64), STAGES * Shape<false>::STAGE, (hipStream_t)stream, a);
+    const int q_rows = group <= 4 ? 4 : group <= 8 ? 8 : 16;          /* with 16 rows of Q for two list entries three waves have room in a CU's LDS */
+    const int most = q_rows == 16 ? MOST_WAVES / 4 * 3 : MOST_WAVES, waves = tiles / 2 < 1 ? 1 : tiles / 2 < most ? (int)(tiles / 2) : most;
+    auto run = [&](auto fp8, auto rows) {
+        constexpr int QROWS = decltype(rows)::value, LDS = STAGES * Shape<decltype(fp8)::value>::STAGE + 2 * QROWS * 2 * HD + 512;
+        hipLaunchKernelGGL((k_paged_hd128<decltype(fp8)::value, QROWS>), dim3(waves), dim3(64), LDS, (hipStream_t)stream, a);
+    };
+    auto run_rows = [&](auto fp8) {
+        if (q_rows == 4) run(fp8, std::integral_constant<int, 4>{});
+        else if (q_rows == 8) run(fp8, std::integral_constant<int, 8>{});
+        else run(fp8, std::integral_constant<int, 16>{});
+    };
+    if (ks) run_rows(std::true_type{});
+    else run_rows(std::false_type{});
     if (waves > 1) hipLaunchKernelGGL(k_paged_join, dim3(waves), dim3(JOIN), 0, (hipStream_t)stream, a, keys);
     return (int)hipGetLastError();
 }

@@ -28,6 +28,14 @@ __device__ __forceinline__ long paged_row(const PagedArg &c, int g, int pos, int
     return (((long)page * c.kv_heads + kvh) << c.shift) + (pos & ((1 << c.shift) - 1));
 }
 
+/* the scale byte of a row whose largest magnitude has these bf16 bits (sign off), the smallest power of two that it is at most 448 times of,
+ * and what the row's values are multiplied by */
+__device__ __forceinline__ unsigned scale_byte(unsigned top, float *factor) {
+    const int exponent = (int)(top >> 7), e = max(exponent - 135 + ((top & 0x7f) > 0x60), -127);
+    *factor = e == -127 ? __uint_as_float(0x7f000000u) : __uint_as_float((unsigned)(127 - e) << 23);
+    return exponent == 255 ? 255 : (unsigned)(e + 127);
+}
+
 __device__ __forceinline__ float paged_scale(unsigned s) {
     return __uint_as_float(s == 255 ? 0x7fc00000u : s ? s << 23 : 0x00400000u);
 }

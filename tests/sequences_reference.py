@@ -44,7 +44,7 @@ def quantise(x):
     lo = np.maximum(hi - 1, 0)
     up, down = E4M3[hi] - r, r - E4M3[lo]
     code = np.where(up < down, hi, np.where(down < up, lo, np.where(hi % 2 == 0, hi, lo))).astype(np.uint8)
-    code = np.where(bad[..., None], 0, code | (np.signbit(x).astype(np.uint8) << 7)).astype(np.uint8)
+    code = np.where(bad[..., None], 0x7f, code | (np.signbit(x).astype(np.uint8) << 7)).astype(np.uint8)
     return code, np.where(bad, 255, e + 127).astype(np.uint8)
 
 
