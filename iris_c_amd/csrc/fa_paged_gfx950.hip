@@ -79,6 +79,7 @@ template <class F> __device__ __forceinline__ float over_column(float v, F f) {
 struct Work {
     PagedArg cache;
     int n, per, keys;                            /* keys of a tile */
+    bool empty;                                  /* there are sequences without tokens */
     int length[4], upto[4], total;               /* this lane's sequences of the last 256 looked at: tokens, and tiles with all in front */
 
     __device__ __forceinline__ void look(int base) {
@@ -91,13 +92,14 @@ struct Work {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             length[i] = base + 64 * i + (int)(threadIdx.x & 63) < n ? (int)min((long)max(length[i], 0), most) : 0;
+            empty = empty || __any(length[i] == 0 && base + 64 * i + (int)(threadIdx.x & 63) < n);
             upto[i] = total + wave_sum_upto(tiles(length[i]) * per);
             total = __builtin_amdgcn_readlane(upto[i], 63);
         }
     }
     __device__ __forceinline__ int tiles(int tokens) const { return (tokens + keys - 1) / keys; }
     __device__ __forceinline__ int count(const PagedArg &c, int sequences, int per_tile, int tile_keys) {
-        cache = c; n = sequences; per = per_tile; keys = tile_keys; total = 0;
+        cache = c; n = sequences; per = per_tile; keys = tile_keys; total = 0; empty = false;
         for (int base = 0; base < n; base += 256) look(base);
         return total;
     }
@@ -128,9 +130,16 @@ struct Work {
     }
 };
 
-/* the tiles of wave w of `waves`, and the wave that has tile u */
-__device__ __forceinline__ int range_begin(int total, int w, int waves) { return (int)((long)total * w / waves); }
-__device__ __forceinline__ int range_of(int total, int u, int waves) { return (int)((((long)u + 1) * waves - 1) / total); }
+/* The tiles in `waves` ranges: `each` or, the first `more` of them, one more. In 32 bits: a 64-bit division takes half a microsecond. */
+struct Ranges {
+    int each, more;
+    __device__ __forceinline__ Ranges(int total, int waves) : each(total / waves) { more = total - each * waves; }
+    __device__ __forceinline__ int begin(int w) const { return w * each + min(w, more); }
+    __device__ __forceinline__ int of(int u) const {                 /* the range that tile u is in */
+        const int front = more * (each + 1);
+        return u < front ? u / (each + 1) : more + (u - front) / each;
+    }
+};
 /* every range has two tiles at least, where there are as many */
 __device__ __forceinline__ int ranges(int total, int most) { return min(most, max(1, total / 2)); }
 
@@ -187,33 +196,45 @@ k_paged_hd128(Args a) {
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)lds);
     Work work;
     const int total = work.count(a.cache, a.n, per, S::KEYS), waves = ranges(total, gridDim.x);
-    for (int g = w; g < a.n; g += gridDim.x)                         /* sequences without keys */
+    for (int g = work.empty ? w : a.n; g < a.n; g += gridDim.x)
         if (paged_length(a.cache, g) == 0)
             for (int c = lane; c < a.group * a.cache.kv_heads * (HD / 4); c += 64)
                 *reinterpret_cast<uint2 *>(a.out + (size_t)g * a.ldo + 4 * (size_t)c) = make_uint2(0, 0);
     if (w >= waves) return;
-    const int begin = range_begin(total, w, waves), end = range_begin(total, w + 1, waves);
+    const Ranges range(total, waves);
+    const int begin = range.begin(w), end = range.begin(w + 1);
     if (begin == end) return;                                        /* no keys at all */
 
-    /* the tile that is asked for next */
-    int u = begin, g, length, tiles, before, q_turn = 0;
-    work.find(u, &g, &length, &tiles, &before);
-    int entry = (u - before) / tiles, tile = u - before - entry * tiles, kvh = entry / a.blocks, block = entry - kvh * a.blocks;
-    bool from_start = false;
-
-    /* The pages of 64 page-fuls of tokens, from the one that a tile begins in. Those that the next tile needs are asked for in front of
-     * the loads of the tile before it: whoever waits for that tile has them. */
-    int run_g = g, run_page = tile * S::KEYS >> shift, run = 0;
-    auto ask_pages = [&]() {
-        const int at = run_page + lane;
-        load_word(lds0 + P0 + 256 * run, at < a.cache.ld ? (const void *)(a.cache.table + (size_t)run_g * a.cache.ld + at) : (const void *)zeros);
+    /* The tile that is asked for next, and the pages of 64 page-fuls of tokens from the one that it begins in. */
+    int u = begin - 1, g = 0, length = 0, tiles = 1, before = 0, tile = 0, kvh = 0, block = 0, q_turn = 0;
+    int run_g = -1, run_page = 0, run = 0;
+    bool from_start = false, asked = false;
+    /* steps to the next tile, and asks for its pages where they are not those that are here */
+    auto step = [&]() {
+        u++; tile++;
+        if (u == begin || tile == tiles) {
+            tile = 0;
+            if (++block == a.blocks) { block = 0; kvh++; }
+            if (u == begin || kvh == a.cache.kv_heads) {
+                work.find(u, &g, &length, &tiles, &before);
+                const int entry = (u - before) / tiles;              /* 0 but for the range's first */
+                tile = u - before - entry * tiles;
+                kvh = entry / a.blocks;
+                block = entry - kvh * a.blocks;
+            }
+        }
+        const int from = tile * S::KEYS >> shift, to = (tile * S::KEYS + S::KEYS - 1) >> shift;
+        if (g != run_g || from < run_page || to >= run_page + 64) {
+            run_g = g; run_page = from; run ^= 1;
+            asked = true;
+            const int at = run_page + lane;
+            load_word(lds0 + P0 + 256 * run, at < a.cache.ld ? (const void *)(a.cache.table + (size_t)run_g * a.cache.ld + at) : (const void *)zeros);
+        }
     };
-    ask_pages();
-    wait_loads<0>();
 
-    /* asks for tile u, steps to the next one; whether that one's pages have been asked for just now */
-    auto request = [&](Tile &t, int stage) -> bool {
-        const int k0 = tile * S::KEYS;
+    /* Asks for tile u and steps to the next one, whose pages are asked for in front of this one's loads: whoever waits for this tile has them. */
+    auto request = [&](Tile &t, int stage) {
+        const int k0 = tile * S::KEYS, head = kvh;
         t.g = g;
         t.head = kvh * a.group + block * COLS;
         t.cols = min(COLS, a.group - block * COLS);
@@ -226,29 +247,10 @@ k_paged_hd128(Args a) {
         const int pos = k0 + (lane & (S::KEYS - 1));
         const unsigned page = reinterpret_cast<const unsigned *>(lds + P0 + 256 * run)[(pos >> shift) - run_page];
         const bool there = pos < length && page < (unsigned)a.cache.pages;
-        const unsigned row = there ? ((page * (unsigned)a.cache.kv_heads + (unsigned)kvh) << shift) + ((unsigned)pos & ((1u << shift) - 1)) : NO_ROW;
+        const unsigned row = there ? ((page * (unsigned)a.cache.kv_heads + (unsigned)head) << shift) + ((unsigned)pos & ((1u << shift) - 1)) : NO_ROW;
         const unsigned long long word = __ballot(there);
         t.seen = S::KEYS == 64 ? word : word & 0xffffffffu;
-
-        /* step, and ask for the next one's pages where they are not those that are here */
-        u++; tile++;
-        bool asked = false;
-        if (u < end) {
-            if (tile == tiles) {
-                tile = 0;
-                if (++block == a.blocks) { block = 0; kvh++; }
-                if (kvh == a.cache.kv_heads) {
-                    kvh = 0;
-                    work.find(u, &g, &length, &tiles, &before);
-                }
-            }
-            const int from = tile * S::KEYS >> shift, to = (tile * S::KEYS + S::KEYS - 1) >> shift;
-            if (g != run_g || from < run_page || to >= run_page + 64) {
-                run_g = g; run_page = from; run ^= 1;
-                ask_pages();
-                asked = true;
-            }
-        }
+        if (u + 1 < end) step();
         if (t.begin) {
 #pragma unroll
             for (int j = 0; j < QROWS / 4; j++) {
@@ -259,10 +261,10 @@ k_paged_hd128(Args a) {
             q_turn ^= 1;
         }
         const uint32_t dst = lds0 + stage * S::STAGE;
-        constexpr int LANES = S::ROW / 16;                           /* to a row */
+        constexpr int LANES = S::ROW / 16, ROWS = 64 / LANES;        /* lanes to a row, rows to a load */
 #pragma unroll
         for (int j = 0; j < S::HALF / 1024; j++) {
-            const int r = j * (64 / LANES) + lane / LANES;
+            const int r = j * ROWS + lane / LANES;
             const unsigned from = (unsigned)__shfl((int)row, r, 64);
             const unsigned piece = 16u * ((lane & (LANES - 1)) ^ swizzle<FP8>(r));
             const size_t at = (size_t)from * S::ROW + piece;
@@ -273,7 +275,6 @@ k_paged_hd128(Args a) {
             load_byte(dst + 2 * S::HALF, row == NO_ROW ? zeros : a.ks + row);
             load_byte(dst + 2 * S::HALF + 256, row == NO_ROW ? zeros : a.vs + row);
         }
-        return asked;
     };
 
     /* O^T: dims 16 db + 4 lg + r of column li; the column's maximum, and this lane's part of the denominator */
@@ -297,141 +298,142 @@ k_paged_hd128(Args a) {
 
     Tile now, next;
     bool stored = false;
-    const bool asked = request(now, 0);
-    if (begin + 1 < end) {
-        if (asked) wait_loads<0>();
-        request(next, 1);
-    }
-    for (int t = begin, stage = 0; t < end; t++, stage ^= 1) {
-        const unsigned char *cur = lds + stage * S::STAGE;
+    step();
+    wait_loads<0>();
+    asked = false;
+    /* The first two turns only ask (one place in the code for it: a short call is as long as its instructions take to come from memory). */
+    for (int t = begin - 2, stage = 0; t < end; t++, stage ^= 1) {
         /* all but the next tile's, and the stores of the last result if there was one: this tile, its Q, the pages of the one after the next */
-        if (t + 1 == end) wait_loads<0>();
+        if (t + 1 >= end) wait_loads<0>();
         else if (stored) wait_loads<S::LOADS + STORES>();
-        else wait_loads<S::LOADS>();
-        stored = now.end;
-        if (now.begin) {
-            const unsigned char *qp = lds + Q0 + Q_BYTES * q_read + (li & (QROWS - 1)) * 2 * HD;
-            if constexpr (FP8) {
-                /* lane (li, lg) holds dims 16 lg .. + 15 and 64 + 16 lg .. + 15 of column li */
-                u32x4 x[4];
-                unsigned most = 0;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    x[i] = *reinterpret_cast<const u32x4 *>(qp + 128 * (i >> 1) + 32 * lg + 16 * (i & 1));
-                    if (QROWS < COLS && li >= QROWS) x[i] = u32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int j = 0; j < 4; j++) most = max(most, max(x[i][j] & 0x7fff, (x[i][j] >> 16) & 0x7fff));
-                }
-                most = max(most, (unsigned)__shfl_xor((int)most, 16, 64));      /* one scale for the column: a lane's 32 values are of two blocks */
-                most = max(most, (unsigned)__shfl_xor((int)most, 32, 64));
-                float factor;
-                q_scale = (int)scale_byte(most, &factor);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    int hi = 0, lo = 0;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint32_t word = x[i >> 1][2 * (i & 1) + h];
-                        const float c0 = __uint_as_float(word << 16) * factor, c1 = __uint_as_float(word & 0xffff0000u) * factor;
-                        hi = h ? __builtin_amdgcn_cvt_pk_fp8_f32(c0, c1, hi, true) : __builtin_amdgcn_cvt_pk_fp8_f32(c0, c1, hi, false);
-                        const f32x2 back = h ? __builtin_amdgcn_cvt_pk_f32_fp8(hi, true) : __builtin_amdgcn_cvt_pk_f32_fp8(hi, false);
-                        lo = h ? __builtin_amdgcn_cvt_pk_fp8_f32(c0 - back[0], c1 - back[1], lo, true) : __builtin_amdgcn_cvt_pk_fp8_f32(c0 - back[0], c1 - back[1], lo, false);
-                    }
-                    q_hi[i] = hi; q_lo[i] = lo;
-                }
-            } else {
-                /* lane (li, lg) holds dims 32 ks + 8 lg .. + 7 of column li */
-#pragma unroll
-                for (int ks = 0; ks < 4; ks++) {
-                    u32x4 x = *reinterpret_cast<const u32x4 *>(qp + 64 * ks + 16 * lg);
-                    if (QROWS < COLS && li >= QROWS) x = u32x4{0, 0, 0, 0};
-                    qb[ks] = __builtin_bit_cast(bf16x8, x);
-                }
-            }
-            q_read ^= 1;
-#pragma unroll
-            for (int db = 0; db < 8; db++) o[db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            top = -INFINITY; sum = 0.0f; base = 0.0f;
-        }
-        constexpr int MB = S::KEYS / 16;
-        f32x4 s[MB];                                                 /* key 16 mb + 4 lg + r against column li, in units of log2 */
-#pragma unroll
-        for (int mb = 0; mb < MB; mb++) {
-            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-            if constexpr (FP8) {
-                const u32x4 k0 = *reinterpret_cast<const u32x4 *>(cur + (k_rd[0] ^ 16 * (mb & 1)) + 16 * mb * S::ROW);        /* swizzle(16 mb + li) */
-                const u32x4 k1 = *reinterpret_cast<const u32x4 *>(cur + (k_rd[1] ^ 16 * (mb & 1)) + 16 * mb * S::ROW);
-                const i32x8 ka = __builtin_bit_cast(i32x8, __builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7));
-                const int scale = *reinterpret_cast<const int *>(cur + 2 * S::HALF + 4 * (16 * mb + li));
-                acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ka, q_lo, acc, 0, 0, 0, scale, 0, q_scale);
-                acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ka, q_hi, acc, 0, 0, 0, scale, 0, q_scale);
-            } else {
-#pragma unroll
-                for (int ks = 0; ks < 4; ks++)
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8 *>(cur + k_rd[ks] + 16 * mb * S::ROW), qb[ks], acc, 0, 0, 0);
-            }
-            s[mb] = acc * a.scale_log2;
-        }
-        const unsigned long long all = S::KEYS == 64 ? ~0ull : 0xffffffffull, mine = now.seen;
-        if (mine != all) {
-#pragma unroll
-            for (int mb = 0; mb < MB; mb++)
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (!((mine >> (16 * mb + 4 * lg + r)) & 1ull)) s[mb][r] = -INFINITY;
-        }
-        float high = -INFINITY;
-#pragma unroll
-        for (int mb = 0; mb < MB; mb++) high = fmaxf(fmaxf(fmaxf(high, s[mb][0]), fmaxf(s[mb][1], s[mb][2])), s[mb][3]);
-        if (__any(high > top + RAISE)) {                          /* the first tile: -infinity + 8 */
-            const float peak = fmaxf(top, over_column(high, [](float x, float y) { return fmaxf(x, y); }));
-            base = peak == -INFINITY ? 0.0f : peak;
-            const float alpha = __builtin_amdgcn_exp2f(top - base);
-            top = peak;
-            sum *= alpha;
-#pragma unroll
-            for (int db = 0; db < 8; db++) o[db] *= alpha;
-        }
-        u32x4 pw[MB / 2];
-#pragma unroll
-        for (int kg = 0; kg < MB / 2; kg++) {
-            float p[8];
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                p[r] = __builtin_amdgcn_exp2f(s[2 * kg][r] - base);
-                p[4 + r] = __builtin_amdgcn_exp2f(s[2 * kg + 1][r] - base);
-            }
-            sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-            if constexpr (FP8) {
-                const u32x4 v0 = *reinterpret_cast<const u32x4 *>(cur + 2 * S::HALF + 256 + 4 * (32 * kg + 4 * lg)), v1 = *reinterpret_cast<const u32x4 *>(cur + 2 * S::HALF + 256 + 4 * (32 * kg + 16 + 4 * lg));
-#pragma unroll
-                for (int r = 0; r < 4; r++) { p[r] = ldexpf(p[r], (int)v0[r] - 127); p[4 + r] = ldexpf(p[4 + r], (int)v1[r] - 127); }
-            }
-            pw[kg] = u32x4{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])};
-        }
-#pragma unroll
-        for (int kg = 0; kg < MB / 2; kg++)
-#pragma unroll
-            for (int db = 0; db < 8; db++) {
-                bf16x8 va;
-                const unsigned char *vp = cur + v_rd[db] + 32 * kg * S::ROW;
+        else if (t >= begin || asked) wait_loads<S::LOADS>();
+        const unsigned char *cur = lds + stage * S::STAGE;
+        if (t >= begin) {
+            stored = now.end;
+            if (now.begin) {
+                const unsigned char *qp = lds + Q0 + Q_BYTES * q_read + (li & (QROWS - 1)) * 2 * HD;
                 if constexpr (FP8) {
-                    const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2 *)vp);
-                    const bf16x2 c0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], 1.0f, false), c1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], 1.0f, true);
-                    const bf16x2 c2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], 1.0f, false), c3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], 1.0f, true);
-                    va = bf16x8{c0[0], c0[1], c1[0], c1[1], c2[0], c2[1], c3[0], c3[1]};
+                    /* lane (li, lg) holds dims 16 lg .. + 15 and 64 + 16 lg .. + 15 of column li */
+                    u32x4 x[4];
+                    unsigned most = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        x[i] = *reinterpret_cast<const u32x4 *>(qp + 128 * (i >> 1) + 32 * lg + 16 * (i & 1));
+                        if (QROWS < COLS && li >= QROWS) x[i] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                        for (int j = 0; j < 4; j++) most = max(most, max(x[i][j] & 0x7fff, (x[i][j] >> 16) & 0x7fff));
+                    }
+                    most = max(most, (unsigned)__shfl_xor((int)most, 16, 64));      /* one scale for the column: a lane's 32 values are of two blocks */
+                    most = max(most, (unsigned)__shfl_xor((int)most, 32, 64));
+                    float factor;
+                    q_scale = (int)scale_byte(most, &factor);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        int hi = 0, lo = 0;
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const uint32_t word = x[i >> 1][2 * (i & 1) + h];
+                            const float c0 = __uint_as_float(word << 16) * factor, c1 = __uint_as_float(word & 0xffff0000u) * factor;
+                            hi = h ? __builtin_amdgcn_cvt_pk_fp8_f32(c0, c1, hi, true) : __builtin_amdgcn_cvt_pk_fp8_f32(c0, c1, hi, false);
+                            const f32x2 back = h ? __builtin_amdgcn_cvt_pk_f32_fp8(hi, true) : __builtin_amdgcn_cvt_pk_f32_fp8(hi, false);
+                            lo = h ? __builtin_amdgcn_cvt_pk_fp8_f32(c0 - back[0], c1 - back[1], lo, true) : __builtin_amdgcn_cvt_pk_fp8_f32(c0 - back[0], c1 - back[1], lo, false);
+                        }
+                        q_hi[i] = hi; q_lo[i] = lo;
+                    }
                 } else {
-                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)vp);
-                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(vp + 16 * S::ROW));
-                    va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                    /* lane (li, lg) holds dims 32 ks + 8 lg .. + 7 of column li */
+#pragma unroll
+                    for (int ks = 0; ks < 4; ks++) {
+                        u32x4 x = *reinterpret_cast<const u32x4 *>(qp + 64 * ks + 16 * lg);
+                        if (QROWS < COLS && li >= QROWS) x = u32x4{0, 0, 0, 0};
+                        qb[ks] = __builtin_bit_cast(bf16x8, x);
+                    }
                 }
-                o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, pw[kg]), o[db], 0, 0, 0);
+                q_read ^= 1;
+#pragma unroll
+                for (int db = 0; db < 8; db++) o[db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                top = -INFINITY; sum = 0.0f; base = 0.0f;
             }
-        wait_lds();                                                  /* this stage has been read */
+            constexpr int MB = S::KEYS / 16;
+            f32x4 s[MB];                                                 /* key 16 mb + 4 lg + r against column li, in units of log2 */
+#pragma unroll
+            for (int mb = 0; mb < MB; mb++) {
+                f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (FP8) {
+                    const u32x4 k0 = *reinterpret_cast<const u32x4 *>(cur + (k_rd[0] ^ 16 * (mb & 1)) + 16 * mb * S::ROW);        /* swizzle(16 mb + li) */
+                    const u32x4 k1 = *reinterpret_cast<const u32x4 *>(cur + (k_rd[1] ^ 16 * (mb & 1)) + 16 * mb * S::ROW);
+                    const i32x8 ka = __builtin_bit_cast(i32x8, __builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7));
+                    const int scale = *reinterpret_cast<const int *>(cur + 2 * S::HALF + 4 * (16 * mb + li));
+                    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ka, q_lo, acc, 0, 0, 0, scale, 0, q_scale);
+                    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ka, q_hi, acc, 0, 0, 0, scale, 0, q_scale);
+                } else {
+#pragma unroll
+                    for (int ks = 0; ks < 4; ks++)
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8 *>(cur + k_rd[ks] + 16 * mb * S::ROW), qb[ks], acc, 0, 0, 0);
+                }
+                s[mb] = acc * a.scale_log2;
+            }
+            const unsigned long long all = S::KEYS == 64 ? ~0ull : 0xffffffffull, mine = now.seen;
+            if (mine != all) {
+#pragma unroll
+                for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (!((mine >> (16 * mb + 4 * lg + r)) & 1ull)) s[mb][r] = -INFINITY;
+            }
+            float high = -INFINITY;
+#pragma unroll
+            for (int mb = 0; mb < MB; mb++) high = fmaxf(fmaxf(fmaxf(high, s[mb][0]), fmaxf(s[mb][1], s[mb][2])), s[mb][3]);
+            if (__any(high > top + RAISE)) {                          /* the first tile: -infinity + 8 */
+                const float peak = fmaxf(top, over_column(high, [](float x, float y) { return fmaxf(x, y); }));
+                base = peak == -INFINITY ? 0.0f : peak;
+                const float alpha = __builtin_amdgcn_exp2f(top - base);
+                top = peak;
+                sum *= alpha;
+#pragma unroll
+                for (int db = 0; db < 8; db++) o[db] *= alpha;
+            }
+            u32x4 pw[MB / 2];
+#pragma unroll
+            for (int kg = 0; kg < MB / 2; kg++) {
+                float p[8];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    p[r] = __builtin_amdgcn_exp2f(s[2 * kg][r] - base);
+                    p[4 + r] = __builtin_amdgcn_exp2f(s[2 * kg + 1][r] - base);
+                }
+                sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                if constexpr (FP8) {
+                    const u32x4 v0 = *reinterpret_cast<const u32x4 *>(cur + 2 * S::HALF + 256 + 4 * (32 * kg + 4 * lg)), v1 = *reinterpret_cast<const u32x4 *>(cur + 2 * S::HALF + 256 + 4 * (32 * kg + 16 + 4 * lg));
+#pragma unroll
+                    for (int r = 0; r < 4; r++) { p[r] = ldexpf(p[r], (int)v0[r] - 127); p[4 + r] = ldexpf(p[4 + r], (int)v1[r] - 127); }
+                }
+                pw[kg] = u32x4{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])};
+            }
+#pragma unroll
+            for (int kg = 0; kg < MB / 2; kg++)
+#pragma unroll
+                for (int db = 0; db < 8; db++) {
+                    bf16x8 va;
+                    const unsigned char *vp = cur + v_rd[db] + 32 * kg * S::ROW;
+                    if constexpr (FP8) {
+                        const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2 *)vp);
+                        const bf16x2 c0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], 1.0f, false), c1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], 1.0f, true);
+                        const bf16x2 c2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], 1.0f, false), c3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], 1.0f, true);
+                        va = bf16x8{c0[0], c0[1], c1[0], c1[1], c2[0], c2[1], c3[0], c3[1]};
+                    } else {
+                        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)vp);
+                        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(vp + 16 * S::ROW));
+                        va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                    }
+                    o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, pw[kg]), o[db], 0, 0, 0);
+                }
+            wait_lds();                                                  /* this stage has been read */
+        }
         const Tile done = now;
         now = next;
         if (t + 2 < end) request(next, stage);
-        if (!done.end) continue;
+        if (t < begin || !done.end) continue;
         const float den = over_column(sum, [](float x, float y) { return x + y; });
         if (li < done.cols && done.whole) {
             const float inv = den > 0.0f ? 1.0f / den : 0.0f;
@@ -452,7 +454,7 @@ k_paged_hd128(Args a) {
 
 /* Workgroup w joins the list entry that the end of range w cuts, if it is the first end in it. 32 lanes take 4 dims each of a column and
  * every so many-th part, eight at a time so that their loads are under way together; the LDS joins what several groups of 32 have. */
-constexpr int JOIN = 512;
+template <int JOIN>
 __global__ void __launch_bounds__(JOIN)
 k_paged_join(Args a, int keys) {
     __shared__ f32x4 sums[JOIN];
@@ -461,62 +463,68 @@ k_paged_join(Args a, int keys) {
     Work work;
     const int total = work.count(a.cache, a.n, per, keys), waves = ranges(total, gridDim.x);
     if (w + 1 >= waves) return;
-    const int u = range_begin(total, w + 1, waves);
+    const Ranges range(total, waves);
+    const int u = range.begin(w + 1);
     int g, length, tiles, before;
     work.find(u, &g, &length, &tiles, &before);
     const int entry = (u - before) / tiles, first = before + entry * tiles;
-    if (first == u || first < range_begin(total, w, waves)) return;
-    const int last = range_of(total, first + tiles - 1, waves);
+    if (first == u || first < range.begin(w)) return;
+    const int last = range.of(first + tiles - 1);
     const int kvh = entry / a.blocks, block = entry - kvh * a.blocks, cols = min(COLS, a.group - block * COLS);
-    const int places = cols <= 1 ? 1 : cols <= 2 ? 2 : cols <= 4 ? 4 : cols <= 8 ? 8 : 16, groups = JOIN / 32 / places;     /* per column */
-    const int unit = threadIdx.x >> 5, c = unit & (places - 1), part = unit / places, at = threadIdx.x & 31;
-    float top = -INFINITY, den = 0.0f;
-    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (c < cols) {
-        for (int i0 = w + part; i0 <= last; i0 += 8 * groups) {
-            float t[8], d[8];
-            f32x4 o[8];
+    constexpr int UNITS = JOIN / 32;
+    int places = 1;                                                  /* columns at a time */
+    while (places < cols && places < UNITS) places *= 2;
+    const int groups = UNITS / places, unit = threadIdx.x >> 5, part = unit / places, at = threadIdx.x & 31;
+    for (int c = unit & (places - 1), turn = 0; turn < cols; turn += places, c += places) {
+        float top = -INFINITY, den = 0.0f;
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (c < cols) {
+            for (int i0 = w + part; i0 <= last; i0 += 8 * groups) {
+                float t[8], d[8];
+                f32x4 o[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int i = min(i0 + j * groups, last);
-                const float *pp = a.part + (size_t)(2 * i + (i == w)) * PART;
-                t[j] = i0 + j * groups <= last ? pp[COLS * HD + c] : -INFINITY;
-                d[j] = pp[COLS * HD + COLS + c];
-                o[j] = *reinterpret_cast<const f32x4 *>(pp + c * HD + 4 * at);
+                for (int j = 0; j < 8; j++) {
+                    const int i = min(i0 + j * groups, last);
+                    const float *pp = a.part + (size_t)(2 * i + (i == w)) * PART;
+                    t[j] = i0 + j * groups <= last ? pp[COLS * HD + c] : -INFINITY;
+                    d[j] = pp[COLS * HD + COLS + c];
+                    o[j] = *reinterpret_cast<const f32x4 *>(pp + c * HD + 4 * at);
+                }
+                float now = top;
+#pragma unroll
+                for (int j = 0; j < 8; j++) now = fmaxf(now, t[j]);
+                const float base = now == -INFINITY ? 0.0f : now, alpha = __builtin_amdgcn_exp2f(top - base);
+                sum *= alpha;
+                den *= alpha;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (i0 + j * groups > last) break;
+                    const float f = __builtin_amdgcn_exp2f(t[j] - base);
+                    sum += o[j] * f;
+                    den += d[j] * f;
+                }
+                top = now;
             }
+        }
+        __syncthreads();                                             /* the columns before these have been read */
+        sums[threadIdx.x] = sum;
+        if (at == 0) { tops[unit] = top; dens[unit] = den; }
+        __syncthreads();
+        if (part == 0 && c < cols) {
             float now = top;
-#pragma unroll
-            for (int j = 0; j < 8; j++) now = fmaxf(now, t[j]);
+            for (int j = 1; j < groups; j++) now = fmaxf(now, tops[unit + j * places]);
             const float base = now == -INFINITY ? 0.0f : now, alpha = __builtin_amdgcn_exp2f(top - base);
             sum *= alpha;
             den *= alpha;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if (i0 + j * groups > last) break;
-                const float f = __builtin_amdgcn_exp2f(t[j] - base);
-                sum += o[j] * f;
-                den += d[j] * f;
+            for (int j = 1; j < groups; j++) {
+                const float f = __builtin_amdgcn_exp2f(tops[unit + j * places] - base);
+                sum += sums[threadIdx.x + 32 * places * j] * f;
+                den += dens[unit + j * places] * f;
             }
-            top = now;
+            const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+            *reinterpret_cast<uint2 *>(a.out + (size_t)g * a.ldo + (size_t)(kvh * a.group + block * COLS + c) * HD + 4 * at) =
+                make_uint2(pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv));
         }
-    }
-    sums[threadIdx.x] = sum;
-    if (at == 0) { tops[unit] = top; dens[unit] = den; }
-    __syncthreads();
-    if (part == 0 && c < cols) {
-        float now = top;
-        for (int j = 1; j < groups; j++) now = fmaxf(now, tops[c + j * places]);
-        const float base = now == -INFINITY ? 0.0f : now, alpha = __builtin_amdgcn_exp2f(top - base);
-        sum *= alpha;
-        den *= alpha;
-        for (int j = 1; j < groups; j++) {
-            const float f = __builtin_amdgcn_exp2f(tops[c + j * places] - base);
-            sum += sums[threadIdx.x + 32 * places * j] * f;
-            den += dens[c + j * places] * f;
-        }
-        const float inv = den > 0.0f ? 1.0f / den : 0.0f;
-        *reinterpret_cast<uint2 *>(a.out + (size_t)g * a.ldo + (size_t)(kvh * a.group + block * COLS + c) * HD + 4 * at) =
-            make_uint2(pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv));
     }
 }
 
@@ -551,6 +559,10 @@ extern "C" int iris_hip_paged_hd128(void *stream, float *part, uint16_t *out, in
     };
     if (ks) run_rows(std::true_type{});
     else run_rows(std::false_type{});
-    if (waves > 1) hipLaunchKernelGGL(k_paged_join, dim3(waves), dim3(JOIN), 0, (hipStream_t)stream, a, keys);
+    /* as many threads as parts are to be expected: a thousand workgroups of 512 take 2 us to start */
+    if (waves > 1) {
+        if (waves <= 8L * n * kv_heads * blocks) hipLaunchKernelGGL(k_paged_join<256>, dim3(waves), dim3(256), 0, (hipStream_t)stream, a, keys);
+        else hipLaunchKernelGGL(k_paged_join<512>, dim3(waves), dim3(512), 0, (hipStream_t)stream, a, keys);
+    }
     return (int)hipGetLastError();
 }
