@@ -20,7 +20,10 @@
  * columns that see them at the end.
  *
  * Workgroups: eight kv heads at a time (one to an XCD, whose L2 then holds the K and V of one head), tile by tile from the last one of
- * the last sequence on, which with a causal limit are the longest of their sequence.
+ * the last sequence on, which with a causal limit are the longest of their sequence. (All long ones of a batch first is no faster.)
+ *
+ * Where there are few columns and many keys, `ranges` workgroups share the key tiles of the same columns, evenly: each leaves its
+ * unnormalised sums, their maximum and denominator in a workspace, and a second launch joins them.
  */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -40,6 +43,7 @@ namespace {
 
 constexpr int HD = 128, KEYS = 64, TILE = KEYS * HD, STAGE = 2 * TILE;      /* elements of K or V; of a stage, 32 KB */
 constexpr float RAISE = 8.0f;
+constexpr int MOST_RANGES = 8;
 
 __device__ __align__(256) const uint16_t zeros[HD] = {};
 
@@ -107,8 +111,21 @@ struct Args {
     const uint16_t *q, *k, *v;
     int ldo, ldq, ldkv, kv_heads;
     SequencesArg seqs;
-    float scale_log2;
+    float scale_log2, *part;                     /* part: partial results, ranges > 1 */
+    int ranges;
 };
+
+/* What a workgroup works on */
+struct Place { bool there; int kvh, tile, range; };
+__device__ __forceinline__ Place place(const Args &a, int count) {
+    const int together = a.kv_heads % 8 == 0 ? 8 : a.kv_heads;       /* kv heads whose tiles are dealt out in turn */
+    const unsigned round = (unsigned)together * (unsigned)count, number = blockIdx.x / a.ranges;
+    if (round == 0 || number / round >= (unsigned)(a.kv_heads / together)) return {false, 0, 0, 0};
+    const unsigned rest = number % round;
+    return {true, (int)(number / round) * together + (int)(rest % together), count - 1 - (int)(rest / together), (int)(blockIdx.x % a.ranges)};
+}
+/* floats of a workgroup's partial result: sums of its columns, their maxima, their denominators */
+constexpr int part_floats(int columns) { return columns * (HD + 2); }
 
 template <int WAVES, int NB, bool CAUSAL>
 __global__ void __launch_bounds__(64 * WAVES, 2)
@@ -120,12 +137,10 @@ k_sequences_hd128(Args a) {
 
     SequenceTiles tiles;
     const int count = tiles.count(a.seqs, COLUMNS);
-    const int together = a.kv_heads % 8 == 0 ? 8 : a.kv_heads;       /* kv heads whose tiles are dealt out in turn */
-    const unsigned round = (unsigned)together * (unsigned)count;
-    if (round == 0 || blockIdx.x / round >= (unsigned)(a.kv_heads / together)) return;
-    const unsigned rest = blockIdx.x % round;
-    const int kvh = (int)(blockIdx.x / round) * together + (int)(rest % together);
-    const SequenceTile s = tiles.tile(count - 1 - (int)(rest / together));
+    const Place at = place(a, count);
+    if (!at.there) return;
+    const SequenceTile s = tiles.tile(at.tile);
+    const int kvh = at.kvh;
 
     /* this lane's columns, one in each block; those behind the sequence's last are computed like it and not stored */
     const int columns = s.n * group, wc0 = s.c0 + wave * 16 * NB, ahead = s.m - s.n;
@@ -138,7 +153,8 @@ k_sequences_hd128(Args a) {
         limit[nb] = CAUSAL ? row[nb] + 1 + ahead : s.m;
     }
     const int last = min(s.c0 + COLUMNS, columns) - 1, k_end = CAUSAL ? max(last / group + 1 + ahead, 0) : s.m;      /* no column of the workgroup sees more */
-    const int ntiles = (k_end + KEYS - 1) / KEYS;
+    const int all_tiles = (k_end + KEYS - 1) / KEYS;
+    const int tile0 = all_tiles * at.range / a.ranges, ntiles = all_tiles * (at.range + 1) / a.ranges;      /* (at most 8 ranges) */
     const bool busy = wc0 < columns;
     /* the wave's columns see all of the tiles in front of the first limit, and nothing from the last one on */
     const int see_all = CAUSAL ? wc0 / group + 1 + ahead : s.m, see_any = CAUSAL ? min(wc0 + 16 * NB - 1, columns - 1) / group + 1 + ahead : s.m;
@@ -153,7 +169,7 @@ k_sequences_hd128(Args a) {
         load_tile<WAVES>(lds + stage * STAGE, kbase + at, vbase + at, a.ldkv, s.m - tile * KEYS, lane_off, wave);
     };
 #pragma unroll
-    for (int t = 0; t < GROUP; t++) request(t, t);
+    for (int t = 0; t < GROUP; t++) request(tile0 + t, t);
 
     bf16x8 qb[NB][4];
 #pragma unroll
@@ -194,7 +210,7 @@ k_sequences_hd128(Args a) {
     wait_loads<0>();
     lds_barrier();
 
-    for (int t0 = 0, half = 0; t0 < ntiles; t0 += GROUP, half ^= 1) {
+    for (int t0 = tile0, half = 0; t0 < ntiles; t0 += GROUP, half ^= 1) {
 #pragma unroll
         for (int step = 0; step < GROUP; step++) {
             const int k0 = (t0 + step) * KEYS;
@@ -351,6 +367,17 @@ k_sequences_hd128(Args a) {
         }
     }
 
+    if (a.ranges > 1) {
+        float *pp = a.part + (size_t)blockIdx.x * part_floats(COLUMNS);
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            const int c = wave * 16 * NB + 16 * nb + li;
+#pragma unroll
+            for (int db = 0; db < 8; db++) *reinterpret_cast<f32x4 *>(pp + c * HD + 16 * db + 4 * lg) = o[db][nb];
+            if (lg == 0) { pp[COLUMNS * HD + c] = top[nb]; pp[COLUMNS * (HD + 1) + c] = den[nb][0]; }
+        }
+        return;
+    }
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
         const float inv = den[nb][0] == 0.0f ? 0.0f : 1.0f / den[nb][0];
@@ -360,6 +387,45 @@ k_sequences_hd128(Args a) {
             for (int db = 0; db < 8; db++)
                 *reinterpret_cast<uint2 *>(op + 16 * db) = make_uint2(pack_bf16(o[db][nb][0] * inv, o[db][nb][1] * inv), pack_bf16(o[db][nb][2] * inv, o[db][nb][3] * inv));
         }
+    }
+}
+
+/* The ranges of a workgroup's columns joined: 32 lanes to a column, 4 dims each, all ranges' loads under way together */
+constexpr int JOIN = 1024;
+template <int COLUMNS>
+__global__ void __launch_bounds__(JOIN)
+k_sequences_join(Args a) {
+    SequenceTiles tiles;
+    const int ranges = a.ranges, count = tiles.count(a.seqs, COLUMNS), group = a.seqs.per_row;
+    a.ranges = 1;                                                     /* a workgroup here for all ranges */
+    const Place at = place(a, count);
+    if (!at.there) return;
+    const SequenceTile s = tiles.tile(at.tile);
+    const int columns = min(COLUMNS, s.n * group - s.c0), lane = threadIdx.x & 31;
+    const float *pp = a.part + (size_t)blockIdx.x * ranges * part_floats(COLUMNS);
+    for (int c = threadIdx.x >> 5; c < columns; c += JOIN / 32) {
+        float t[MOST_RANGES], d[MOST_RANGES], top = -INFINITY, den = 0.0f;
+        f32x4 o[MOST_RANGES], sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < MOST_RANGES; i++) {
+            const float *p = pp + (size_t)min(i, ranges - 1) * part_floats(COLUMNS);
+            t[i] = i < ranges ? p[COLUMNS * HD + c] : -INFINITY;
+            d[i] = p[COLUMNS * (HD + 1) + c];
+            o[i] = *reinterpret_cast<const f32x4 *>(p + c * HD + 4 * lane);
+            top = fmaxf(top, t[i]);
+        }
+        const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int i = 0; i < MOST_RANGES; i++) {
+            if (i >= ranges) break;
+            const float f = __builtin_amdgcn_exp2f(t[i] - base);
+            sum += o[i] * f;
+            den += d[i] * f;
+        }
+        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+        const int row = (s.c0 + c) / group, head = at.kvh * group + (s.c0 + c) - row * group;
+        *reinterpret_cast<uint2 *>(a.out + (size_t)(s.row0 + row) * a.ldo + (size_t)head * HD + 4 * lane) =
+            make_uint2(pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv));
     }
 }
 
@@ -374,30 +440,50 @@ int launch(hipStream_t stream, const Args &a) {
     }
     const long wgs = sequence_tiles_at_most(a.seqs, 16 * NB * WAVES) * a.kv_heads;
     if (!wgs) return 0;
-    if (wgs > ((1L << 32) - 1) / (64 * WAVES)) return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_sequences_hd128<WAVES, NB, CAUSAL>), dim3((unsigned)wgs), dim3(64 * WAVES), LDS, stream, a);
+    if (wgs * a.ranges > ((1L << 32) - 1) / (64 * WAVES)) return (int)hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_sequences_hd128<WAVES, NB, CAUSAL>), dim3((unsigned)(wgs * a.ranges)), dim3(64 * WAVES), LDS, stream, a);
+    if constexpr (NB == 1 && WAVES == 4)
+        if (a.ranges > 1) hipLaunchKernelGGL((k_sequences_join<16 * NB * WAVES>), dim3((unsigned)wgs), dim3(JOIN), 0, stream, a);
     return (int)hipGetLastError();
 }
 
 }  // namespace
 
-/* Which workgroups a call takes: waves x blocks of 16 columns a wave; host arithmetic only */
-extern "C" void iris_hip_sequences_plan(int n, int rows, int heads, int kv_heads, int *waves, int *blocks) {
+/* Which workgroups a call takes: waves x blocks of 16 columns a wave, and in how many ranges the keys of each are cut; host arithmetic only */
+extern "C" void iris_hip_sequences_plan(int n, int rows, int keys, int heads, int kv_heads, int causal, int own_keys, int *waves, int *blocks, int *ranges) {
     const int group = heads / kv_heads;
     const long some = n < rows ? n : rows, blocks16 = ((long)rows * group + some * 8) / 16 * kv_heads, each = (long)rows * group / some;
-    *blocks = 1;
-    *waves = blocks16 <= 256 ? 1 : blocks16 <= 640 ? 2 : blocks16 <= 1024 ? 4 : 8;
-    if (blocks16 > 2048) { *blocks = 2; *waves = 8; }
+    *blocks = *ranges = 1;
+    if (causal) {
+        *waves = blocks16 <= 640 ? 2 : 4;
+        if (blocks16 > 3500) *blocks = 2;
+    } else {
+        *waves = blocks16 <= 640 ? 2 : blocks16 <= 1024 ? 4 : 8;
+        if (blocks16 > 2048) *blocks = 2;
+    }
     while (*waves > 1 && each <= 8 * *waves * *blocks) *waves /= 2;
     if (*blocks == 2 && *waves < 4) { *waves = 2 * *waves; *blocks = 1; }
+    /* key tiles that a workgroup sees, about, and workgroups of 64 columns */
+    const long chain = (long)keys / some / KEYS / (causal && own_keys ? 2 : 1), wgs = (((long)rows * group + some * 32) / 64 + 1) * kv_heads;
+    const long room = (long)(IRIS_LINEAR_PART_BYTES / sizeof(float) / part_floats(64)) / (sequence_tiles_at_most({nullptr, nullptr, n, rows, keys, group}, 64) * kv_heads);
+    if (chain >= 12 && wgs <= 256) {
+        long r = 512 / wgs;
+        if (r > chain / 4) r = chain / 4;
+        if (r > MOST_RANGES) r = MOST_RANGES;
+        if (r > room) r = room;
+        if (r > 1) { *waves = 4; *blocks = 1; *ranges = (int)r; }
+    }
 }
 
-extern "C" int iris_hip_sequences_hd128(void *stream, uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k, const uint16_t *v, int ldkv,
-                                        const int *first_row, const int *first_key, int n, int rows, int keys, int heads, int kv_heads, float scale, int causal) {
-    const Args a = {out, q, k, v, ldo, ldq, ldkv, kv_heads, {first_row, first_key, n, rows, keys, heads / kv_heads}, scale * 1.4426950408889634f};
+/* part: IRIS_LINEAR_PART_BYTES of private workspace, 16-byte aligned, or null: the keys of a workgroup are then not cut */
+extern "C" int iris_hip_sequences_hd128(void *stream, float *part, uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k, const uint16_t *v,
+                                        int ldkv, const int *first_row, const int *first_key, int n, int rows, int keys, int heads, int kv_heads, float scale,
+                                        int causal) {
+    Args a = {out, q, k, v, ldo, ldq, ldkv, kv_heads, {first_row, first_key, n, rows, keys, heads / kv_heads}, scale * 1.4426950408889634f, part, 1};
     const hipStream_t st = (hipStream_t)stream;
-    int waves, blocks;
-    iris_hip_sequences_plan(n, rows, heads, kv_heads, &waves, &blocks);
+    int waves, blocks, ranges;
+    iris_hip_sequences_plan(n, rows, keys, heads, kv_heads, causal, first_key == nullptr, &waves, &blocks, &ranges);
+    if (part) a.ranges = ranges;
     if (blocks == 2 && waves == 8) return causal ? launch<8, 2, true>(st, a) : launch<8, 2, false>(st, a);
     if (blocks == 2) return causal ? launch<4, 2, true>(st, a) : launch<4, 2, false>(st, a);
     if (waves == 8) return causal ? launch<8, 1, true>(st, a) : launch<8, 1, false>(st, a);

@@ -225,10 +225,13 @@ int iris_hip_sequences_any(void *stream, uint16_t *out, int ldo, const uint16_t 
                            const int *first_row, const int *first_key, int n, int rows, int keys, int heads, int kv_heads, int head_dim,
                            float scale, int causal);
 /* The same on the matrix cores: head_dim 128, scale > 0, q, k, v 16-byte and out 8-byte aligned, ldq and ldkv % 8 == 0, ldo % 4 == 0,
- * ldkv < 2^27. plan: its workgroups for these sizes, waves x blocks of 16 columns a wave, host arithmetic only. */
-void iris_hip_sequences_plan(int n, int rows, int heads, int kv_heads, int *waves, int *blocks);
-int iris_hip_sequences_hd128(void *stream, uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k, const uint16_t *v, int ldkv,
-                             const int *first_row, const int *first_key, int n, int rows, int keys, int heads, int kv_heads, float scale, int causal);
+ * ldkv < 2^27. part: IRIS_LINEAR_PART_BYTES of private workspace, 16-byte aligned, that the stream orders with its other users, or null: the
+ * keys of few columns are then not cut into ranges. plan: the workgroups for these sizes, waves x blocks of 16 columns a wave, and the
+ * ranges (own_keys: first_key is NULL); host arithmetic only. */
+void iris_hip_sequences_plan(int n, int rows, int keys, int heads, int kv_heads, int causal, int own_keys, int *waves, int *blocks, int *ranges);
+int iris_hip_sequences_hd128(void *stream, float *part, uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k, const uint16_t *v,
+                             int ldkv, const int *first_row, const int *first_key, int n, int rows, int keys, int heads, int kv_heads, float scale,
+                             int causal);
 /* One row a sequence over the pages; ks, vs NULL: bf16, otherwise e4m3 codes and scale bytes. Pages of 2^page_shift rows. */
 int iris_hip_paged_any(void *stream, uint16_t *out, int ldo, const uint16_t *q, int ldq, const void *k, const void *v, const uint8_t *ks,
                        const uint8_t *vs, int pages, int page_shift, const int *table, int table_ld, const int *lengths, int n, int heads,

@@ -663,7 +663,7 @@ void iris_dev_attention_sequences(uint16_t *out, int ldo, const uint16_t *q, int
     if (head_dim == 128 && scale > 0.0f && keys && ldq % 8 == 0 && ldkv % 8 == 0 && ldo % 4 == 0 && ldkv < 1 << 27 && aligned(q, 16) && aligned(k, 16) &&
         aligned(v, 16) && aligned(out, 8)) {
         g_last_kernel = "fa_sequences_hd128";
-        LAUNCH("attention_sequences", iris_hip_sequences_hd128(g_stream, out, ldo, q, ldq, k, v, ldkv, first_row, first_key, sequences, rows, keys, heads,
+        LAUNCH("attention_sequences", iris_hip_sequences_hd128(g_stream, linear_part(), out, ldo, q, ldq, k, v, ldkv, first_row, first_key, sequences, rows, keys, heads,
                                                                 kv_heads, scale, causal != 0));
         return;
     }

@@ -3,8 +3,8 @@
  * its keys are [first_key[g], first_key[g + 1]) of `keys` (first_key NULL: its own rows).
  *
  * Every row has `per_row` columns (the query heads that share a key-value head, or one), numbered row by row inside a sequence. The
- * kernels walk one list of tiles of `height` columns: those of sequence 0, of sequence 1, ... No tile straddles sequences. The host
- * knows an upper bound of their number; a workgroup finds the true number and its own tile, 64 sequences at a time, one to a lane.
+ * kernels walk one list of tiles of `height` columns, sequence by sequence. No tile straddles two. The host knows an upper bound of their number; a
+ * workgroup finds the true number and its own tile, 256 sequences at a time, four to a lane.
  *
  * Whatever the arrays hold, every tile lies inside [0, rows) and [0, keys): a value counts as the largest up to its place, limited to
  * 0 .. rows (keys). Rows outside [first[0], first[n]) are in no tile. first NULL: row g is sequence g.
@@ -42,59 +42,76 @@ __device__ __forceinline__ int wave_max_upto(int v) {                    /* of v
 }
 
 struct SequenceTiles {
+    static constexpr int AT_ONCE = 4;                                /* 64 sequences at once: their bounds are one trip to memory */
     SequencesArg a;
     int height;
-    int lo, hi, upto, tiles, most;               /* this lane's sequence of the last 64 looked at: its rows, its tiles with all before it */
-    int key_most;                                /* the largest value of first_key before those 64 */
+    int lo[AT_ONCE], hi[AT_ONCE], klo[AT_ONCE], khi[AT_ONCE];        /* this lane's sequences of the last looked at: rows, keys */
+    int upto[AT_ONCE], total, most, key_most;    /* tiles of all sequences up to each; of all so far; the largest values in front of those */
 
-    /* first[base + lane] and the next one, each as the largest value up to its place, limited to 0 .. limit */
-    static __device__ __forceinline__ void range(const int *first, int n, int g, int limit, int &most, int &lo, int &hi) {
-        lo = max(wave_max_upto(g < n ? max(first[g], 0) : 0), most);
-        hi = max(lo, g < n ? first[g + 1] : 0);
-        most = __builtin_amdgcn_readlane(hi, 63);
-        lo = min(lo, limit);
-        hi = min(hi, limit);
+    /* first[g] and the next one, each as the largest value up to its place, limited to 0 .. limit */
+    static __device__ __forceinline__ void range(int from, int to, int limit, int &most, int &lo, int &hi) {
+        const int x = max(wave_max_upto(max(from, 0)), most), y = max(x, to);
+        most = __builtin_amdgcn_readlane(y, 63);
+        lo = min(x, limit);
+        hi = min(y, limit);
     }
+    __device__ __forceinline__ int tiles(int i) const { return ((hi[i] - lo[i]) * a.per_row + height - 1) / height; }
     __device__ __forceinline__ void look(int base) {
-        const int g = base + (threadIdx.x & 63);
-        if (a.first_row) {
-            range(a.first_row, a.n, g, a.rows, most, lo, hi);
-        } else {
-            lo = min(g, min(a.rows, a.n));
-            hi = min(g + 1, min(a.rows, a.n));
+        const int lane = threadIdx.x & 63;
+        int from[AT_ONCE], to[AT_ONCE], kfrom[AT_ONCE], kto[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i++) {
+            const int g = min(base + 64 * i + lane, a.n), next = min(g + 1, a.n);        /* behind the last one: no rows */
+            from[i] = a.first_row ? a.first_row[g] : g;
+            to[i] = a.first_row ? a.first_row[next] : next;
+            kfrom[i] = a.first_key ? a.first_key[g] : 0;
+            kto[i] = a.first_key ? a.first_key[next] : 0;
         }
-        upto = tiles + wave_sum_upto(((hi - lo) * a.per_row + height - 1) / height);
-        tiles = __builtin_amdgcn_readlane(upto, 63);
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i++) {
+            lo[i] = hi[i] = klo[i] = khi[i] = 0;
+            upto[i] = total;
+            if (base + 64 * i < a.n) {
+                range(from[i], to[i], a.rows, most, lo[i], hi[i]);
+                klo[i] = lo[i]; khi[i] = hi[i];
+                if (a.first_key) range(kfrom[i], kto[i], a.keys, key_most, klo[i], khi[i]);
+                upto[i] += wave_sum_upto(tiles(i));
+                total = __builtin_amdgcn_readlane(upto[i], 63);
+            }
+        }
     }
+    /* all tiles */
     __device__ __forceinline__ int count(const SequencesArg &arg, int columns) {
-        a = arg; height = columns; tiles = 0; most = 0;
-        for (int base = 0; base < a.n; base += 64) look(base);
-        return tiles;
+        a = arg; height = columns;
+        most = key_most = total = 0;
+        for (int base = 0; base < a.n; base += 64 * AT_ONCE) look(base);
+        return total;
     }
     /* tile t of them, t < count() */
     __device__ __forceinline__ SequenceTile tile(int t) {
         int base = 0;
-        if (a.n > 64) {
-            tiles = 0; most = 0;
-            for (; base < a.n; base += 64) {
+        if (a.n > 64 * AT_ONCE) {
+            most = key_most = total = 0;
+            for (; base < a.n; base += 64 * AT_ONCE) {
                 look(base);
-                if (t < tiles) break;
+                if (t < total) break;
             }
         }
-        const unsigned long long past = __ballot(upto > t);
-        const int at = past ? __ffsll(past) - 1 : 0;
-        SequenceTile s;
-        s.g = base + at;
-        s.row0 = __builtin_amdgcn_readlane(lo, at);
-        s.n = __builtin_amdgcn_readlane(hi, at) - s.row0;
-        s.c0 = (t - (__builtin_amdgcn_readlane(upto, at) - (s.n * a.per_row + height - 1) / height)) * height;
-        s.key0 = s.row0; s.m = s.n;
-        if (a.first_key) {
-            int klo = 0, khi = 0;
-            key_most = 0;
-            for (int b = 0; b <= base; b += 64) range(a.first_key, a.n, b + (threadIdx.x & 63), a.keys, key_most, klo, khi);
-            s.key0 = __builtin_amdgcn_readlane(klo, at);
-            s.m = __builtin_amdgcn_readlane(khi, at) - s.key0;
+        SequenceTile s = {0, 0, 0, 0, 0, 0};
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i++) {
+            const unsigned long long past = __ballot(upto[i] > t);
+            if (past && !found) {
+                found = true;
+                const int at = __ffsll(past) - 1;
+                s.g = base + 64 * i + at;
+                s.row0 = __builtin_amdgcn_readlane(lo[i], at);
+                s.n = __builtin_amdgcn_readlane(hi[i], at) - s.row0;
+                s.key0 = __builtin_amdgcn_readlane(klo[i], at);
+                s.m = __builtin_amdgcn_readlane(khi[i], at) - s.key0;
+                s.c0 = (t - (__builtin_amdgcn_readlane(upto[i], at) - (s.n * a.per_row + height - 1) / height)) * height;
+            }
         }
         return s;
     }
