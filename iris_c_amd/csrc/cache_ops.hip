@@ -12,6 +12,7 @@
  */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "iris_kernels_hip.h"
 #include "paged_cache.h"
@@ -22,7 +23,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 namespace {
 
-constexpr int ROWS = 16, THREADS = 256;
+constexpr int ROWS = 16, THREADS = 256;                              /* rows of a workgroup; of one in a large call four times as many */
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const f32x2 p = {lo, hi};
@@ -38,58 +39,89 @@ __device__ __forceinline__ int position(const PagedArg &c, const SequenceTile &s
 struct Pair { void *k, *v; };
 struct ConstPair { const void *k, *v; };
 
-/* head_dim = 8 LANES, rows 16-byte aligned: 16 bytes of bf16 to a lane, LANES lanes to a row of a head */
-template <int LANES, bool FP8, bool WRITE>
+/* head_dim HEAD, rows 16-byte aligned. A unit is 8 values of bf16, 16 of 8 bits (16 bytes of the pages), of consecutive lanes; a thread has
+ * the loads of UNROLL units under way together. The places of the rows are looked up once, a row to a thread. magic: 2^32 / kv_heads rounded
+ * up, which divides numbers of rows of heads up to ROWS * kv_heads exactly while kv_heads < 8192; 0 for one head.
+ * Where a workgroup has no more units than threads (the newest token of each text) UNROLL is 1: 48 rows of 8 heads in bf16 take 3 us and 10
+ * with the longer code of UNROLL 4, whose instructions come from memory at each launch. */
+template <int HEAD, bool FP8, bool WRITE, int ROWS, int UNROLL>
 __global__ void __launch_bounds__(THREADS)
-k_cache_rows(Pair pages, Pair scales, ConstPair rows, Pair out, int ld, PagedArg cache, SequencesArg seqs) {
+k_cache_rows(Pair pages, Pair scales, ConstPair rows, Pair out, int ld, PagedArg cache, SequencesArg seqs, uint32_t magic) {
+    constexpr int VALUES = FP8 ? 16 : 8, LANES = HEAD / VALUES, WORDS = FP8 ? 2 : 1;      /* 16-byte words of bf16 to a unit */
+    __shared__ long places[ROWS];
     SequenceTiles tiles;
     const int count = tiles.count(seqs, ROWS), t = blockIdx.x >> 1;
     if (t >= count) return;
     const bool second = blockIdx.x & 1;
     const SequenceTile s = tiles.tile(t);
     const int n = min(ROWS, s.n - s.c0), units = n * cache.kv_heads * LANES;
-    uint8_t *codes = (uint8_t *)(second ? pages.v : pages.k), *bytes = (uint8_t *)(second ? scales.v : scales.k);
-    uint16_t *plain = (uint16_t *)(second ? pages.v : pages.k);
+    if (threadIdx.x < n) {
+        const int pos = position(cache, s, s.c0 + threadIdx.x);
+        places[threadIdx.x] = pos < 0 ? -1 : paged_row(cache, s.g, pos, 0);
+    }
+    __syncthreads();
+    uint8_t *bytes = (uint8_t *)(second ? scales.v : scales.k);
+    uint4 *in_pages = (uint4 *)(second ? pages.v : pages.k);         /* of LANES words to a row */
     const uint16_t *from = (const uint16_t *)(second ? rows.v : rows.k);
     uint16_t *to = (uint16_t *)(second ? out.v : out.k);
-    for (int u = threadIdx.x; u < units; u += THREADS) {
-        const int lane = u % LANES, head = u / LANES % cache.kv_heads, row = s.c0 + u / LANES / cache.kv_heads;
-        const int pos = position(cache, s, row);
-        const long place = pos < 0 ? -1 : paged_row(cache, s.g, pos, head);
-        if (place < 0) continue;                                     /* the same for the LANES lanes of a row */
-        const size_t at = (size_t)(s.row0 + row) * ld + (size_t)head * (8 * LANES) + 8 * lane, in_pages = (size_t)place * (8 * LANES) + 8 * lane;
-        if constexpr (!FP8) {
-            if (WRITE) *reinterpret_cast<uint4 *>(plain + in_pages) = *reinterpret_cast<const uint4 *>(from + at);
-            else *reinterpret_cast<uint4 *>(to + at) = *reinterpret_cast<const uint4 *>(plain + in_pages);
-        } else if constexpr (WRITE) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(from + at);
-            const unsigned w[4] = {x.x, x.y, x.z, x.w};
-            unsigned top = 0;
+    for (int u0 = threadIdx.x; u0 < units; u0 += THREADS * UNROLL) {
+        long place[UNROLL];
+        size_t at[UNROLL];
+        uint4 x[UNROLL][WORDS], code[UNROLL];
+        unsigned byte[UNROLL];
 #pragma unroll
-            for (int i = 0; i < 4; i++) top = max(top, max(w[i] & 0x7fff, (w[i] >> 16) & 0x7fff));
+        for (int j = 0; j < UNROLL; j++) {
+            const int u = min(u0 + j * THREADS, units - 1), lane = u % LANES, row = magic ? (int)__umulhi((unsigned)(u / LANES), magic) : u / LANES;
+            const int head = u / LANES - row * cache.kv_heads;
+            const long first = u0 + j * THREADS < units ? places[row] : -1;
+            place[j] = first < 0 ? -1 : first + ((long)head << cache.shift);       /* the same for the LANES lanes of a row */
+            at[j] = (size_t)(s.row0 + s.c0 + row) * ld + (size_t)head * HEAD + VALUES * lane;
+            const long safe = max(place[j], 0L) * LANES + lane;
+            if (WRITE) {
 #pragma unroll
-            for (int d = 1; d < LANES; d <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, d, 64));
-            float factor;
-            const unsigned byte = scale_byte(top, &factor);
-            int c[2] = {0, 0};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float lo = __uint_as_float(w[i] << 16) * factor, hi = __uint_as_float(w[i] & 0xffff0000u) * factor;
-                c[i / 2] = i % 2 ? __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, c[i / 2], true) : __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, c[i / 2], false);
+                for (int i = 0; i < WORDS; i++) x[j][i] = *reinterpret_cast<const uint4 *>(from + at[j] + 8 * i);
+            } else if (place[j] >= 0) {
+                code[j] = in_pages[safe];
+                if (FP8) byte[j] = bytes[place[j]];
             }
-            *reinterpret_cast<int2 *>(codes + in_pages) = byte == 255 ? make_int2(0x7f7f7f7f, 0x7f7f7f7f) : make_int2(c[0], c[1]);
-            if (lane == 0) bytes[place] = (uint8_t)byte;
-        } else {
-            const int2 c = *reinterpret_cast<const int2 *>(codes + in_pages);
-            const float scale = paged_scale(bytes[place]);
-            uint32_t w[4];
+        }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int word = i < 2 ? c.x : c.y;
-                const f32x2 f = i % 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(word, true) : __builtin_amdgcn_cvt_pk_f32_fp8(word, false);
-                w[i] = pack_bf16(f[0] * scale, f[1] * scale);
+        for (int j = 0; j < UNROLL; j++) {
+            const int lane = (u0 + j * THREADS) % LANES;
+            if constexpr (WRITE && FP8) {
+                unsigned w[8] = {x[j][0].x, x[j][0].y, x[j][0].z, x[j][0].w, x[j][WORDS - 1].x, x[j][WORDS - 1].y, x[j][WORDS - 1].z, x[j][WORDS - 1].w}, top = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) top = max(top, max(w[i] & 0x7fff, (w[i] >> 16) & 0x7fff));
+#pragma unroll
+                for (int d = 1; d < LANES; d <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, d, 64));
+                float factor;
+                byte[j] = scale_byte(top, &factor);
+                int c[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float lo = __uint_as_float(w[i] << 16) * factor, hi = __uint_as_float(w[i] & 0xffff0000u) * factor;
+                    c[i / 2] = i % 2 ? __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, c[i / 2], true) : __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, c[i / 2], false);
+                }
+                code[j] = byte[j] == 255 ? make_uint4(0x7f7f7f7f, 0x7f7f7f7f, 0x7f7f7f7f, 0x7f7f7f7f) : make_uint4(c[0], c[1], c[2], c[3]);
             }
-            *reinterpret_cast<uint4 *>(to + at) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (place[j] < 0) continue;
+            if constexpr (WRITE) {
+                in_pages[place[j] * LANES + lane] = FP8 ? code[j] : x[j][0];
+                if (FP8 && lane == 0) bytes[place[j]] = (uint8_t)byte[j];
+            } else if constexpr (FP8) {
+                const float scale = paged_scale(byte[j]);
+                const unsigned c[4] = {code[j].x, code[j].y, code[j].z, code[j].w};
+                uint32_t w[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const f32x2 f = i % 2 ? __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i / 2], true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i / 2], false);
+                    w[i] = pack_bf16(f[0] * scale, f[1] * scale);
+                }
+                *reinterpret_cast<uint4 *>(to + at[j]) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4 *>(to + at[j] + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+            } else {
+                *reinterpret_cast<uint4 *>(to + at[j]) = code[j];
+            }
         }
     }
 }
@@ -141,15 +173,24 @@ bool aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 template <bool FP8, bool WRITE>
 int launch(hipStream_t stream, Pair pages, Pair scales, ConstPair rows, Pair out, int ld, const PagedArg &c, const SequencesArg &seqs) {
-    const long wgs = 2 * sequence_tiles_at_most(seqs, ROWS);
+    const bool wide = ld % 8 == 0 && aligned(WRITE ? rows.k : out.k, 16) && aligned(WRITE ? rows.v : out.v, 16) && aligned(pages.k, 16) &&
+                      aligned(pages.v, 16) && (c.head_dim == 128 || c.head_dim == 64 || c.head_dim == 256) && c.kv_heads < 8192;
+    const bool large = wide && (long)seqs.rows * c.kv_heads >= 1 << 16;
+    const bool few = (long)seqs.rows * c.kv_heads * c.head_dim <= (long)seqs.n * THREADS * (FP8 ? 16 : 8);
+    const long wgs = 2 * sequence_tiles_at_most(seqs, large ? 4 * ROWS : ROWS);
     if (!wgs) return 0;
     if (wgs > ((1L << 32) - 1) / THREADS) return (int)hipErrorInvalidValue;
-    const bool wide = ld % 8 == 0 && aligned(WRITE ? rows.k : out.k, 16) && aligned(WRITE ? rows.v : out.v, 16) && aligned(pages.k, FP8 ? 8 : 16) &&
-                      aligned(pages.v, FP8 ? 8 : 16);
     const dim3 grid((unsigned)wgs), block(THREADS);
-    if (wide && c.head_dim == 128) hipLaunchKernelGGL((k_cache_rows<16, FP8, WRITE>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs);
-    else if (wide && c.head_dim == 64) hipLaunchKernelGGL((k_cache_rows<8, FP8, WRITE>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs);
-    else if (wide && c.head_dim == 256) hipLaunchKernelGGL((k_cache_rows<32, FP8, WRITE>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs);
+    const uint32_t magic = c.kv_heads > 1 ? (uint32_t)(((1ull << 32) + c.kv_heads - 1) / c.kv_heads) : 0;
+    auto rows_of = [&](auto head) {
+        constexpr int HEAD = decltype(head)::value;
+        if (large) hipLaunchKernelGGL((k_cache_rows<HEAD, FP8, WRITE, 4 * ROWS, 4>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs, magic);
+        else if (few) hipLaunchKernelGGL((k_cache_rows<HEAD, FP8, WRITE, ROWS, 1>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs, magic);
+        else hipLaunchKernelGGL((k_cache_rows<HEAD, FP8, WRITE, ROWS, 4>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs, magic);
+    };
+    if (wide && c.head_dim == 128) rows_of(std::integral_constant<int, 128>{});
+    else if (wide && c.head_dim == 64) rows_of(std::integral_constant<int, 64>{});
+    else if (wide) rows_of(std::integral_constant<int, 256>{});
     else hipLaunchKernelGGL((k_cache_rows_any<FP8, WRITE>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs);
     return (int)hipGetLastError();
 }

@@ -91,10 +91,14 @@ struct Work {
         const long most = (long)cache.ld << cache.shift;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            length[i] = base + 64 * i + (int)(threadIdx.x & 63) < n ? (int)min((long)max(length[i], 0), most) : 0;
-            empty = empty || __any(length[i] == 0 && base + 64 * i + (int)(threadIdx.x & 63) < n);
-            upto[i] = total + wave_sum_upto(tiles(length[i]) * per);
-            total = __builtin_amdgcn_readlane(upto[i], 63);
+            upto[i] = total;
+            if (base + 64 * i < n) {
+                const bool there = base + 64 * i + (int)(threadIdx.x & 63) < n;
+                length[i] = there ? (int)min((long)max(length[i], 0), most) : 0;
+                empty = empty || __any(there && length[i] == 0);
+                upto[i] += wave_sum_upto(tiles(length[i]) * per);
+                total = __builtin_amdgcn_readlane(upto[i], 63);
+            }
         }
     }
     __device__ __forceinline__ int tiles(int tokens) const { return (tokens + keys - 1) / keys; }
