@@ -140,7 +140,7 @@ __device__ __forceinline__ void walk(const Keys &keys, int nq, int m, int hd, fl
 __global__ void __launch_bounds__(64)
 k_sequences_any(uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k, const uint16_t *v, int ldkv, SequencesArg seqs,
                 int kv_heads, int hd, float scale, int causal) {
-    SequenceTiles tiles;
+    SequenceTiles<> tiles;
     const int count = tiles.count(seqs, QB), t = blockIdx.x / kv_heads, kvh = blockIdx.x % kv_heads, group = seqs.per_row;
     if (t >= count) return;
     const SequenceTile s = tiles.tile(t);

@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(THREADS)
 k_cache_rows(Pair pages, Pair scales, ConstPair rows, Pair out, int ld, PagedArg cache, SequencesArg seqs, uint32_t magic) {
     constexpr int VALUES = FP8 ? 16 : 8, LANES = HEAD / VALUES, WORDS = FP8 ? 2 : 1;      /* 16-byte words of bf16 to a unit */
     __shared__ long places[ROWS];
-    SequenceTiles tiles;
+    SequenceTiles<> tiles;
     const int count = tiles.count(seqs, ROWS), t = blockIdx.x >> 1;
     if (t >= count) return;
     const bool second = blockIdx.x & 1;
@@ -130,7 +130,7 @@ k_cache_rows(Pair pages, Pair scales, ConstPair rows, Pair out, int ld, PagedArg
 template <bool FP8, bool WRITE>
 __global__ void __launch_bounds__(THREADS)
 k_cache_rows_any(Pair pages, Pair scales, ConstPair rows, Pair out, int ld, PagedArg cache, SequencesArg seqs) {
-    SequenceTiles tiles;
+    SequenceTiles<> tiles;
     const int count = tiles.count(seqs, ROWS), t = blockIdx.x >> 1, hd = cache.head_dim;
     if (t >= count) return;
     const bool second = blockIdx.x & 1;

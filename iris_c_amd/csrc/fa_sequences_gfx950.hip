@@ -19,8 +19,9 @@
  * multiplied by zeros first, and if that gives anything but zeros its infinities and NaN are taken out of V, and put into the sums of the
  * columns that see them at the end.
  *
- * Workgroups: eight kv heads at a time (one to an XCD, whose L2 then holds the K and V of one head), tile by tile from the last one of
- * the last sequence on, which with a causal limit are the longest of their sequence. (All long ones of a batch first is no faster.)
+ * Workgroups: eight kv heads at a time (one to an XCD, whose L2 then holds the K and V of one head); with a causal limit from the last tile
+ * of the last sequence down, so that of each sequence the longest come first (those of all sequences first is no faster), otherwise
+ * sequence by sequence from the one with the most keys down.
  *
  * Where there are few columns and many keys, `ranges` workgroups share the key tiles of the same columns, evenly: each leaves its
  * unnormalised sums, their maximum and denominator in a workspace, and a second launch joins them.
@@ -117,12 +118,12 @@ struct Args {
 
 /* What a workgroup works on */
 struct Place { bool there; int kvh, tile, range; };
-__device__ __forceinline__ Place place(const Args &a, int count) {
+__device__ __forceinline__ Place place(const Args &a, int count, bool last_first) {
     const int together = a.kv_heads % 8 == 0 ? 8 : a.kv_heads;       /* kv heads whose tiles are dealt out in turn */
     const unsigned round = (unsigned)together * (unsigned)count, number = blockIdx.x / a.ranges;
     if (round == 0 || number / round >= (unsigned)(a.kv_heads / together)) return {false, 0, 0, 0};
     const unsigned rest = number % round;
-    return {true, (int)(number / round) * together + (int)(rest % together), count - 1 - (int)(rest / together), (int)(blockIdx.x % a.ranges)};
+    return {true, (int)(number / round) * together + (int)(rest % together), last_first ? count - 1 - (int)(rest / together) : (int)(rest / together), (int)(blockIdx.x % a.ranges)};
 }
 /* floats of a workgroup's partial result: sums of its columns, their maxima, their denominators */
 constexpr int part_floats(int columns) { return columns * (HD + 2); }
@@ -135,9 +136,9 @@ k_sequences_hd128(Args a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lg = lane >> 4;
     const int group = a.seqs.per_row;
 
-    SequenceTiles tiles;
+    SequenceTiles<!CAUSAL> tiles;
     const int count = tiles.count(a.seqs, COLUMNS);
-    const Place at = place(a, count);
+    const Place at = place(a, count, CAUSAL);
     if (!at.there) return;
     const SequenceTile s = tiles.tile(at.tile);
     const int kvh = at.kvh;
@@ -392,13 +393,13 @@ k_sequences_hd128(Args a) {
 
 /* The ranges of a workgroup's columns joined: 32 lanes to a column, 4 dims each, all ranges' loads under way together */
 constexpr int JOIN = 1024;
-template <int COLUMNS>
+template <int COLUMNS, bool CAUSAL>
 __global__ void __launch_bounds__(JOIN)
 k_sequences_join(Args a) {
-    SequenceTiles tiles;
+    SequenceTiles<!CAUSAL> tiles;
     const int ranges = a.ranges, count = tiles.count(a.seqs, COLUMNS), group = a.seqs.per_row;
     a.ranges = 1;                                                     /* a workgroup here for all ranges */
-    const Place at = place(a, count);
+    const Place at = place(a, count, CAUSAL);
     if (!at.there) return;
     const SequenceTile s = tiles.tile(at.tile);
     const int columns = min(COLUMNS, s.n * group - s.c0), lane = threadIdx.x & 31;
@@ -443,7 +444,7 @@ int launch(hipStream_t stream, const Args &a) {
     if (wgs * a.ranges > ((1L << 32) - 1) / (64 * WAVES)) return (int)hipErrorInvalidValue;
     hipLaunchKernelGGL((k_sequences_hd128<WAVES, NB, CAUSAL>), dim3((unsigned)(wgs * a.ranges)), dim3(64 * WAVES), LDS, stream, a);
     if constexpr (NB == 1 && WAVES == 4)
-        if (a.ranges > 1) hipLaunchKernelGGL((k_sequences_join<16 * NB * WAVES>), dim3((unsigned)wgs), dim3(JOIN), 0, stream, a);
+        if (a.ranges > 1) hipLaunchKernelGGL((k_sequences_join<16 * NB * WAVES, CAUSAL>), dim3((unsigned)wgs), dim3(JOIN), 0, stream, a);
     return (int)hipGetLastError();
 }
 

@@ -15,7 +15,7 @@
 struct SequencesArg { const int *first_row, *first_key; int n, rows, keys, per_row; };       /* the kernels' argument */
 
 /* the tile's columns are c0 .. c0 + height - 1 of the sequence's n * per_row; column c is row row0 + c / per_row */
-struct SequenceTile { int row0, n, c0, key0, m, g; };
+struct SequenceTile { int row0, n, c0, key0, m, g; };        /* g: the sequence's number, in order */
 
 /* inclusive sum and maximum over the lanes up to each one, in the vector registers (shifts inside rows of 16, then the rows' last
  * lanes to those behind them): a tenth of the time of six trips through the LDS */
@@ -41,6 +41,9 @@ __device__ __forceinline__ int wave_max_upto(int v) {                    /* of v
     return v;
 }
 
+/* BY_LENGTH: up to 64 sequences in the order of their keys, the most first, for kernels whose tiles take as long as the keys are many: the
+ * last workgroups of a call are then short ones. */
+template <bool BY_LENGTH = false>
 struct SequenceTiles {
     static constexpr int AT_ONCE = 4;                                /* 64 sequences at once: their bounds are one trip to memory */
     SequencesArg a;
@@ -56,6 +59,19 @@ struct SequenceTiles {
         hi = min(y, limit);
     }
     __device__ __forceinline__ int tiles(int i) const { return ((hi[i] - lo[i]) * a.per_row + height - 1) / height; }
+    /* the first 64: each to the lane that is the number of those with more keys, or as many and in front */
+    __device__ __forceinline__ void by_length() {
+        const int lane = threadIdx.x & 63, m = khi[0] - klo[0];
+        int to = lane < a.n ? 0 : lane;
+        for (int j = 0; j < a.n; j++) {
+            const int other = __builtin_amdgcn_readlane(m, j);
+            if (lane < a.n) to += other > m || (other == m && j < lane);
+        }
+        lo[0] = __builtin_amdgcn_ds_permute(4 * to, lo[0]);
+        hi[0] = __builtin_amdgcn_ds_permute(4 * to, hi[0]);
+        klo[0] = __builtin_amdgcn_ds_permute(4 * to, klo[0]);
+        khi[0] = __builtin_amdgcn_ds_permute(4 * to, khi[0]);
+    }
     __device__ __forceinline__ void look(int base) {
         const int lane = threadIdx.x & 63;
         int from[AT_ONCE], to[AT_ONCE], kfrom[AT_ONCE], kto[AT_ONCE];
@@ -75,6 +91,7 @@ struct SequenceTiles {
                 range(from[i], to[i], a.rows, most, lo[i], hi[i]);
                 klo[i] = lo[i]; khi[i] = hi[i];
                 if (a.first_key) range(kfrom[i], kto[i], a.keys, key_most, klo[i], khi[i]);
+                if (BY_LENGTH && i == 0 && a.n > 1 && a.n <= 64) by_length();
                 upto[i] += wave_sum_upto(tiles(i));
                 total = __builtin_amdgcn_readlane(upto[i], 63);
             }
