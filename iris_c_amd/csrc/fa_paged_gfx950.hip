@@ -397,7 +397,7 @@ k_paged_hd128(Args a) {
 #pragma unroll
                 for (int db = 0; db < 8; db++) o[db] *= alpha;
             }
-            u32x4 pw[MB / 2];
+            u32x4 pw[MB / 2], rest[MB / 2];                               /* p in bf16 and what is left of it: together 16 bits */
 #pragma unroll
             for (int kg = 0; kg < MB / 2; kg++) {
                 float p[8];
@@ -412,7 +412,14 @@ k_paged_hd128(Args a) {
 #pragma unroll
                     for (int r = 0; r < 4; r++) { p[r] = ldexpf(p[r], (int)v0[r] - 127); p[4 + r] = ldexpf(p[4 + r], (int)v1[r] - 127); }
                 }
-                pw[kg] = u32x4{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])};
+                /* The upper part is cut off and not rounded, and the rest made more than zero: an infinity in V times both is that infinity. (Masked
+                 * keys have zeros for V.) */
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t c0 = __float_as_uint(p[2 * i]) & 0xffff0000u, c1 = __float_as_uint(p[2 * i + 1]) & 0xffff0000u;
+                    pw[kg][i] = (c0 >> 16) | c1;
+                    rest[kg][i] = pack_bf16(fmaxf(p[2 * i] - __uint_as_float(c0), 0x1p-126f), fmaxf(p[2 * i + 1] - __uint_as_float(c1), 0x1p-126f));
+                }
             }
 #pragma unroll
             for (int kg = 0; kg < MB / 2; kg++)
@@ -430,6 +437,7 @@ k_paged_hd128(Args a) {
                         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(vp + 16 * S::ROW));
                         va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
                     }
+                    o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, rest[kg]), o[db], 0, 0, 0);
                     o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, pw[kg]), o[db], 0, 0, 0);
                 }
             wait_lds();                                                  /* this stage has been read */

@@ -361,6 +361,19 @@ def test_values_that_are_not_numbers_reach_their_own_sequence(dev, bad, kind):
     dev.free_all()
 
 
+@pytest.mark.parametrize("bad", [np.inf, -np.inf])
+def test_every_infinity_comes_through_as_itself(dev, bad):
+    """One in each row of V, in a dim of its own: whatever the probability of the row, the sum over the keys is that infinity in these dims"""
+    kv, hd, heads, n = 1, 128, 16, 100
+    c = filled(dev, "bf16", [n], 16, kv, hd)
+    v = rows(9, n, kv * hd)
+    v[np.arange(n), np.arange(n)] = sr.bf16_round(np.float32(bad))
+    c.write([n], rows(8, n, kv * hd), v, [0, n])
+    got = sr.bf16_value(c.attend([n], rows(3, 1, heads * hd), heads, hd ** -0.5, compare=False)).reshape(heads, hd)
+    assert (got[:, :n] == bad).all() and np.isfinite(got[:, n:]).all()
+    dev.free_all()
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_a_query_that_is_not_a_number_is_the_only_one(dev, kind):
     c = filled(dev, kind, [50, 60, 40], 16, 2, 128)
