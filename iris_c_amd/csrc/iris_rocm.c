@@ -654,9 +654,9 @@ void iris_dev_attention_sequences(uint16_t *out, int ldo, const uint16_t *q, int
     }
     if (!first_row || !out || !q || (keys && (!k || !v))) { fail(-1, what, "first_row, out, q, k or v is missing"); return; }
     if (!first_key && keys != rows) { fail(-1, what, "without first_key the keys are the rows: need keys == rows"); return; }
-    if ((long long)rows * heads > INT32_MAX || (long long)heads * head_dim > INT32_MAX || ldo < heads * head_dim || ldq < heads * head_dim ||
+    if ((long long)rows * heads > INT32_MAX || keys > INT32_MAX - 64 || (long long)heads * head_dim > INT32_MAX || ldo < heads * head_dim || ldq < heads * head_dim ||
         (keys && ldkv < kv_heads * head_dim)) {
-        fail(-1, what, "need rows * heads < 2^31, ldo and ldq >= heads * head_dim, ldkv >= kv_heads * head_dim");
+        fail(-1, what, "need rows * heads < 2^31, keys < 2^31 - 64, ldo and ldq >= heads * head_dim, ldkv >= kv_heads * head_dim");
         return;
     }
     if (!need_ready(what)) return;
@@ -684,6 +684,7 @@ static int cache_args(const char *what, const void *k_pages, const void *v_pages
         fail(-1, what, "need pages >= 0, table_ld >= 0 and page_size a power of two");
         return 0;
     }
+    if ((long long)table_ld * page_size > INT32_MAX - 64) { fail(-1, what, "need table_ld * page_size < 2^31 - 64"); return 0; }
     if (!k_pages || !v_pages || !page_table || !lengths || (fp8 && (!k_scales || !v_scales))) {
         fail(-1, what, "pages, scales, page_table or lengths are missing");
         return 0;

@@ -32,9 +32,9 @@ ENTRIES = {
     "cache_write_fp8": with_scales(WRITE), "cache_read_bf16": READ, "cache_read_fp8": with_scales(READ),
 }
 SEQ_BAD = [dict(out=None), dict(q=None), dict(k=None), dict(v=None), dict(first_row=None), dict(keys=9), dict(keys=-1), dict(kv=3), dict(kv=0), dict(kv=-2), dict(hd=0),
-           dict(sequences=-1), dict(ldo=1023), dict(ldq=1000), dict(ldkv=255), dict(rows=2 ** 28, keys=2 ** 28), dict(heads=2 ** 24, kv=2 ** 24)]
+           dict(sequences=-1), dict(ldo=1023), dict(ldq=1000), dict(ldkv=255), dict(rows=2 ** 28, keys=2 ** 28), dict(heads=2 ** 24, kv=2 ** 24), dict(first_key=A, keys=2 ** 31 - 63)]
 CACHE_BAD = [dict(k=None), dict(v=None), dict(table=None), dict(lengths=None), dict(page=0), dict(page=24), dict(page=-16), dict(pages=-1), dict(ld=-1), dict(sequences=-1),
-             dict(kv=0), dict(hd=0), dict(hd=-128)]
+             dict(kv=0), dict(hd=0), dict(hd=-128), dict(ld=2 ** 27), dict(ld=2, page=2 ** 30)]
 ROWS_BAD = [dict(kn=None), dict(vn=None), dict(ldn=255), dict(first=None)]
 BAD = [("attention_sequences", b) for b in SEQ_BAD]
 BAD += [(e, b) for e in ENTRIES if e != "attention_sequences" for b in CACHE_BAD]
@@ -83,3 +83,52 @@ def test_the_numbers_of_the_tests_against_torch():
     assert np.array_equal(c, torch.tensor(x / scale).to(torch.float8_e4m3fn).view(torch.uint8).numpy())
     got = sr.e4m3_value(c) * scale
     assert (np.abs(got - x) <= np.maximum(np.abs(x) * 2.0 ** -4, scale * 2.0 ** -10)).all()
+
+
+PART = 64 << 20                             # the workspace that the ranges of a call share with the linear layers
+
+
+def plan(lib, n, rows, keys, heads, kv, causal, own):
+    import ctypes as C
+    out = [C.c_int() for _ in range(3)]
+    lib.iris_hip_sequences_plan(n, rows, keys, heads, kv, causal, own, *(C.byref(x) for x in out))
+    return tuple(x.value for x in out)
+
+
+def test_ranges_of_keys_fit_the_workspace(lib):
+    """Any sizes: the shape is one that there is a kernel for, keys are cut with 64 columns to a workgroup only, and what all workgroups that
+    the launch may have leave there fits"""
+    rng = np.random.default_rng(0)
+    cut = 0
+    for _ in range(20000):
+        kv = int(rng.choice([1, 2, 3, 6, 8, 24, 100]))
+        heads = kv * int(rng.choice([1, 2, 4, 5, 8, 16, 60]))
+        n, rows = int(2 ** rng.uniform(0, 12)), int(2 ** rng.uniform(0, 18))
+        own = bool(rng.integers(2))
+        keys = rows if own else int(2 ** rng.uniform(0, 24))
+        waves, blocks, ranges = plan(lib, n, rows, keys, heads, kv, int(rng.integers(2)), own)
+        assert (waves, blocks) in {(1, 1), (2, 1), (4, 1), (8, 1), (4, 2), (8, 2)} and 1 <= ranges <= 8
+        if ranges > 1:
+            cut += 1
+            assert (waves, blocks) == (4, 1)
+            tiles = (rows * (heads // kv) + min(n, rows) * 63) // 64 * kv
+            assert tiles * ranges * 64 * 130 * 4 <= PART, (n, rows, keys, heads, kv)
+    assert cut > 1000
+
+
+def test_shapes_of_known_calls(lib):
+    assert plan(lib, 1, 31, 31, 32, 8, 1, 1) == (2, 1, 1)
+    assert plan(lib, 1, 512, 512, 32, 8, 1, 1) == (4, 1, 1)
+    assert plan(lib, 1, 4608, 4608, 24, 24, 0, 1) == (8, 2, 1)
+    assert plan(lib, 4, 16797, 16797, 32, 8, 1, 1) == (4, 2, 1)
+    assert plan(lib, 1, 32, 16000, 32, 8, 1, 0) == (4, 1, 8)
+    assert plan(lib, 1, 64, 200, 32, 8, 1, 0)[2] == 1
+
+
+def test_sizes_that_the_matrix_core_kernel_has_numbers_for(lib):
+    takes = lambda pages, shift, ld, n, heads, kv: lib.iris_hip_paged_hd128_takes(pages, shift, ld, n, heads, kv)
+    assert takes(1000, 6, 64, 256, 32, 8) == 1
+    assert takes(2 ** 23, 6, 10, 1, 8, 8) == 0                       # 2^32 rows
+    assert takes(2 ** 23 - 1, 6, 10, 1, 8, 8) == 1
+    assert takes(10, 6, 2 ** 20, 2048, 32, 32) == 0                  # 2^37 tiles, if all were as long as the table
+    assert lib.iris_dev_attention_paged_workspace() == 2 * 1024 * (16 * 128 + 32) * 4
