@@ -144,8 +144,7 @@ struct Ranges {
         return u < front ? u / (each + 1) : more + (u - front) / each;
     }
 };
-/* every range has two tiles at least, where there are as many */
-__device__ __forceinline__ int ranges(int total, int most) { return min(most, max(1, total / 2)); }
+__device__ __forceinline__ int ranges(int total, int most) { return min(most, max(1, total)); }
 
 struct Args {
     uint16_t *out;
@@ -464,9 +463,10 @@ k_paged_hd128(Args a) {
     }
 }
 
-/* Workgroup w joins the list entry that the end of range w cuts, if it is the first end in it. 32 lanes take 4 dims each of a column and
- * every so many-th part, eight at a time so that their loads are under way together; the LDS joins what several groups of 32 have. */
-template <int JOIN>
+/* Workgroup w stands for the end of range w. Those whose ends cut the same list entry share its columns: the entry's parts are those of
+ * the ranges w0 .. last, and w takes every (last - w0)-th column from w - w0 on. 32 lanes take 4 dims each of a column and every so many-th
+ * part, eight at a time so that their loads are under way together; the LDS joins what several groups of 32 have. */
+constexpr int JOIN = 256;
 __global__ void __launch_bounds__(JOIN)
 k_paged_join(Args a, int keys) {
     __shared__ f32x4 sums[JOIN];
@@ -480,24 +480,26 @@ k_paged_join(Args a, int keys) {
     int g, length, tiles, before;
     work.find(u, &g, &length, &tiles, &before);
     const int entry = (u - before) / tiles, first = before + entry * tiles;
-    if (first == u || first < range.begin(w)) return;
-    const int last = range.of(first + tiles - 1);
-    const int kvh = entry / a.blocks, block = entry - kvh * a.blocks, cols = min(COLS, a.group - block * COLS);
+    if (first == u) return;                                          /* nothing is cut here */
+    const int w0 = range.of(first), last = range.of(first + tiles - 1), sharers = last - w0;
+    const int kvh = entry / a.blocks, block = entry - kvh * a.blocks, all = min(COLS, a.group - block * COLS);
+    const int cols = (all - (w - w0) + sharers - 1) / sharers;       /* of this workgroup; not more than none where there are fewer than sharers */
     constexpr int UNITS = JOIN / 32;
     int places = 1;                                                  /* columns at a time */
     while (places < cols && places < UNITS) places *= 2;
     const int groups = UNITS / places, unit = threadIdx.x >> 5, part = unit / places, at = threadIdx.x & 31;
-    for (int c = unit & (places - 1), turn = 0; turn < cols; turn += places, c += places) {
+    for (int n = unit & (places - 1), turn = 0; turn < cols; turn += places, n += places) {
+        const int c = w - w0 + n * sharers;
         float top = -INFINITY, den = 0.0f;
         f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (c < cols) {
-            for (int i0 = w + part; i0 <= last; i0 += 8 * groups) {
+        if (n < cols) {
+            for (int i0 = w0 + part; i0 <= last; i0 += 8 * groups) {
                 float t[8], d[8];
                 f32x4 o[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int i = min(i0 + j * groups, last);
-                    const float *pp = a.part + (size_t)(2 * i + (i == w)) * PART;
+                    const float *pp = a.part + (size_t)(2 * i + (i == w0)) * PART;
                     t[j] = i0 + j * groups <= last ? pp[COLS * HD + c] : -INFINITY;
                     d[j] = pp[COLS * HD + COLS + c];
                     o[j] = *reinterpret_cast<const f32x4 *>(pp + c * HD + 4 * at);
@@ -522,7 +524,7 @@ k_paged_join(Args a, int keys) {
         sums[threadIdx.x] = sum;
         if (at == 0) { tops[unit] = top; dens[unit] = den; }
         __syncthreads();
-        if (part == 0 && c < cols) {
+        if (part == 0 && n < cols) {
             float now = top;
             for (int j = 1; j < groups; j++) now = fmaxf(now, tops[unit + j * places]);
             const float base = now == -INFINITY ? 0.0f : now, alpha = __builtin_amdgcn_exp2f(top - base);
@@ -559,7 +561,7 @@ extern "C" int iris_hip_paged_hd128(void *stream, float *part, uint16_t *out, in
                     ldo, ldq, n, group, blocks, scale * 1.4426950408889634f, part};
     const long tiles = ((((long)table_ld << page_shift) + keys - 1) / keys) * n * kv_heads * blocks;
     const int q_rows = group <= 4 ? 4 : group <= 8 ? 8 : 16;          /* with 16 rows of Q for two list entries three waves have room in a CU's LDS */
-    const int most = q_rows == 16 ? MOST_WAVES / 4 * 3 : MOST_WAVES, waves = tiles / 2 < 1 ? 1 : tiles / 2 < most ? (int)(tiles / 2) : most;
+    const int most = q_rows == 16 ? MOST_WAVES / 4 * 3 : MOST_WAVES, waves = tiles < 1 ? 1 : tiles < most ? (int)tiles : most;
     auto run = [&](auto fp8, auto rows) {
         constexpr int QROWS = decltype(rows)::value, LDS = STAGES * Shape<decltype(fp8)::value>::STAGE + 2 * QROWS * 2 * HD + 512;
         hipLaunchKernelGGL((k_paged_hd128<decltype(fp8)::value, QROWS>), dim3(waves), dim3(64), LDS, (hipStream_t)stream, a);
@@ -571,10 +573,6 @@ extern "C" int iris_hip_paged_hd128(void *stream, float *part, uint16_t *out, in
     };
     if (ks) run_rows(std::true_type{});
     else run_rows(std::false_type{});
-    /* as many threads as parts are to be expected: a thousand workgroups of 512 take 2 us to start */
-    if (waves > 1) {
-        if (waves <= 8L * n * kv_heads * blocks) hipLaunchKernelGGL(k_paged_join<256>, dim3(waves), dim3(256), 0, (hipStream_t)stream, a, keys);
-        else hipLaunchKernelGGL(k_paged_join<512>, dim3(waves), dim3(512), 0, (hipStream_t)stream, a, keys);
-    }
+    if (waves > 1) hipLaunchKernelGGL(k_paged_join, dim3(waves), dim3(JOIN), 0, (hipStream_t)stream, a, keys);
     return (int)hipGetLastError();
 }
