@@ -78,10 +78,11 @@ struct SequenceTiles {
 #pragma unroll
         for (int i = 0; i < AT_ONCE; i++) {
             const int g = min(base + 64 * i + lane, a.n), next = min(g + 1, a.n);        /* behind the last one: no rows */
-            from[i] = a.first_row ? a.first_row[g] : g;
-            to[i] = a.first_row ? a.first_row[next] : next;
-            kfrom[i] = a.first_key ? a.first_key[g] : 0;
-            kto[i] = a.first_key ? a.first_key[next] : 0;
+            from[i] = g; to[i] = next; kfrom[i] = kto[i] = 0;
+            if (base + 64 * i < a.n) {
+                if (a.first_row) { from[i] = a.first_row[g]; to[i] = a.first_row[next]; }
+                if (a.first_key) { kfrom[i] = a.first_key[g]; kto[i] = a.first_key[next]; }
+            }
         }
 #pragma unroll
         for (int i = 0; i < AT_ONCE; i++) {
