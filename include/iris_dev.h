@@ -271,8 +271,10 @@ void iris_dev_linear_mxfp4_bf16_grouped(uint16_t *y, const uint8_t *x, const uin
  * causal: the last row of a sequence sees all of its keys, each row in front of it one key less: row i of n sees the keys
  * j <= i + (m - n) of m. A row that sees no key gives zeros. What it does not see has no part in its result, infinities and NaN included.
  * head_dim 128 on rows that are 16-byte aligned (out: 8) and scale > 0 run on the matrix cores, everything else on a scalar kernel. P is
- * rounded to bf16 for the P V product and the row sums are those of the rounded values, as in iris_dev_attention.
- * Needs rows * heads < 2^31; larger calls, and those that no launch holds, are reported. */
+ * rounded to bf16 for the P V product and the row sums are those of the rounded values, as in iris_dev_attention. The keys of a few rows
+ * over many keys are cut into ranges whose partial results pass through the private memory of the linear layers; under stream capture they
+ * are not, and the f32 sums are then taken in another order. A call gives the same bits every time.
+ * Needs rows * heads < 2^31 and keys < 2^31 - 64; larger calls, and those that no launch holds, are reported. */
 void iris_dev_attention_sequences(uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k, const uint16_t *v, int ldkv,
                                   const int *first_row, const int *first_key, int sequences, int rows, int keys,
                                   int heads, int kv_heads, int head_dim, float scale, int causal);
@@ -281,8 +283,9 @@ void iris_dev_attention_sequences(uint16_t *out, int ldo, const uint16_t *q, int
  * bits (e4m3: sign, four bits of exponent, three of fraction, largest 448) with a scale byte s, 2^(s - 127), 255 for NaN, for each token's
  * row of a head: [pages, kv_heads, page_size]. page_table: device int [sequences, table_ld], position p of sequence g is place
  * p % page_size of page page_table[g * table_ld + p / page_size]; lengths: device int [sequences], the tokens of each sequence, those
- * that the call brings included. Both are read when the call runs. A page number outside 0 .. pages - 1 is a page that is not there: its
- * positions are not written, not read, and no keys. Lengths count as limited to 0 .. table_ld * page_size. Sequences may share pages. */
+ * that the call brings included. Both are read when the call runs. A page number outside 0 .. pages - 1 is a page that is not there, and so is
+ * what lies past the table: its positions are not written, not read, and no keys. A length below 0 counts as 0. table_ld * page_size has to be
+ * less than 2^31 - 64. Sequences may share pages. */
 
 /* The rows of the sequences (k and v: rows of kv_heads * head_dim, stride ld) into their pages: of a sequence with n rows, row i goes to
  * position lengths[g] - n + i; positions below 0, and those that the table does not reach, are left out. first_row NULL: row g is the one

@@ -23,8 +23,15 @@
  * of the last sequence down, so that of each sequence the longest come first (those of all sequences first is no faster), otherwise
  * sequence by sequence from the one with the most keys down.
  *
+ * What bounds it: 12001 + 4096 + 700 + 1 causal rows, 32 heads on 8, take 1.28 - 1.36 ms (by box), 0.97 - 1.03 PFLOP/s; pictures of 4608,
+ * 1536, 2627 and 576 rows, 24 heads, 360 - 390 us (1.05 PFLOP/s). The matrix cores are busy 45 % of the cycles of all SIMDs, no LDS access
+ * conflicts, 95 % of the requests of the first are served by the L2s; as in the kernel for one sequence the rest is the softmax's vector
+ * instructions (a thousand cycles beside 1088 of products per wave and tile) and what the chip's power leaves of the clock. 24 prompts of 4
+ * to 512 rows take 20 us: workgroups of about 4 us of dependent reads (bounds, first tiles) and up to 8 tiles of 1.3 us, two on a CU.
+ *
  * Where there are few columns and many keys, `ranges` workgroups share the key tiles of the same columns, evenly: each leaves its
- * unnormalised sums, their maximum and denominator in a workspace, and a second launch joins them.
+ * unnormalised sums, their maximum and denominator in a workspace, and a second launch joins them: 64 + 1 + 200 + 17 rows over 8294 keys
+ * 90 us in one range, 46 in three (6 of them to join), 32 rows over 16000 keys 314 and 53.
  */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -454,6 +461,10 @@ int launch(hipStream_t stream, const Args &a) {
 extern "C" void iris_hip_sequences_plan(int n, int rows, int keys, int heads, int kv_heads, int causal, int own_keys, int *waves, int *blocks, int *ranges) {
     const int group = heads / kv_heads;
     const long some = n < rows ? n : rows, blocks16 = ((long)rows * group + some * 8) / 16 * kv_heads, each = (long)rows * group / some;
+    /* Measured, us, by waves x blocks (all with 32 query heads on 8 unless noted). Causal: 118 rows 8.0 with 2 x 1, 8.3 with 4 x 1, 9.9 with 8 x 1;
+     * 512 rows 17.8 / 16.8 / 18.8, 4 x 2 20.6; 1024 40.6 / 28.1 / 31.1, 4 x 2 34.0; 2048 4 x 1 67.7, 8 x 1 65.1, 4 x 2 62.1, 8 x 2 73.4; 4096 219 / 212 / 161 /
+     * 154; 8192 800 / 757 / 546 / 548; 64 prompts of 4 to 512 78.3 / 84.2 / 63.9 / 76.6; 24 heads on 24, 2048 rows 64.3 / 69.9 / 75.5 / 71.6. Not causal, 24 heads on
+     * 24: 1280 rows 32.3 / 30.3 / 33.4 / 43.0; 4608 349 / 348 / 277 / 257; 600 + 320 + 900 37.4 / 39.5 / 38.3 / 36.6. */
     *blocks = *ranges = 1;
     if (causal) {
         *waves = blocks16 <= 640 ? 2 : 4;
@@ -464,7 +475,9 @@ extern "C" void iris_hip_sequences_plan(int n, int rows, int keys, int heads, in
     }
     while (*waves > 1 && each <= 8 * *waves * *blocks) *waves /= 2;
     if (*blocks == 2 && *waves < 4) { *waves = 2 * *waves; *blocks = 1; }
-    /* key tiles that a workgroup sees, about, and workgroups of 64 columns */
+    /* Key tiles that a workgroup sees, about, and workgroups of 64 columns: where those leave CUs idle (two have room on one) and walk long. us, 1 / 2 / 3 /
+     * 4 / 6 / 8 ranges: 64 + 1 + 200 + 17 rows over 8294 keys 85 / 57 / 46 / 50 / 51 / 54; 32 over 16000 314 / 167 / 116 / 89 / 65 / 53; 8 x 16 rows over 9464 keys 65 / 43 / 34 / 30 / 26 / 27;
+     * 118 rows over their own 8.3 / 16.6 (a second launch). */
     const long chain = (long)keys / some / KEYS / (causal && own_keys ? 2 : 1), wgs = (((long)rows * group + some * 32) / 64 + 1) * kv_heads;
     const long room = (long)(IRIS_LINEAR_PART_BYTES / sizeof(float) / part_floats(64)) / (sequence_tiles_at_most({nullptr, nullptr, n, rows, keys, group}, 64) * kv_heads);
     if (chain >= 12 && wgs <= 256) {
