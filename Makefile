@@ -59,7 +59,7 @@ iris_c_amd/libiris_microbench.so: $(CSRC)/microbench.hip
 	$(HIPCC) $(HIPFLAGS) -shared -o $@ $<
 
 $(CSRC)/%.o: $(CSRC)/%.hip $(CSRC)/iris_kernels_hip.h $(CSRC)/norm_rope_math.h $(CSRC)/write_through.h $(CSRC)/row_groups.h $(CSRC)/half_words.h \
-                   $(CSRC)/sequences.h $(CSRC)/paged_cache.h
+                   $(CSRC)/sequences.h $(CSRC)/paged_cache.h $(CSRC)/join_parts.h
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@
 
 $(CSRC)/iris_rocm.o: $(CSRC)/iris_rocm.c $(HOST_HDRS)

@@ -37,6 +37,7 @@
 #include <type_traits>
 
 #include "iris_kernels_hip.h"
+#include "join_parts.h"
 #include "paged_cache.h"
 #include "sequences.h"
 
@@ -55,7 +56,9 @@ namespace {
 
 constexpr int HD = 128, COLS = 16, STAGES = 2;
 constexpr int MOST_WAVES = 1024;                                     /* ranges: four waves on each of 256 CUs, as the LDS holds */
-constexpr int PART = COLS * HD + 2 * COLS;                           /* floats of a place in the workspace: sums, maxima, denominators */
+constexpr int PART = part_floats(COLS, HD);                          /* floats of a place in the workspace: sums, maxima, denominators */
+/* The list entry that the end of a range cuts: its first tile and their number (0: none is cut); and the tiles of the call */
+struct Cut { int g, head, cols, first, tiles, total, unused[2]; };
 constexpr float RAISE = 8.0f;                                        /* the maximum is raised by more than 2^8 only: p stays below that */
 constexpr unsigned NO_ROW = 0xffffffffu;
 
@@ -160,8 +163,9 @@ struct Args {
     const uint8_t *ks, *vs;
     PagedArg cache;
     int ldo, ldq, n, group, blocks;              /* group: query heads of a kv head, in blocks of 16 */
-    float scale_log2, *part;
+    float scale_log2, *part;                     /* part: two places a range, then a Cut each */
 };
+__device__ __forceinline__ Cut *cut_at(const Args &a, int w) { return reinterpret_cast<Cut *>(a.part + (size_t)2 * MOST_WAVES * PART) + w; }
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -206,14 +210,14 @@ k_paged_hd128(Args a) {
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)lds);
     Work work;
     const int total = work.count(a.cache, a.n, per, S::KEYS), waves = ranges(total, gridDim.x);
+    if (w >= total && lane == 0) cut_at(a, w)->tiles = 0;
     for (int g = work.empty ? w : a.n; g < a.n; g += gridDim.x)
         if (paged_length(a.cache, g) == 0)
             for (int c = lane; c < a.group * a.cache.kv_heads * (HD / 4); c += 64)
                 *reinterpret_cast<uint2 *>(a.out + (size_t)g * a.ldo + 4 * (size_t)c) = make_uint2(0, 0);
-    if (w >= waves) return;
     const Ranges range(total, waves);
     const int begin = range.begin(w), end = range.begin(w + 1);
-    if (begin == end) return;                                        /* no keys at all */
+    if (w >= waves || begin == end) return;                          /* no keys at all */
 
     /* The tile that is asked for next, and the pages of 64 page-fuls of tokens from the one that it begins in. */
     int u = begin - 1, g = 0, length = 0, tiles = 1, before = 0, tile = 0, kvh = 0, block = 0, q_turn = 0;
@@ -309,7 +313,14 @@ k_paged_hd128(Args a) {
     Tile now, next;
     bool stored = false;
     step();
-    wait_loads<0>();
+    {
+        /* meanwhile, for the second launch: the entry that the range ends in */
+        int g1, length1, tiles1, before1;
+        work.find(end - 1, &g1, &length1, &tiles1, &before1);
+        const int entry1 = (end - 1 - before1) / tiles1, first1 = before1 + entry1 * tiles1, kvh1 = entry1 / a.blocks, c1 = (entry1 - kvh1 * a.blocks) * COLS;
+        if (lane == 0) *cut_at(a, w) = Cut{g1, kvh1 * a.group + c1, min(COLS, a.group - c1), first1, first1 + tiles1 > end ? tiles1 : 0, total, {}};
+    }
+    wait_loads<1>();                                                 /* all but that store */
     asked = false;
     /* The first two turns only ask (one place in the code for it: a short call is as long as its instructions take to come from memory). */
     for (int t = begin - 2, stage = 0; t < end; t++, stage ^= 1) {
@@ -471,87 +482,23 @@ k_paged_hd128(Args a) {
 }
 
 /* Workgroup w stands for the end of range w. Those whose ends cut the same list entry share its columns: the entry's parts are those of
- * the ranges w0 .. last, and w takes every (last - w0)-th column from w - w0 on. 32 lanes take 4 dims each of a column and every so many-th
- * part, eight at a time so that their loads are under way together; the LDS joins what several groups of 32 have. */
+ * the ranges w0 .. last, and w takes every (last - w0)-th column from w - w0 on. */
 constexpr int JOIN = 256;
 __global__ void __launch_bounds__(JOIN)
-k_paged_join(Args a, int keys) {
-    __shared__ f32x4 sums[JOIN];
-    __shared__ float tops[JOIN / 32], dens[JOIN / 32];
-    const int w = blockIdx.x, per = a.cache.kv_heads * a.blocks;
-    Work work;
-    const int total = work.count(a.cache, a.n, per, keys), waves = ranges(total, gridDim.x);
-    if (w + 1 >= waves) return;
-    const Ranges range(total, waves);
-    const int u = range.begin(w + 1);
-    int g, length, tiles, before;
-    work.find(u, &g, &length, &tiles, &before);
-    const int entry = (u - before) / tiles, first = before + entry * tiles;
-    if (first == u) return;                                          /* nothing is cut here */
-    const int w0 = range.of(first), last = range.of(first + tiles - 1), sharers = last - w0;
-    const int kvh = entry / a.blocks, block = entry - kvh * a.blocks, all = min(COLS, a.group - block * COLS);
-    const int cols = (all - (w - w0) + sharers - 1) / sharers;       /* of this workgroup; not more than none where there are fewer than sharers */
-    constexpr int UNITS = JOIN / 32;
-    int places = 1;                                                  /* columns at a time */
-    while (places < cols && places < UNITS) places *= 2;
-    const int groups = UNITS / places, unit = threadIdx.x >> 5, part = unit / places, at = threadIdx.x & 31;
-    for (int n = unit & (places - 1), turn = 0; turn < cols; turn += places, n += places) {
-        const int c = w - w0 + n * sharers;
-        float top = -INFINITY, den = 0.0f;
-        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (n < cols) {
-            for (int i0 = w0 + part; i0 <= last; i0 += 8 * groups) {
-                float t[8], d[8];
-                f32x4 o[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int i = min(i0 + j * groups, last);
-                    const float *pp = a.part + (size_t)(2 * i + (i == w0)) * PART;
-                    t[j] = i0 + j * groups <= last ? pp[COLS * HD + c] : -INFINITY;
-                    d[j] = pp[COLS * HD + COLS + c];
-                    o[j] = *reinterpret_cast<const f32x4 *>(pp + c * HD + 4 * at);
-                }
-                float now = top;
-#pragma unroll
-                for (int j = 0; j < 8; j++) now = fmaxf(now, t[j]);
-                const float base = now == -INFINITY ? 0.0f : now, alpha = __builtin_amdgcn_exp2f(top - base);
-                sum *= alpha;
-                den *= alpha;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    if (i0 + j * groups > last) break;
-                    const float f = __builtin_amdgcn_exp2f(t[j] - base);
-                    sum += o[j] * f;
-                    den += d[j] * f;
-                }
-                top = now;
-            }
-        }
-        __syncthreads();                                             /* the columns before these have been read */
-        sums[threadIdx.x] = sum;
-        if (at == 0) { tops[unit] = top; dens[unit] = den; }
-        __syncthreads();
-        if (part == 0 && n < cols) {
-            float now = top;
-            for (int j = 1; j < groups; j++) now = fmaxf(now, tops[unit + j * places]);
-            const float base = now == -INFINITY ? 0.0f : now, alpha = __builtin_amdgcn_exp2f(top - base);
-            sum *= alpha;
-            den *= alpha;
-            for (int j = 1; j < groups; j++) {
-                const float f = __builtin_amdgcn_exp2f(tops[unit + j * places] - base);
-                sum += sums[threadIdx.x + 32 * places * j] * f;
-                den += dens[unit + j * places] * f;
-            }
-            const float inv = den > 0.0f ? 1.0f / den : 0.0f;
-            *reinterpret_cast<uint2 *>(a.out + (size_t)g * a.ldo + (size_t)(kvh * a.group + block * COLS + c) * HD + 4 * at) =
-                make_uint2(pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv));
-        }
-    }
+k_paged_join(Args a) {
+    const int w = blockIdx.x;
+    const Cut cut = *cut_at(a, w);
+    if (!cut.tiles) return;
+    const Ranges range(cut.total, ranges(cut.total, gridDim.x));
+    const int w0 = range.of(cut.first), sharers = range.of(cut.first + cut.tiles - 1) - w0;
+    join_parts<JOIN, COLS, HD>(
+        (cut.cols - (w - w0) + sharers - 1) / sharers, sharers + 1, [&](int i) { return a.part + (size_t)(2 * (w0 + i) + (i == 0)) * PART; },      /* (perhaps no columns) */
+        [&](int n) { return w - w0 + n * sharers; }, [&](int n) { return a.out + (size_t)cut.g * a.ldo + (size_t)(cut.head + w - w0 + n * sharers) * HD; });
 }
 
 }  // namespace
 
-extern "C" size_t iris_hip_paged_workspace(void) { return (size_t)2 * MOST_WAVES * PART * sizeof(float); }
+extern "C" size_t iris_hip_paged_workspace(void) { return MOST_WAVES * (2 * PART * sizeof(float) + sizeof(Cut)); }
 
 /* 1 where iris_hip_paged_hd128 takes these sizes: row numbers and the number of tiles in 32 bits */
 extern "C" int iris_hip_paged_hd128_takes(int pages, int page_shift, int table_ld, int n, int heads, int kv_heads) {
@@ -580,6 +527,6 @@ extern "C" int iris_hip_paged_hd128(void *stream, float *part, uint16_t *out, in
     };
     if (ks) run_rows(std::true_type{});
     else run_rows(std::false_type{});
-    if (waves > 1) hipLaunchKernelGGL(k_paged_join, dim3(waves), dim3(JOIN), 0, (hipStream_t)stream, a, keys);
+    if (waves > 1) hipLaunchKernelGGL(k_paged_join, dim3(waves), dim3(JOIN), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }

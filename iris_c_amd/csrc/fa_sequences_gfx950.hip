@@ -23,20 +23,24 @@
  * of the last sequence down, so that of each sequence the longest come first (those of all sequences first is no faster), otherwise
  * sequence by sequence from the one with the most keys down.
  *
- * What bounds it: 12001 + 4096 + 700 + 1 causal rows, 32 heads on 8, take 1.28 - 1.36 ms (by box), 0.97 - 1.03 PFLOP/s; pictures of 4608,
+ * What bounds it: 12001 + 4096 + 700 + 1 causal rows, 32 heads on 8, take 1.26 - 1.36 ms, 0.97 - 1.05 PFLOP/s; pictures of 4608,
  * 1536, 2627 and 576 rows, 24 heads, 360 - 390 us (1.05 PFLOP/s). The matrix cores are busy 45 % of the cycles of all SIMDs, no LDS access
  * conflicts, 95 % of the requests of the first are served by the L2s; as in the kernel for one sequence the rest is the softmax's vector
  * instructions (a thousand cycles beside 1088 of products per wave and tile) and what the chip's power leaves of the clock. 24 prompts of 4
  * to 512 rows take 20 us: workgroups of about 4 us of dependent reads (bounds, first tiles) and up to 8 tiles of 1.3 us, two on a CU.
  *
- * Where there are few columns and many keys, `ranges` workgroups share the key tiles of the same columns, evenly: each leaves its
- * unnormalised sums, their maximum and denominator in a workspace, and a second launch joins them: 64 + 1 + 200 + 17 rows over 8294 keys
- * 90 us in one range, 46 in three (6 of them to join), 32 rows over 16000 keys 314 and 53.
+ * Where there are few columns and many keys, the keys of every workgroup's columns are cut into parts, of as many key blocks each as gives about
+ * two workgroups to a CU; the lengths are in device memory, so the kernel itself finds how many (sequences.h). Each part leaves its unnormalised
+ * sums, their maximum and denominator in a workspace, and a second launch joins them, as many workgroups as there are parts, which find what
+ * they join in the workspace too (looked up anew it would take 3 us more): 64 + 1 + 200 + 17 rows over 8294 keys, 32 heads on 8, 95 us whole, 44 cut
+ * (7 of them to join 27 MB); 32 rows over 16000 keys 335 and 32. Equal numbers of parts for all sequences, as many as the host can tell from their
+ * average, leave the longest to be waited for: 46 and 53.
  */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include "iris_kernels_hip.h"
+#include "join_parts.h"
 #include "sequences.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -51,7 +55,7 @@ namespace {
 
 constexpr int HD = 128, KEYS = 64, TILE = KEYS * HD, STAGE = 2 * TILE;      /* elements of K or V; of a stage, 32 KB */
 constexpr float RAISE = 8.0f;
-constexpr int MOST_RANGES = 8;
+constexpr int MOST_PARTS = 512;                                     /* two workgroups on each of 256 CUs */
 
 __device__ __align__(256) const uint16_t zeros[HD] = {};
 
@@ -119,23 +123,24 @@ struct Args {
     const uint16_t *q, *k, *v;
     int ldo, ldq, ldkv, kv_heads;
     SequencesArg seqs;
-    float scale_log2, *part;                     /* part: partial results, ranges > 1 */
-    int ranges;
+    float scale_log2, *part;                     /* part: partial results, where the keys are cut */
 };
 
 /* What a workgroup works on */
-struct Place { bool there; int kvh, tile, range; };
+struct Place { bool there; int kvh, tile; };
 __device__ __forceinline__ Place place(const Args &a, int count, bool last_first) {
     const int together = a.kv_heads % 8 == 0 ? 8 : a.kv_heads;       /* kv heads whose tiles are dealt out in turn */
-    const unsigned round = (unsigned)together * (unsigned)count, number = blockIdx.x / a.ranges;
-    if (round == 0 || number / round >= (unsigned)(a.kv_heads / together)) return {false, 0, 0, 0};
+    const unsigned round = (unsigned)together * (unsigned)count, number = blockIdx.x;
+    if (round == 0 || number / round >= (unsigned)(a.kv_heads / together)) return {false, 0, 0};
     const unsigned rest = number % round;
-    return {true, (int)(number / round) * together + (int)(rest % together), last_first ? count - 1 - (int)(rest / together) : (int)(rest / together), (int)(blockIdx.x % a.ranges)};
+    return {true, (int)(number / round) * together + (int)(rest % together), last_first ? count - 1 - (int)(rest / together) : (int)(rest / together)};
 }
-/* floats of a workgroup's partial result: sums of its columns, their maxima, their denominators */
-constexpr int part_floats(int columns) { return columns * (HD + 2); }
+/* What the second launch finds about a workgroup of the first: part `part` of `parts` of `columns` columns from c0 on; place: of part 0 */
+struct Cut { int parts, part, place, row0, c0, columns, kvh, unused; };
+__device__ __forceinline__ float *part_at(const Args &a, int place) { return a.part + (size_t)place * part_floats(128, HD); }
+__device__ __forceinline__ Cut *cut_at(const Args &a, int wg) { return reinterpret_cast<Cut *>(part_at(a, MOST_PARTS)) + wg; }
 
-template <int WAVES, int NB, bool CAUSAL>
+template <int WAVES, int NB, bool CAUSAL, bool CUT>
 __global__ void __launch_bounds__(64 * WAVES, 2)
 k_sequences_hd128(Args a) {
     extern __shared__ __align__(16) uint16_t lds[];                  /* 2 GROUP stages */
@@ -143,12 +148,18 @@ k_sequences_hd128(Args a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lg = lane >> 4;
     const int group = a.seqs.per_row;
 
-    SequenceTiles<!CAUSAL> tiles;
-    const int count = tiles.count(a.seqs, COLUMNS);
+    SequenceTiles<!CAUSAL && !CUT, CUT> tiles;
+    int count = tiles.count(a.seqs, COLUMNS);
+    if constexpr (CUT) count = tiles.cut(a.kv_heads, MOST_PARTS);
     const Place at = place(a, count, CAUSAL);
-    if (!at.there) return;
+    if (!at.there) {
+        if (CUT && threadIdx.x == 0) cut_at(a, blockIdx.x)->parts = 0;
+        return;
+    }
     const SequenceTile s = tiles.tile(at.tile);
     const int kvh = at.kvh;
+    if (CUT && threadIdx.x == 0)
+        *cut_at(a, blockIdx.x) = Cut{s.parts, s.part, kvh * count + at.tile - s.part, s.row0, s.c0, min(COLUMNS, s.n * group - s.c0), kvh, 0};
 
     /* this lane's columns, one in each block; those behind the sequence's last are computed like it and not stored */
     const int columns = s.n * group, wc0 = s.c0 + wave * 16 * NB, ahead = s.m - s.n;
@@ -162,7 +173,7 @@ k_sequences_hd128(Args a) {
     }
     const int last = min(s.c0 + COLUMNS, columns) - 1, k_end = CAUSAL ? max(last / group + 1 + ahead, 0) : s.m;      /* no column of the workgroup sees more */
     const int all_tiles = (k_end + KEYS - 1) / KEYS;
-    const int tile0 = all_tiles * at.range / a.ranges, ntiles = all_tiles * (at.range + 1) / a.ranges;      /* (at most 8 ranges) */
+    const int each = CUT ? (all_tiles + s.parts - 1) / s.parts : all_tiles, tile0 = CUT ? min(s.part * each, all_tiles) : 0, ntiles = min(tile0 + each, all_tiles);
     const bool busy = wc0 < columns;
     /* the wave's columns see all of the tiles in front of the first limit, and nothing from the last one on */
     const int see_all = CAUSAL ? wc0 / group + 1 + ahead : s.m, see_any = CAUSAL ? min(wc0 + 16 * NB - 1, columns - 1) / group + 1 + ahead : s.m;
@@ -375,11 +386,13 @@ k_sequences_hd128(Args a) {
         }
     }
 
-    if (a.ranges > 1) {
-        float *pp = a.part + (size_t)blockIdx.x * part_floats(COLUMNS);
+    if (CUT && s.parts > 1) {
+        static_assert(!CUT || COLUMNS == 128, "");
+        float *pp = part_at(a, kvh * count + at.tile);
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
             const int c = wave * 16 * NB + 16 * nb + li;
+            if (s.c0 + c >= columns) continue;
 #pragma unroll
             for (int db = 0; db < 8; db++) *reinterpret_cast<f32x4 *>(pp + c * HD + 16 * db + 4 * lg) = o[db][nb];
             if (lg == 0) { pp[COLUMNS * HD + c] = top[nb]; pp[COLUMNS * (HD + 1) + c] = den[nb][0]; }
@@ -398,74 +411,51 @@ k_sequences_hd128(Args a) {
     }
 }
 
-/* The ranges of a workgroup's columns joined: 32 lanes to a column, 4 dims each, all ranges' loads under way together */
-constexpr int JOIN = 1024;
-template <int COLUMNS, bool CAUSAL>
+/* The parts of a workgroup's columns joined, by as many workgroups as there are parts: each takes every parts-th column */
+constexpr int JOIN = 512;
 __global__ void __launch_bounds__(JOIN)
 k_sequences_join(Args a) {
-    SequenceTiles<!CAUSAL> tiles;
-    const int ranges = a.ranges, count = tiles.count(a.seqs, COLUMNS), group = a.seqs.per_row;
-    a.ranges = 1;                                                     /* a workgroup here for all ranges */
-    const Place at = place(a, count, CAUSAL);
-    if (!at.there) return;
-    const SequenceTile s = tiles.tile(at.tile);
-    const int columns = min(COLUMNS, s.n * group - s.c0), lane = threadIdx.x & 31;
-    const float *pp = a.part + (size_t)blockIdx.x * ranges * part_floats(COLUMNS);
-    for (int c = threadIdx.x >> 5; c < columns; c += JOIN / 32) {
-        float t[MOST_RANGES], d[MOST_RANGES], top = -INFINITY, den = 0.0f;
-        f32x4 o[MOST_RANGES], sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < MOST_RANGES; i++) {
-            const float *p = pp + (size_t)min(i, ranges - 1) * part_floats(COLUMNS);
-            t[i] = i < ranges ? p[COLUMNS * HD + c] : -INFINITY;
-            d[i] = p[COLUMNS * (HD + 1) + c];
-            o[i] = *reinterpret_cast<const f32x4 *>(p + c * HD + 4 * lane);
-            top = fmaxf(top, t[i]);
-        }
-        const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int i = 0; i < MOST_RANGES; i++) {
-            if (i >= ranges) break;
-            const float f = __builtin_amdgcn_exp2f(t[i] - base);
-            sum += o[i] * f;
-            den += d[i] * f;
-        }
-        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-        const int row = (s.c0 + c) / group, head = at.kvh * group + (s.c0 + c) - row * group;
-        *reinterpret_cast<uint2 *>(a.out + (size_t)(s.row0 + row) * a.ldo + (size_t)head * HD + 4 * lane) =
-            make_uint2(pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv));
-    }
+    const Cut cut = *cut_at(a, blockIdx.x);
+    if (cut.parts < 2) return;
+    const int group = a.seqs.per_row;
+    join_parts<JOIN, 128, HD>(
+        (cut.columns - cut.part + cut.parts - 1) / cut.parts, cut.parts, [&](int i) { return part_at(a, cut.place + i); },
+        [&](int n) { return cut.part + n * cut.parts; },
+        [&](int n) {
+            const int c = cut.c0 + cut.part + n * cut.parts, row = c / group;
+            return a.out + (size_t)(cut.row0 + row) * a.ldo + (size_t)(cut.kvh * group + c - row * group) * HD;
+        });
 }
 
-template <int WAVES, int NB, bool CAUSAL>
+template <int WAVES, int NB, bool CAUSAL, bool CUT = false>
 int launch(hipStream_t stream, const Args &a) {
     constexpr int LDS = (WAVES * NB >= 16 ? 4 : 2) * STAGE * (int)sizeof(uint16_t);
     static bool configured = false;
     if (!configured) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k_sequences_hd128<WAVES, NB, CAUSAL>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k_sequences_hd128<WAVES, NB, CAUSAL, CUT>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) return (int)e;
         configured = true;
     }
-    const long wgs = sequence_tiles_at_most(a.seqs, 16 * NB * WAVES) * a.kv_heads;
+    const long wgs = CUT ? MOST_PARTS : sequence_tiles_at_most(a.seqs, 16 * NB * WAVES) * a.kv_heads;
     if (!wgs) return 0;
-    if (wgs * a.ranges > ((1L << 32) - 1) / (64 * WAVES)) return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_sequences_hd128<WAVES, NB, CAUSAL>), dim3((unsigned)(wgs * a.ranges)), dim3(64 * WAVES), LDS, stream, a);
-    if constexpr (NB == 1 && WAVES == 4)
-        if (a.ranges > 1) hipLaunchKernelGGL((k_sequences_join<16 * NB * WAVES, CAUSAL>), dim3((unsigned)wgs), dim3(JOIN), 0, stream, a);
+    if (wgs > ((1L << 32) - 1) / (64 * WAVES)) return (int)hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_sequences_hd128<WAVES, NB, CAUSAL, CUT>), dim3((unsigned)wgs), dim3(64 * WAVES), LDS, stream, a);
+    if constexpr (CUT) hipLaunchKernelGGL(k_sequences_join, dim3((unsigned)wgs), dim3(JOIN), 0, stream, a);
     return (int)hipGetLastError();
 }
 
 }  // namespace
 
-/* Which workgroups a call takes: waves x blocks of 16 columns a wave, and in how many ranges the keys of each are cut; host arithmetic only */
-extern "C" void iris_hip_sequences_plan(int n, int rows, int keys, int heads, int kv_heads, int causal, int own_keys, int *waves, int *blocks, int *ranges) {
+/* Which workgroups a call takes: waves x blocks of 16 columns a wave; and whether it cuts their keys where it has a workspace (4 x 2 then), into at
+ * most `parts` for all of them; 1: it does not. Host arithmetic only */
+extern "C" void iris_hip_sequences_plan(int n, int rows, int keys, int heads, int kv_heads, int causal, int own_keys, int *waves, int *blocks, int *parts) {
     const int group = heads / kv_heads;
     const long some = n < rows ? n : rows, blocks16 = ((long)rows * group + some * 8) / 16 * kv_heads, each = (long)rows * group / some;
     /* Measured, us, by waves x blocks (all with 32 query heads on 8 unless noted). Causal: 118 rows 8.0 with 2 x 1, 8.3 with 4 x 1, 9.9 with 8 x 1;
      * 512 rows 17.8 / 16.8 / 18.8, 4 x 2 20.6; 1024 40.6 / 28.1 / 31.1, 4 x 2 34.0; 2048 4 x 1 67.7, 8 x 1 65.1, 4 x 2 62.1, 8 x 2 73.4; 4096 219 / 212 / 161 /
      * 154; 8192 800 / 757 / 546 / 548; 64 prompts of 4 to 512 78.3 / 84.2 / 63.9 / 76.6; 24 heads on 24, 2048 rows 64.3 / 69.9 / 75.5 / 71.6. Not causal, 24 heads on
      * 24: 1280 rows 32.3 / 30.3 / 33.4 / 43.0; 4608 349 / 348 / 277 / 257; 600 + 320 + 900 37.4 / 39.5 / 38.3 / 36.6. */
-    *blocks = *ranges = 1;
+    *blocks = *parts = 1;
     if (causal) {
         *waves = blocks16 <= 640 ? 2 : 4;
         if (blocks16 > 3500) *blocks = 2;
@@ -475,29 +465,29 @@ extern "C" void iris_hip_sequences_plan(int n, int rows, int keys, int heads, in
     }
     while (*waves > 1 && each <= 8 * *waves * *blocks) *waves /= 2;
     if (*blocks == 2 && *waves < 4) { *waves = 2 * *waves; *blocks = 1; }
-    /* Key tiles that a workgroup sees, about, and workgroups of 64 columns: where those leave CUs idle (two have room on one) and walk long. us, 1 / 2 / 3 /
-     * 4 / 6 / 8 ranges: 64 + 1 + 200 + 17 rows over 8294 keys 85 / 57 / 46 / 50 / 51 / 54; 32 over 16000 314 / 167 / 116 / 89 / 65 / 53; 8 x 16 rows over 9464 keys 65 / 43 / 34 / 30 / 26 / 27;
-     * 118 rows over their own 8.3 / 16.6 (a second launch). */
-    const long chain = (long)keys / some / KEYS / (causal && own_keys ? 2 : 1), wgs = (((long)rows * group + some * 32) / 64 + 1) * kv_heads;
-    const long room = (long)(IRIS_LINEAR_PART_BYTES / sizeof(float) / part_floats(64)) / (sequence_tiles_at_most({nullptr, nullptr, n, rows, keys, group}, 64) * kv_heads);
-    if (chain >= 12 && wgs <= 256) {
-        long r = 512 / wgs;
-        if (r > chain / 4) r = chain / 4;
-        if (r > MOST_RANGES) r = MOST_RANGES;
-        if (r > room) r = room;
-        if (r > 1) { *waves = 4; *blocks = 1; *ranges = (int)r; }
-    }
+    /* Whether the key blocks of a workgroup are cut into parts: where few workgroups walk long. tiles: workgroups of 128 columns, chain: key
+     * blocks that one walks, on the average of the sequences. us, whole and cut, causal / not:
+     *     tiles  16, chain  8  15.1 19.2 /  12.8 17.8         16  25.5 17.6 /  21.9 16.6         32  46.1 17.9 / 39.7 16.7
+     *     tiles  95, chain  8  17.1 22.5 /  16.8 21.0         16  28.1 23.7 /  25.9 22.5         32  48.8 31.8 / 45.2 29.9
+     *     tiles 128, chain 16  26.8 27.1 /  20.8 27.7         32  46.7 36.6 /  34.8 36.0         64  85.1 52.8 / 62.1 51.0
+     *     tiles 232, chain 31  46.0 47.3 /  41.5 50.6         93   134  108 /   108  107
+     * Nothing is cut where there might be more than half as many tiles as parts, or more than the 256 sequences that a wave looks at at once. */
+    const long tiles = sequence_tiles_at_most({nullptr, nullptr, n, rows, keys, group}, 128) * kv_heads, chain = (long)keys / some / KEYS / (causal && own_keys ? 2 : 1);
+    static_assert(MOST_PARTS * (part_floats(128, HD) * sizeof(float) + sizeof(Cut)) <= IRIS_LINEAR_PART_BYTES, "");
+    if (n <= 256 && tiles <= MOST_PARTS / 2 && tiles * ((long)keys / KEYS + 1) < 1L << 30 &&
+        (causal ? chain * (400 - tiles) >= 12 * 400 : chain * (256 - tiles) >= 11 * 256))
+        *parts = MOST_PARTS;
 }
 
 /* part: IRIS_LINEAR_PART_BYTES of private workspace, 16-byte aligned, or null: the keys of a workgroup are then not cut */
 extern "C" int iris_hip_sequences_hd128(void *stream, float *part, uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k, const uint16_t *v,
                                         int ldkv, const int *first_row, const int *first_key, int n, int rows, int keys, int heads, int kv_heads, float scale,
                                         int causal) {
-    Args a = {out, q, k, v, ldo, ldq, ldkv, kv_heads, {first_row, first_key, n, rows, keys, heads / kv_heads}, scale * 1.4426950408889634f, part, 1};
+    Args a = {out, q, k, v, ldo, ldq, ldkv, kv_heads, {first_row, first_key, n, rows, keys, heads / kv_heads}, scale * 1.4426950408889634f, part};
     const hipStream_t st = (hipStream_t)stream;
-    int waves, blocks, ranges;
-    iris_hip_sequences_plan(n, rows, keys, heads, kv_heads, causal, first_key == nullptr, &waves, &blocks, &ranges);
-    if (part) a.ranges = ranges;
+    int waves, blocks, parts;
+    iris_hip_sequences_plan(n, rows, keys, heads, kv_heads, causal, first_key == nullptr, &waves, &blocks, &parts);
+    if (part && parts > 1) return causal ? launch<4, 2, true, true>(st, a) : launch<4, 2, false, true>(st, a);
     if (blocks == 2 && waves == 8) return causal ? launch<8, 2, true>(st, a) : launch<8, 2, false>(st, a);
     if (blocks == 2) return causal ? launch<4, 2, true>(st, a) : launch<4, 2, false>(st, a);
     if (waves == 8) return causal ? launch<8, 1, true>(st, a) : launch<8, 1, false>(st, a);

@@ -228,7 +228,7 @@ int iris_hip_sequences_any(void *stream, uint16_t *out, int ldo, const uint16_t 
  * ldkv < 2^27. part: IRIS_LINEAR_PART_BYTES of private workspace, 16-byte aligned, that the stream orders with its other users, or null: the
  * keys of few columns are then not cut into ranges. plan: the workgroups for these sizes, waves x blocks of 16 columns a wave, and the
  * ranges (own_keys: first_key is NULL); host arithmetic only. */
-void iris_hip_sequences_plan(int n, int rows, int keys, int heads, int kv_heads, int causal, int own_keys, int *waves, int *blocks, int *ranges);
+void iris_hip_sequences_plan(int n, int rows, int keys, int heads, int kv_heads, int causal, int own_keys, int *waves, int *blocks, int *parts);
 int iris_hip_sequences_hd128(void *stream, float *part, uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k, const uint16_t *v,
                              int ldkv, const int *first_row, const int *first_key, int n, int rows, int keys, int heads, int kv_heads, float scale,
                              int causal);

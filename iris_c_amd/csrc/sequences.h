@@ -14,8 +14,8 @@
 
 struct SequencesArg { const int *first_row, *first_key; int n, rows, keys, per_row; };       /* the kernels' argument */
 
-/* the tile's columns are c0 .. c0 + height - 1 of the sequence's n * per_row; column c is row row0 + c / per_row */
-struct SequenceTile { int row0, n, c0, key0, m, g; };        /* g: the sequence's number, in order */
+/* the tile's columns are c0 .. c0 + height - 1 of the sequence's n * per_row; column c is row row0 + c / per_row. Cut: part `part` of `parts` */
+struct SequenceTile { int row0, n, c0, key0, m, g, part, parts; };        /* g: the sequence's number, in order */
 
 /* inclusive sum and maximum over the lanes up to each one, in the vector registers (shifts inside rows of 16, then the rows' last
  * lanes to those behind them): a tenth of the time of six trips through the LDS */
@@ -42,14 +42,17 @@ __device__ __forceinline__ int wave_max_upto(int v) {                    /* of v
 }
 
 /* BY_LENGTH: up to 64 sequences in the order of their keys, the most first, for kernels whose tiles take as long as the keys are many: the
- * last workgroups of a call are then short ones. */
-template <bool BY_LENGTH = false>
+ * last workgroups of a call are then short ones. CUT, up to 256 sequences: every tile is in the list as several parts of at most `each` key
+ * blocks of 64, so many that there are about as many entries as wanted, and each about as long as the others. */
+template <bool BY_LENGTH = false, bool CUT = false>
 struct SequenceTiles {
+    static constexpr int LEAST = 4;                                  /* blocks of keys in a part */
     static constexpr int AT_ONCE = 4;                                /* 64 sequences at once: their bounds are one trip to memory */
     SequencesArg a;
     int height;
     int lo[AT_ONCE], hi[AT_ONCE], klo[AT_ONCE], khi[AT_ONCE];        /* this lane's sequences of the last looked at: rows, keys */
     int upto[AT_ONCE], total, most, key_most;    /* tiles of all sequences up to each; of all so far; the largest values in front of those */
+    int each;                                    /* of the cut */
 
     /* first[g] and the next one, each as the largest value up to its place, limited to 0 .. limit */
     static __device__ __forceinline__ void range(int from, int to, int limit, int &most, int &lo, int &hi) {
@@ -105,7 +108,41 @@ struct SequenceTiles {
         for (int base = 0; base < a.n; base += 64 * AT_ONCE) look(base);
         return total;
     }
-    /* tile t of them, t < count() */
+    /* Cuts the tiles of count(), for each of `heads` heads: `each` is the least number of blocks, within an eighth, that makes not more than
+     * most_entries entries for all heads. most_entries is more than there are tiles for them, so that this one does:
+     * entries <= sum of heads (keys / each + 1) over the tiles <= most_entries. */
+    __device__ __forceinline__ int cut(int heads, int most_entries) {
+        int work = 0;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i++)
+            if (64 * i < a.n) work += __builtin_amdgcn_readlane(wave_sum_upto(tiles(i) * blocks(khi[i] - klo[i])), 63);
+        work *= heads;
+        const int more = most_entries - total * heads;
+        int few = max(LEAST, work / most_entries) - 1, many = max(LEAST, (work + more - 1) / more);      /* too few, or not to be tried, and enough */
+        while (many - few > 1 + many / 8) {                              /* at least 2: `each` lies between them, and takes the place of one */
+            each = (few + many) / 2;
+            int entries = 0;
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; i++)
+                if (64 * i < a.n) entries += __builtin_amdgcn_readlane(wave_sum_upto(tiles(i) * parts(khi[i] - klo[i])), 63);
+            if (entries * heads <= most_entries) many = each;
+            else few = each;
+        }
+        each = many;
+        total = 0;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i++) {
+            upto[i] = total;
+            if (64 * i < a.n) {
+                upto[i] += wave_sum_upto(tiles(i) * parts(khi[i] - klo[i]));
+                total = __builtin_amdgcn_readlane(upto[i], 63);
+            }
+        }
+        return total;
+    }
+    static __device__ __forceinline__ int blocks(int keys) { return (keys + 63) / 64; }
+    __device__ __forceinline__ int parts(int keys) const { return max(1, (blocks(keys) + each - 1) / each); }
+    /* tile t of them, t < count(), or entry t < cut() */
     __device__ __forceinline__ SequenceTile tile(int t) {
         int base = 0;
         if (a.n > 64 * AT_ONCE) {
@@ -115,7 +152,7 @@ struct SequenceTiles {
                 if (t < total) break;
             }
         }
-        SequenceTile s = {0, 0, 0, 0, 0, 0};
+        SequenceTile s = {0, 0, 0, 0, 0, 0, 0, 1};
         bool found = false;
 #pragma unroll
         for (int i = 0; i < AT_ONCE; i++) {
@@ -128,7 +165,15 @@ struct SequenceTiles {
                 s.n = __builtin_amdgcn_readlane(hi[i], at) - s.row0;
                 s.key0 = __builtin_amdgcn_readlane(klo[i], at);
                 s.m = __builtin_amdgcn_readlane(khi[i], at) - s.key0;
-                s.c0 = (t - (__builtin_amdgcn_readlane(upto[i], at) - (s.n * a.per_row + height - 1) / height)) * height;
+                const int mine = (s.n * a.per_row + height - 1) / height;
+                if constexpr (CUT) {
+                    s.parts = parts(s.m);
+                    const int entry = t - (__builtin_amdgcn_readlane(upto[i], at) - mine * s.parts), tile = entry / s.parts;
+                    s.part = entry - tile * s.parts;
+                    s.c0 = tile * height;
+                } else {
+                    s.c0 = (t - (__builtin_amdgcn_readlane(upto[i], at) - mine)) * height;
+                }
             }
         }
         return s;

@@ -260,3 +260,63 @@ def test_the_same_bits_every_time_and_from_a_graph(dev):
         assert np.array_equal(dev.get(do, q.shape, np.uint16), want)
     g.rt.hipGraphExecDestroy(captured)
     dev.free_all()
+
+
+def parts(dev, n, rows, keys, heads, kv, causal, own=False):
+    out = [C.c_int() for _ in range(3)]
+    dev.lib.iris_hip_sequences_plan(n, rows, keys, heads, kv, int(causal), int(own), *(C.byref(x) for x in out))
+    return out[2].value
+
+
+def ends(lengths):
+    return [int(x) for x in np.concatenate([[0], np.cumsum(lengths)])]
+
+
+CUT = {
+    "one row": ([1], [20011], 4, 1), "uneven": ([5, 0, 130, 1, 33], [4000, 77, 64, 1, 9000], 6, 3), "fewer keys than rows": ([40, 20], [10, 5000], 8, 8),
+    "no keys": ([3, 9, 4], [0, 3001, 0], 16, 2), "65 sequences": ([1] * 65, [1 + 97 * (i % 41) for i in range(65)], 2, 1), "150 sequences": ([1] * 150, [0] * 90 + [4400] * 60, 1, 1),
+    "several tiles": ([300, 77], [3003, 2100], 5, 1), "ten kv heads": ([17], [2222], 20, 10),
+}
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("case", CUT, ids=str)
+def test_keys_cut_into_parts(dev, case, causal):
+    rows, keys, heads, kv = CUT[case]
+    first, first_key = ends(rows), ends(keys)
+    assert parts(dev, len(rows), first[-1] + 2, first_key[-1] + 9, heads, kv, causal) > 1
+    both(dev, first, first_key, heads, kv, 128, causal, rows=first[-1] + 2, keys=first_key[-1] + 9, kernel="fa_sequences_hd128")
+
+
+def test_own_keys_cut_into_parts(dev):
+    assert parts(dev, 1, 2777, 2777, 1, 1, True, True) > 1
+    both(dev, [5, 2770], None, 1, 1, 128, True, rows=2777, fused=True)
+
+
+def test_infinities_behind_the_limit_where_keys_are_cut(dev):
+    """Each in a dim of its own, near the limits of 90 rows, whose columns and tiles end at several places: infinite for the rows that see it"""
+    n, m, heads = 90, 2300, 2
+    assert parts(dev, 1, n, m, heads, heads, True) > 1
+    q, k, v = make(4, n, m, heads, heads, 128)
+    clean = v.copy()
+    at = [0, 3, 31, 32, 40, 57, 58, 63, 64, 88, 89]
+    for d, i in enumerate(at):
+        for h in range(heads):
+            v[m - n + i, 128 * h + d] = 0xff80 if d % 2 else 0x7f80
+            clean[m - n + i, 128 * h + d] = 0
+    got = run(dev, q, k, v, [0, n], [0, m], heads, heads, 128, 128 ** -0.5, True, kernel="fa_sequences_hd128")
+    want, limit = reference(q, k, clean, [0, n], [0, m], heads, heads, 128, 128 ** -0.5, True, True)
+    have = sr.bf16_value(got).astype(np.float64)
+    for d, i in enumerate(at):
+        for h in range(heads):
+            c = 128 * h + d
+            assert (have[i:, c] == (-np.inf if d % 2 else np.inf)).all() and np.isfinite(have[:i, c]).all(), (i, h)
+            have[i:, c] = want[i:, c] = 0
+    sr.check(have, (want, limit))
+
+
+def test_lists_of_parts_are_read_anew_by_a_call(dev):
+    """A call with many parts, one with few sequences that are cut, one with none: what an earlier one left in the workspace is not read"""
+    for rows, keys in (([1] * 30, [3000] * 30), ([7], [9000]), ([2] * 64, [900] * 63 + [1])):
+        both(dev, ends(rows), ends(keys), 4, 2, 128, True, seed=len(rows))
+    both(dev, [0, 0, 0], [0, 3000, 9000], 4, 2, 128, True, rows=3, keys=9000)

@@ -85,7 +85,7 @@ def test_the_numbers_of_the_tests_against_torch():
     assert (np.abs(got - x) <= np.maximum(np.abs(x) * 2.0 ** -4, scale * 2.0 ** -10)).all()
 
 
-PART = 64 << 20                             # the workspace that the ranges of a call share with the linear layers
+PART = 64 << 20                             # the workspace that the parts of a call share with the linear layers
 
 
 def plan(lib, n, rows, keys, heads, kv, causal, own):
@@ -95,25 +95,47 @@ def plan(lib, n, rows, keys, heads, kv, causal, own):
     return tuple(x.value for x in out)
 
 
-def test_ranges_of_keys_fit_the_workspace(lib):
-    """Any sizes: the shape is one that there is a kernel for, keys are cut with 64 columns to a workgroup only, and what all workgroups that
-    the launch may have leave there fits"""
+def cut(tiles, blocks, heads, most):
+    """What the kernel does with the tiles of sequences of so many blocks of keys: blocks of a part, entries of its list"""
+    parts = lambda each: sum(t * max(1, -(-b // each)) for t, b in zip(tiles, blocks)) * heads
+    work, more = sum(t * b for t, b in zip(tiles, blocks)) * heads, most - sum(tiles) * heads
+    few, many, turns = max(4, work // most) - 1, max(4, (work + more - 1) // more), 0
+    assert more > 0 and work + more < 2 ** 31
+    while many - few > 1 + many // 8:
+        each, turns = (few + many) // 2, turns + 1
+        assert few < each < many and turns < 32
+        if parts(each) <= most:
+            many = each
+        else:
+            few = each
+    return many, parts(many)
+
+
+def test_parts_of_keys_fit_the_workspace(lib):
+    """Any sizes: the shape is one that there is a kernel for, and where keys are cut, the list is not longer than the workspace has places for,
+    whatever the sequences of those sizes are"""
     rng = np.random.default_rng(0)
-    cut = 0
+    known = 0
     for _ in range(20000):
         kv = int(rng.choice([1, 2, 3, 6, 8, 24, 100]))
         heads = kv * int(rng.choice([1, 2, 4, 5, 8, 16, 60]))
         n, rows = int(2 ** rng.uniform(0, 12)), int(2 ** rng.uniform(0, 18))
         own = bool(rng.integers(2))
         keys = rows if own else int(2 ** rng.uniform(0, 24))
-        waves, blocks, ranges = plan(lib, n, rows, keys, heads, kv, int(rng.integers(2)), own)
-        assert (waves, blocks) in {(1, 1), (2, 1), (4, 1), (8, 1), (4, 2), (8, 2)} and 1 <= ranges <= 8
-        if ranges > 1:
-            cut += 1
-            assert (waves, blocks) == (4, 1)
-            tiles = (rows * (heads // kv) + min(n, rows) * 63) // 64 * kv
-            assert tiles * ranges * 64 * 130 * 4 <= PART, (n, rows, keys, heads, kv)
-    assert cut > 1000
+        waves, blocks, parts = plan(lib, n, rows, keys, heads, kv, int(rng.integers(2)), own)
+        assert (waves, blocks) in {(1, 1), (2, 1), (4, 1), (8, 1), (4, 2), (8, 2)} and parts in (1, 512)
+        if parts == 1:
+            continue
+        known += 1
+        assert n <= 256 and parts * (128 * 130 * 4 + 32) <= PART
+        for _ in range(3):
+            ends = np.sort(rng.integers(0, rows + 1, n - 1)) if rng.integers(2) else np.minimum(np.arange(1, n), rows)
+            tiles = [-(-int(r) * (heads // kv) // 128) for r in np.diff(np.concatenate([[0], ends, [rows]]))]
+            k = np.sort(rng.integers(0, keys + 1, n - 1)) if rng.integers(2) else np.full(n - 1, keys * int(rng.integers(2)))
+            m = [-(-int(c) // 64) for c in np.diff(np.concatenate([[0], k, [keys]]))]
+            each, entries = cut(tiles, m, kv, parts)
+            assert each >= 4 and sum(tiles) * kv <= entries <= parts, (n, rows, keys, heads, kv)
+    assert known > 1000
 
 
 def test_shapes_of_known_calls(lib):
@@ -121,7 +143,7 @@ def test_shapes_of_known_calls(lib):
     assert plan(lib, 1, 512, 512, 32, 8, 1, 1) == (4, 1, 1)
     assert plan(lib, 1, 4608, 4608, 24, 24, 0, 1) == (8, 2, 1)
     assert plan(lib, 4, 16797, 16797, 32, 8, 1, 1) == (4, 2, 1)
-    assert plan(lib, 1, 32, 16000, 32, 8, 1, 0) == (4, 1, 8)
+    assert plan(lib, 1, 32, 16000, 32, 8, 1, 0)[2] == 512
     assert plan(lib, 1, 64, 200, 32, 8, 1, 0)[2] == 1
 
 
@@ -131,4 +153,4 @@ def test_sizes_that_the_matrix_core_kernel_has_numbers_for(lib):
     assert takes(2 ** 23, 6, 10, 1, 8, 8) == 0                       # 2^32 rows
     assert takes(2 ** 23 - 1, 6, 10, 1, 8, 8) == 1
     assert takes(10, 6, 2 ** 20, 2048, 32, 32) == 0                  # 2^37 tiles, if all were as long as the table
-    assert lib.iris_dev_attention_paged_workspace() == 2 * 1024 * (16 * 128 + 32) * 4
+    assert lib.iris_dev_attention_paged_workspace() == 1024 * (2 * (16 * 128 + 32) * 4 + 32)
