@@ -32,12 +32,13 @@
  * Where there are few columns and many keys, the keys of every workgroup's columns are cut into parts, of as many key blocks each as gives about
  * two workgroups to a CU; the lengths are in device memory, so the kernel itself finds how many (sequences.h). Each part leaves its unnormalised
  * sums, their maximum and denominator in a workspace, and a second launch joins them, as many workgroups as there are parts, which find what
- * they join in the workspace too (looked up anew it would take 3 us more): 64 + 1 + 200 + 17 rows over 8294 keys, 32 heads on 8, 95 us whole, 44 cut
- * (7 of them to join 27 MB); 32 rows over 16000 keys 335 and 32. Equal numbers of parts for all sequences, as many as the host can tell from their
+ * they join in the workspace too (looked up anew it would take 3 us more): 64 + 1 + 200 + 17 rows over 8294 keys, 32 heads on 8, 67 us whole, 40 cut
+ * (7 of them to join 30 MB); 32 rows over 16000 keys 227 and 31. Equal numbers of parts for all sequences, as many as the host can tell from their
  * average, leave the longest to be waited for: 46 and 53.
  */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "iris_kernels_hip.h"
 #include "join_parts.h"
@@ -126,6 +127,9 @@ struct Args {
     float scale_log2, *part;                     /* part: partial results, where the keys are cut */
 };
 
+/* tiles between two barriers: two where only one workgroup has room on a CU anyway */
+constexpr int group_of(int waves, int blocks) { return waves * blocks >= 16 ? 2 : 1; }
+
 /* What a workgroup works on */
 struct Place { bool there; int kvh, tile; };
 __device__ __forceinline__ Place place(const Args &a, int count, bool last_first) {
@@ -144,7 +148,7 @@ template <int WAVES, int NB, bool CAUSAL, bool CUT>
 __global__ void __launch_bounds__(64 * WAVES, 2)
 k_sequences_hd128(Args a) {
     extern __shared__ __align__(16) uint16_t lds[];                  /* 2 GROUP stages */
-    constexpr int COLUMNS = 16 * NB * WAVES, GROUP = WAVES * NB >= 16 ? 2 : 1;
+    constexpr int COLUMNS = 16 * NB * WAVES, GROUP = group_of(WAVES, NB);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lg = lane >> 4;
     const int group = a.seqs.per_row;
 
@@ -229,7 +233,11 @@ k_sequences_hd128(Args a) {
     wait_loads<0>();
     lds_barrier();
 
-    for (int t0 = tile0, half = 0; t0 < ntiles; t0 += GROUP, half ^= 1) {
+    /* Tiles that all of the wave's columns see as a whole have a loop of their own: in one loop, where they jump over what the others need, 512 rows
+     * take 15.8 us and not 13.2, 12001 + 4096 + 700 + 1 rows 1350 and not 1240 (32 heads on 8). The loops' turns have the same barriers. */
+    const int whole = min(max(see_all, 0) / KEYS, ntiles);
+    int t0 = tile0, half = 0;
+    auto group_of_tiles = [&](auto is_cut) {
 #pragma unroll
         for (int step = 0; step < GROUP; step++) {
             const int k0 = (t0 + step) * KEYS;
@@ -268,7 +276,7 @@ k_sequences_hd128(Args a) {
             if (!work) continue;
 
             /* key k0 + 16 mb + 4 lg + r against column li of block nb */
-            const bool cut = k0 + KEYS > see_all;
+            const bool cut = is_cut && k0 + KEYS > see_all;
             if (cut) {
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++) {
@@ -366,7 +374,11 @@ k_sequences_hd128(Args a) {
         }
         wait_loads<0>();                                              /* the next group has landed, this wave's pieces; behind the barrier everybody's */
         lds_barrier();
-    }
+        t0 += GROUP;
+        half ^= 1;
+    };
+    while (t0 + GROUP <= whole) group_of_tiles(std::false_type{});
+    while (t0 < ntiles) group_of_tiles(std::true_type{});
 
     if (CAUSAL && put_back) {
         /* what was left out of the tiles that a limit passes through, for the columns that see it */
@@ -429,7 +441,7 @@ k_sequences_join(Args a) {
 
 template <int WAVES, int NB, bool CAUSAL, bool CUT = false>
 int launch(hipStream_t stream, const Args &a) {
-    constexpr int LDS = (WAVES * NB >= 16 ? 4 : 2) * STAGE * (int)sizeof(uint16_t);
+    constexpr int LDS = 2 * group_of(WAVES, NB) * STAGE * (int)sizeof(uint16_t);
     static bool configured = false;
     if (!configured) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k_sequences_hd128<WAVES, NB, CAUSAL, CUT>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
@@ -451,32 +463,27 @@ int launch(hipStream_t stream, const Args &a) {
 extern "C" void iris_hip_sequences_plan(int n, int rows, int keys, int heads, int kv_heads, int causal, int own_keys, int *waves, int *blocks, int *parts) {
     const int group = heads / kv_heads;
     const long some = n < rows ? n : rows, blocks16 = ((long)rows * group + some * 8) / 16 * kv_heads, each = (long)rows * group / some;
-    /* Measured, us, by waves x blocks (all with 32 query heads on 8 unless noted). Causal: 118 rows 8.0 with 2 x 1, 8.3 with 4 x 1, 9.9 with 8 x 1;
-     * 512 rows 17.8 / 16.8 / 18.8, 4 x 2 20.6; 1024 40.6 / 28.1 / 31.1, 4 x 2 34.0; 2048 4 x 1 67.7, 8 x 1 65.1, 4 x 2 62.1, 8 x 2 73.4; 4096 219 / 212 / 161 /
-     * 154; 8192 800 / 757 / 546 / 548; 64 prompts of 4 to 512 78.3 / 84.2 / 63.9 / 76.6; 24 heads on 24, 2048 rows 64.3 / 69.9 / 75.5 / 71.6. Not causal, 24 heads on
-     * 24: 1280 rows 32.3 / 30.3 / 33.4 / 43.0; 4608 349 / 348 / 277 / 257; 600 + 320 + 900 37.4 / 39.5 / 38.3 / 36.6. */
-    *blocks = *parts = 1;
-    if (causal) {
-        *waves = blocks16 <= 640 ? 2 : 4;
-        if (blocks16 > 3500) *blocks = 2;
-    } else {
-        *waves = blocks16 <= 640 ? 2 : blocks16 <= 1024 ? 4 : 8;
-        if (blocks16 > 2048) *blocks = 2;
-    }
-    while (*waves > 1 && each <= 8 * *waves * *blocks) *waves /= 2;
-    if (*blocks == 2 && *waves < 4) { *waves = 2 * *waves; *blocks = 1; }
+    /* Measured, us, by waves x blocks, with 32 query heads on 8 unless noted. Causal: 31 rows 5.9 with 2 x 1, 6.4 with 4 x 1; 118 rows 7.4 / 7.5, 8 x 1 9.1, 4 x 2 9.6;
+     * 512 rows 13.6 / 13.0, 4 x 2 17.3; 1000 rows 31.1 / 22.6, 4 x 2 28.0; 24 prompts of 4 to 512 21.8 with 4 x 1, 18.9 with 4 x 2; 61 of 40 rows 21.8 / 20.6; 4608 rows
+     * 231 / 180, 8 x 2 188. Not causal, 4 x 1 / 8 x 1 / 4 x 2 / 8 x 2: 1000 rows 28.4 / 25.4 / 28.7 / -; the 24 prompts 27.8 / 22.8 / 22.5 / 26.2; 11 of 200 rows, 24 heads on 24,
+     * 23.5 / 19.0 / 19.8 / 24.4; 4608 rows so 339 / 299 / 288 / 262. Sequences of few columns leave waves of large workgroups without any: 101 of 16 rows, 24 on 24, 23.3 with
+     * 4 x 1, 25.3 with 8 x 1, 26.7 with 4 x 2; one wave alone is slower for every one of these (its loads wait for each other). */
+    *parts = 1;
+    *waves = causal || blocks16 <= 1024 ? 4 : 8;
+    *blocks = (causal ? blocks16 > 3500 : blocks16 > 2048 && each >= 1024) ? 2 : 1;
+    if (each <= 64) { *waves = 4; *blocks = 1; }
+    if (blocks16 <= 128 && keys / some <= KEYS) { *waves = 2; *blocks = 1; }
     /* Whether the key blocks of a workgroup are cut into parts: where few workgroups walk long. tiles: workgroups of 128 columns, chain: key
      * blocks that one walks, on the average of the sequences. us, whole and cut, causal / not:
-     *     tiles  16, chain  8  15.1 19.2 /  12.8 17.8         16  25.5 17.6 /  21.9 16.6         32  46.1 17.9 / 39.7 16.7
-     *     tiles  95, chain  8  17.1 22.5 /  16.8 21.0         16  28.1 23.7 /  25.9 22.5         32  48.8 31.8 / 45.2 29.9
-     *     tiles 128, chain 16  26.8 27.1 /  20.8 27.7         32  46.7 36.6 /  34.8 36.0         64  85.1 52.8 / 62.1 51.0
-     *     tiles 232, chain 31  46.0 47.3 /  41.5 50.6         93   134  108 /   108  107
-     * Nothing is cut where there might be more than half as many tiles as parts, or more than the 256 sequences that a wave looks at at once. */
+     *     tiles  16, chain  8  12.6 18.9 /  11.6 17.8         16  19.5 17.2 /  18.8 16.3         32  32.9 17.0 / 32.2 16.4
+     *     tiles  64, chain 16  20.2 23.0 /  19.7 23.1         32  34.1 30.0 /  33.2 30.5         64  61.6 38.6 / 60.6 38.6
+     *     tiles 128, chain 16  21.1 26.6 /  20.7 27.5         32  36.2 35.4 /  35.2 36.0         64  65.2 52.0 / 63.0 50.8
+     *     tiles 232, chain 31  40.2 47.1 /  41.1 51.5         93   114  106 /   106  109
+     * and where lengths differ, 96 tiles, chains of 15 to 65, 66.8 39.6. Nothing is cut where there might be more than half as many tiles as
+     * parts, or more than the 256 sequences that a wave looks at at once. */
     const long tiles = sequence_tiles_at_most({nullptr, nullptr, n, rows, keys, group}, 128) * kv_heads, chain = (long)keys / some / KEYS / (causal && own_keys ? 2 : 1);
     static_assert(MOST_PARTS * (part_floats(128, HD) * sizeof(float) + sizeof(Cut)) <= IRIS_LINEAR_PART_BYTES, "");
-    if (n <= 256 && tiles <= MOST_PARTS / 2 && tiles * ((long)keys / KEYS + 1) < 1L << 30 &&
-        (causal ? chain * (400 - tiles) >= 12 * 400 : chain * (256 - tiles) >= 11 * 256))
-        *parts = MOST_PARTS;
+    if (n <= 256 && tiles <= MOST_PARTS / 2 && tiles * ((long)keys / KEYS + 1) < 1L << 30 && chain * (360 - tiles) >= 4800) *parts = MOST_PARTS;
 }
 
 /* part: IRIS_LINEAR_PART_BYTES of private workspace, 16-byte aligned, or null: the keys of a workgroup are then not cut */
@@ -488,10 +495,7 @@ extern "C" int iris_hip_sequences_hd128(void *stream, float *part, uint16_t *out
     int waves, blocks, parts;
     iris_hip_sequences_plan(n, rows, keys, heads, kv_heads, causal, first_key == nullptr, &waves, &blocks, &parts);
     if (part && parts > 1) return causal ? launch<4, 2, true, true>(st, a) : launch<4, 2, false, true>(st, a);
-    if (blocks == 2 && waves == 8) return causal ? launch<8, 2, true>(st, a) : launch<8, 2, false>(st, a);
-    if (blocks == 2) return causal ? launch<4, 2, true>(st, a) : launch<4, 2, false>(st, a);
-    if (waves == 8) return causal ? launch<8, 1, true>(st, a) : launch<8, 1, false>(st, a);
-    if (waves == 4) return causal ? launch<4, 1, true>(st, a) : launch<4, 1, false>(st, a);
-    if (waves == 2) return causal ? launch<2, 1, true>(st, a) : launch<2, 1, false>(st, a);
-    return causal ? launch<1, 1, true>(st, a) : launch<1, 1, false>(st, a);
+    if (causal) return blocks == 2 ? launch<4, 2, true>(st, a) : waves == 4 ? launch<4, 1, true>(st, a) : launch<2, 1, true>(st, a);
+    if (waves == 8) return blocks == 2 ? launch<8, 2, false>(st, a) : launch<8, 1, false>(st, a);
+    return waves == 4 ? launch<4, 1, false>(st, a) : launch<2, 1, false>(st, a);
 }

@@ -108,7 +108,7 @@ struct SequenceTiles {
         for (int base = 0; base < a.n; base += 64 * AT_ONCE) look(base);
         return total;
     }
-    /* Cuts the tiles of count(), for each of `heads` heads: `each` is the least number of blocks, within an eighth, that makes not more than
+    /* Cuts the tiles of count(), for each of `heads` heads: `each` is the least number of blocks, within a 32nd, that makes not more than
      * most_entries entries for all heads. most_entries is more than there are tiles for them, so that this one does:
      * entries <= sum of heads (keys / each + 1) over the tiles <= most_entries. */
     __device__ __forceinline__ int cut(int heads, int most_entries) {
@@ -119,7 +119,7 @@ struct SequenceTiles {
         work *= heads;
         const int more = most_entries - total * heads;
         int few = max(LEAST, work / most_entries) - 1, many = max(LEAST, (work + more - 1) / more);      /* too few, or not to be tried, and enough */
-        while (many - few > 1 + many / 8) {                              /* at least 2: `each` lies between them, and takes the place of one */
+        while (many - few > 1 + many / 32) {                              /* at least 2: `each` lies between them, and takes the place of one */
             each = (few + many) / 2;
             int entries = 0;
 #pragma unroll

@@ -123,7 +123,7 @@ def test_parts_of_keys_fit_the_workspace(lib):
         own = bool(rng.integers(2))
         keys = rows if own else int(2 ** rng.uniform(0, 24))
         waves, blocks, parts = plan(lib, n, rows, keys, heads, kv, int(rng.integers(2)), own)
-        assert (waves, blocks) in {(1, 1), (2, 1), (4, 1), (8, 1), (4, 2), (8, 2)} and parts in (1, 512)
+        assert (waves, blocks) in {(2, 1), (4, 1), (8, 1), (4, 2), (8, 2)} and parts in (1, 512)
         if parts == 1:
             continue
         known += 1
