@@ -21,11 +21,12 @@
 #include "sequences.h"
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 namespace {
 
-constexpr int ROWS = 16, THREADS = 256;                              /* rows of a workgroup; of one in a large call four times as many */
+constexpr int ROWS = 16, THREADS = 256, UNROLL = 4;                  /* rows of a workgroup; four times as many in a large call, a quarter in a small one */
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const f32x2 p = {lo, hi};
@@ -43,10 +44,8 @@ struct ConstPair { const void *k, *v; };
 
 /* head_dim HEAD, rows 16-byte aligned. A unit is 8 values of bf16, 16 of 8 bits (16 bytes of the pages), of consecutive lanes; a thread has
  * the loads of UNROLL units under way together. The places of the rows are looked up once, a row to a thread. magic: 2^32 / kv_heads rounded
- * up, which divides numbers of rows of heads up to ROWS * kv_heads exactly while kv_heads < 8192; 0 for one head.
- * Where a workgroup has no more units than threads (the newest token of each text) UNROLL is 1: 48 rows of 8 heads in bf16 take 3 us and 10
- * with the longer code of UNROLL 4, whose instructions come from memory at each launch. */
-template <int HEAD, bool FP8, bool WRITE, int ROWS, int UNROLL>
+ * up, which divides numbers of rows of heads up to ROWS * kv_heads exactly while kv_heads < 8192; 0 for one head. */
+template <int HEAD, bool FP8, bool WRITE, int ROWS>
 __global__ void __launch_bounds__(THREADS)
 k_cache_rows(Pair pages, Pair scales, ConstPair rows, Pair out, int ld, PagedArg cache, SequencesArg seqs, uint32_t magic) {
     constexpr int VALUES = FP8 ? 16 : 8, LANES = HEAD / VALUES, WORDS = FP8 ? 2 : 1;      /* 16-byte words of bf16 to a unit */
@@ -63,13 +62,14 @@ k_cache_rows(Pair pages, Pair scales, ConstPair rows, Pair out, int ld, PagedArg
     }
     __syncthreads();
     uint8_t *bytes = (uint8_t *)(second ? scales.v : scales.k);
-    uint4 *in_pages = (uint4 *)(second ? pages.v : pages.k);         /* of LANES words to a row */
+    u32x4 *in_pages = (u32x4 *)(second ? pages.v : pages.k);         /* of LANES words to a row */
     const uint16_t *from = (const uint16_t *)(second ? rows.v : rows.k);
     uint16_t *to = (uint16_t *)(second ? out.v : out.k);
     for (int u0 = threadIdx.x; u0 < units; u0 += THREADS * UNROLL) {
         long place[UNROLL];
         size_t at[UNROLL];
-        uint4 x[UNROLL][WORDS], code[UNROLL];
+        u32x4 x[UNROLL][WORDS], code[UNROLL];                        /* of a vector type: arrays of structs go into the LDS, by an address that is
+                                                                      * read from the host's memory: 1690 rows 15 us, with these 4 */
         unsigned byte[UNROLL];
 #pragma unroll
         for (int j = 0; j < UNROLL; j++) {
@@ -81,7 +81,7 @@ k_cache_rows(Pair pages, Pair scales, ConstPair rows, Pair out, int ld, PagedArg
             const long safe = max(place[j], 0L) * LANES + lane;
             if (WRITE) {
 #pragma unroll
-                for (int i = 0; i < WORDS; i++) x[j][i] = *reinterpret_cast<const uint4 *>(from + at[j] + 8 * i);
+                for (int i = 0; i < WORDS; i++) x[j][i] = *reinterpret_cast<const u32x4 *>(from + at[j] + 8 * i);
             } else if (place[j] >= 0) {
                 code[j] = in_pages[safe];
                 if (FP8) byte[j] = bytes[place[j]];
@@ -91,7 +91,8 @@ k_cache_rows(Pair pages, Pair scales, ConstPair rows, Pair out, int ld, PagedArg
         for (int j = 0; j < UNROLL; j++) {
             const int lane = (u0 + j * THREADS) % LANES;
             if constexpr (WRITE && FP8) {
-                unsigned w[8] = {x[j][0].x, x[j][0].y, x[j][0].z, x[j][0].w, x[j][WORDS - 1].x, x[j][WORDS - 1].y, x[j][WORDS - 1].z, x[j][WORDS - 1].w}, top = 0;
+                const unsigned w[8] = {x[j][0][0], x[j][0][1], x[j][0][2], x[j][0][3], x[j][WORDS - 1][0], x[j][WORDS - 1][1], x[j][WORDS - 1][2], x[j][WORDS - 1][3]};
+                unsigned top = 0;
 #pragma unroll
                 for (int i = 0; i < 8; i++) top = max(top, max(w[i] & 0x7fff, (w[i] >> 16) & 0x7fff));
 #pragma unroll
@@ -104,7 +105,7 @@ k_cache_rows(Pair pages, Pair scales, ConstPair rows, Pair out, int ld, PagedArg
                     const float lo = __uint_as_float(w[i] << 16) * factor, hi = __uint_as_float(w[i] & 0xffff0000u) * factor;
                     c[i / 2] = i % 2 ? __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, c[i / 2], true) : __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, c[i / 2], false);
                 }
-                code[j] = byte[j] == 255 ? make_uint4(0x7f7f7f7f, 0x7f7f7f7f, 0x7f7f7f7f, 0x7f7f7f7f) : make_uint4(c[0], c[1], c[2], c[3]);
+                code[j] = byte[j] == 255 ? u32x4{0x7f7f7f7f, 0x7f7f7f7f, 0x7f7f7f7f, 0x7f7f7f7f} : u32x4{(unsigned)c[0], (unsigned)c[1], (unsigned)c[2], (unsigned)c[3]};
             }
             if (place[j] < 0) continue;
             if constexpr (WRITE) {
@@ -112,17 +113,17 @@ k_cache_rows(Pair pages, Pair scales, ConstPair rows, Pair out, int ld, PagedArg
                 if (FP8 && lane == 0) bytes[place[j]] = (uint8_t)byte[j];
             } else if constexpr (FP8) {
                 const float scale = paged_scale(byte[j]);
-                const unsigned c[4] = {code[j].x, code[j].y, code[j].z, code[j].w};
+                const u32x4 c = code[j];
                 uint32_t w[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const f32x2 f = i % 2 ? __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i / 2], true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i / 2], false);
                     w[i] = pack_bf16(f[0] * scale, f[1] * scale);
                 }
-                *reinterpret_cast<uint4 *>(to + at[j]) = make_uint4(w[0], w[1], w[2], w[3]);
-                *reinterpret_cast<uint4 *>(to + at[j] + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                *reinterpret_cast<u32x4 *>(to + at[j]) = u32x4{w[0], w[1], w[2], w[3]};
+                *reinterpret_cast<u32x4 *>(to + at[j] + 8) = u32x4{w[4], w[5], w[6], w[7]};
             } else {
-                *reinterpret_cast<uint4 *>(to + at[j]) = code[j];
+                *reinterpret_cast<u32x4 *>(to + at[j]) = code[j];
             }
         }
     }
@@ -180,17 +181,19 @@ int launch(hipStream_t stream, Pair pages, Pair scales, ConstPair rows, Pair out
     /* many rows (95547 of 8 heads in 8 bits read back 162 us with 16 rows a workgroup, 147 with 64); or rows of few bytes, of which 16 are
      * little work for what finding them takes (2600 of one head written and 44000 read back, 149 texts: 26 and 24) */
     const bool large = wide && ((long)seqs.rows * c.kv_heads >= 1 << 16 || ((long)c.kv_heads * c.head_dim <= 512 && seqs.rows >= 1 << 14 && seqs.rows / 32 >= seqs.n));
-    const bool few = (long)seqs.rows * c.kv_heads * c.head_dim <= (long)seqs.n * THREADS * (FP8 ? 16 : 8);
-    const long wgs = 2 * sequence_tiles_at_most(seqs, large ? 4 * ROWS : ROWS);
+    /* few rows: with 16 to a workgroup most CUs would have none (300 rows of 24 heads in 8 bits written 8.0 us, 5.0 with 4; 3219 rows of 8 heads, which
+     * leave none without, 5.7 and 7.7), or single rows */
+    const bool small = wide && !large && (sequence_tiles_at_most(seqs, ROWS) <= 128 || seqs.rows / 4 <= seqs.n);
+    const long wgs = 2 * sequence_tiles_at_most(seqs, large ? 4 * ROWS : small ? ROWS / 4 : ROWS);
     if (!wgs) return 0;
     if (wgs > ((1L << 32) - 1) / THREADS) return (int)hipErrorInvalidValue;
     const dim3 grid((unsigned)wgs), block(THREADS);
     const uint32_t magic = c.kv_heads > 1 ? (uint32_t)(((1ull << 32) + c.kv_heads - 1) / c.kv_heads) : 0;
     auto rows_of = [&](auto head) {
         constexpr int HEAD = decltype(head)::value;
-        if (large) hipLaunchKernelGGL((k_cache_rows<HEAD, FP8, WRITE, 4 * ROWS, 4>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs, magic);
-        else if (few) hipLaunchKernelGGL((k_cache_rows<HEAD, FP8, WRITE, ROWS, 1>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs, magic);
-        else hipLaunchKernelGGL((k_cache_rows<HEAD, FP8, WRITE, ROWS, 4>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs, magic);
+        if (large) hipLaunchKernelGGL((k_cache_rows<HEAD, FP8, WRITE, 4 * ROWS>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs, magic);
+        else if (small) hipLaunchKernelGGL((k_cache_rows<HEAD, FP8, WRITE, ROWS / 4>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs, magic);
+        else hipLaunchKernelGGL((k_cache_rows<HEAD, FP8, WRITE, ROWS>), grid, block, 0, stream, pages, scales, rows, out, ld, c, seqs, magic);
     };
     if (wide && c.head_dim == 128) rows_of(std::integral_constant<int, 128>{});
     else if (wide && c.head_dim == 64) rows_of(std::integral_constant<int, 64>{});
