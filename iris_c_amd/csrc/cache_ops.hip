@@ -9,8 +9,8 @@
  *
  * The rows of a call are the last ones of their sequences: row i of n is position length - n + i. A workgroup takes ROWS rows of one
  * sequence, of K or of V. Bound by memory: each value is read and written once. 95547 rows of 8 heads x 128 read back from 8 bits (587 MB)
- * take 146 us, 4.0 TB/s, two thirds of it written (a copy reaches 4.9); 5131 rows written in 8 bits 6.4 us and read back 7.1 (16 MB each);
- * 48 rows 2.9 us, a launch and four dependent reads (bounds, length, page, row).
+ * take 125 us, 4.7 TB/s, two thirds of it written (a copy reaches 4.9); 5131 rows written in 8 bits 6.3 us and read back 7.1 (16 MB each);
+ * 48 rows 3 us, a launch and four dependent reads (bounds, length, page, row).
  */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -178,12 +178,14 @@ template <bool FP8, bool WRITE>
 int launch(hipStream_t stream, Pair pages, Pair scales, ConstPair rows, Pair out, int ld, const PagedArg &c, const SequencesArg &seqs) {
     const bool wide = ld % 8 == 0 && aligned(WRITE ? rows.k : out.k, 16) && aligned(WRITE ? rows.v : out.v, 16) && aligned(pages.k, 16) &&
                       aligned(pages.v, 16) && (c.head_dim == 128 || c.head_dim == 64 || c.head_dim == 256) && c.kv_heads < 8192;
-    /* many rows (95547 of 8 heads in 8 bits read back 162 us with 16 rows a workgroup, 147 with 64); or rows of few bytes, of which 16 are
-     * little work for what finding them takes (2600 of one head written and 44000 read back, 149 texts: 26 and 24) */
-    const bool large = wide && ((long)seqs.rows * c.kv_heads >= 1 << 16 || ((long)c.kv_heads * c.head_dim <= 512 && seqs.rows >= 1 << 14 && seqs.rows / 32 >= seqs.n));
-    /* few rows: with 16 to a workgroup most CUs would have none (300 rows of 24 heads in 8 bits written 8.0 us, 5.0 with 4; 3219 rows of 8 heads, which
-     * leave none without, 5.7 and 7.7), or single rows */
-    const bool small = wide && !large && (sequence_tiles_at_most(seqs, ROWS) <= 128 || seqs.rows / 4 <= seqs.n);
+    const long bytes = (long)c.kv_heads * c.head_dim * (FP8 ? 1 : 2);                     /* of a row in the pages */
+    /* many rows of few bytes, of which 16 are little work for what finding them takes: 100000 of one head in 8 bits written in 25 us, with 64 to a workgroup
+     * 15; of 8 heads 118 and 128, and read back 132 and 153 */
+    const bool large = wide && bytes <= 256 && seqs.rows >= 1 << 14 && seqs.rows / 32 >= seqs.n;
+    /* 4 to a workgroup: few rows, of which 16 would leave most CUs without any (300 rows of 24 heads in 8 bits written 8.0 us, with 4 5.0; but 3219 of 8
+     * heads 5.7 and 7.7), single ones, and rows of many bytes (30000 of 24 heads in 8 bits 112 and 105, read back 145 and 128; 100000 of 8 in bf16 156 and
+     * 140; but in 8 bits 118 and 148) */
+    const bool small = wide && !large && (sequence_tiles_at_most(seqs, ROWS) <= 128 || seqs.rows / 4 <= seqs.n || bytes >= 2048);
     const long wgs = 2 * sequence_tiles_at_most(seqs, large ? 4 * ROWS : small ? ROWS / 4 : ROWS);
     if (!wgs) return 0;
     if (wgs > ((1L << 32) - 1) / THREADS) return (int)hipErrorInvalidValue;
