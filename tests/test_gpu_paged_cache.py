@@ -222,6 +222,21 @@ def test_strides_and_alignments(dev, pad, offset, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("lengths,kv,hd", [([17001, 30], 1, 128), ([9, 16500], 2, 64), ([2500, 0, 33, 900], 6, 64), ([2100, 40], 3, 128), ([700, 1, 1200], 24, 128),
+                                           ([300], 24, 128), ([1500, 801], 5, 256), ([1] * 500, 2, 128)], ids=str)
+def test_any_number_of_rows(dev, lengths, kv, hd, kind):
+    c = filled(dev, kind, lengths, 32, kv, hd, extra_columns=1)
+    c.check()
+    first = np.concatenate([[0], np.cumsum(lengths)])
+    c.read(lengths, first[-1] + 1, first)
+    new = np.minimum(lengths, 77)
+    c.write(lengths, rows(9, new.sum(), kv * hd), rows(10, new.sum(), kv * hd), np.concatenate([[0], np.cumsum(new)]))
+    c.check()
+    c.read(lengths, first[-1], first)
+    dev.free_all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_token_by_token(dev, kind):
     """The newest token of each sequence, first_row NULL: as many calls as tokens give the cache that one call gives"""
     kv, hd, heads, page = 2, 128, 4, 4
