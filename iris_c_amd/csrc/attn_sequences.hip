@@ -9,7 +9,7 @@
  * sequence and walks its keys 64 at a time with a running maximum and sum, all in f32: first a key to a lane (its row dotted with every
  * column's query), then an output dim to a lane. A key that a column does not see is passed over and not multiplied by zero, whatever
  * its row holds. head_dim beyond 512 walks the keys once for each 512 output dims. Bound by the uncoalesced reads of K: 512 causal rows
- * of 64 dims, 32 heads on 8, take 317 us, and one token of each of 48 texts of 1024 721 us; the matrix-core kernels on 128 dims 17 and 39.
+ * of 64 dims, 32 heads on 8, take 317 us, and one token of each of 48 texts of 1024 721 us; the matrix-core kernels on 128 dims 15 and 39.
  */
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -9,7 +9,7 @@
  *
  * The rows of a call are the last ones of their sequences: row i of n is position length - n + i. A workgroup takes ROWS rows of one
  * sequence, of K or of V. Bound by memory: each value is read and written once. 95547 rows of 8 heads x 128 read back from 8 bits (587 MB)
- * take 125 us, 4.7 TB/s, two thirds of it written (a copy reaches 4.9); 5131 rows written in 8 bits 6.3 us and read back 7.1 (16 MB each);
+ * take 125 us, 4.7 TB/s, two thirds of it written (a copy reaches 4.9); 2692 rows written in 8 bits 6.2 us and read back 7.0 (16 MB each);
  * 48 rows 3 us, a launch and four dependent reads (bounds, length, page, row).
  */
 #include <hip/hip_runtime.h>

@@ -11,7 +11,8 @@
  * head, block of 16 by block). It is cut into as many equal ranges as there are waves, wherever that falls: the balance does not depend
  * on how long the sequences are, which the host does not know. A wave finds its range from the lengths (64 sequences at a time, one to a
  * lane). A list entry that lies in one range as a whole is finished there; of one that is cut, each part leaves its unnormalised sums
- * and their maximum in the workspace and a second launch joins them. A range cuts its first and its last entry at most: two places each.
+ * and their maximum in the workspace and a second launch joins them. It finds what a range's end cuts in the workspace too, written while the range's wave waits for its
+ * first pages: looked up from the lengths again the second launch takes 1 to 2 us more. A range cuts its first and its last entry at most: two places each.
  *
  * In a tile S^T = K Q^T (A = K, a key a row; B = Q, a query head a column, 16 of them, zeros behind the last) and O^T += V^T P^T
  * (A = V^T from the transposing LDS read), so that a lane holds one query's scores for 4 keys of every 16, and P^T in bf16 is the
@@ -20,10 +21,10 @@
  * 128 dims: Q is cut into two parts of 4 bits, which together hold its 8 (to 2^-18 of its largest value). Values in 8 bits become bf16,
  * which holds them exactly, behind the LDS reads, and their scales multiply the probabilities.
  *
- * What bounds it: memory in long texts: 131072 + 70001 + 4097 tokens of 8 kv heads in 8 bits (424 MB) take 79 us, 5.4 TB/s, and 7 to join;
- * 64 texts of 4096 in bf16 (1.07 GB) 191 us, 5.6 TB/s (both with the join). In short ones the instructions around a list entry, some 2 us
- * of a wave that is alone on its SIMD (two waves of half the tile are no faster): 256 texts of up to 2048 in 8 bits (157 MB) 44 us + 6. Calls of one text are a
- * chain of launches and dependent reads (lengths, pages, tiles): 300 tokens 5 us + 4.
+ * What bounds it: memory in long texts: 131072 + 70001 + 4097 tokens of 8 kv heads in 8 bits (424 MB) take 79 us, 5.4 TB/s, and 6 to join;
+ * 64 texts of 4096 in bf16 (1.07 GB) 189 us, 5.7 TB/s (with the join). In short ones the instructions around a list entry, some 2 us
+ * of a wave that is alone on its SIMD (two waves of half the tile are no faster): 256 texts of up to 2048 in 8 bits (157 MB) 44 us + 5. Calls of one text are a
+ * chain of launches and dependent reads (lengths, pages, tiles): 300 tokens 5.5 us + 4.
  *
  * LDS: the 16-byte piece c of row r is kept in place c ^ swizzle(r) of its row (the loads' source addresses are permuted), so that
  * neither the K reads (16 rows at a time) nor the transposing reads (8 rows) meet in a bank: rows of 256 bytes 2 (r % 8), rows of 128

@@ -134,13 +134,14 @@ class Cache:
         assert (got[:, cols:] == 0x4321).all()
         got = got[:, :cols]
         if compare:
+            values = self.values()
             for g in range(n):
-                sr.check(sr.bf16_value(got[g]).astype(np.float64).reshape(1, heads, self.hd), self.expected(lengths, g, q[g], heads, scale), f"sequence {g}")
+                sr.check(sr.bf16_value(got[g]).astype(np.float64).reshape(1, heads, self.hd), self.expected(lengths, g, q[g], heads, scale, values), f"sequence {g}")
         return got
 
-    def expected(self, lengths, g, q, heads, scale):
+    def expected(self, lengths, g, q, heads, scale, values=None):
         at = [p for p in (self.place(g, i) for i in range(self.length(lengths, g))) if p]
-        kf, vf = self.values()
+        kf, vf = values or self.values()
         k = np.array([kf[page, :, i] for page, i in at]).reshape(len(at), self.kv, self.hd)
         v = np.array([vf[page, :, i] for page, i in at]).reshape(len(at), self.kv, self.hd)
         o, w, s = sr.softmax_rows(sr.bf16_value(q).astype(np.float64).reshape(1, heads, self.hd), k, v, scale, [len(at)])
@@ -233,6 +234,17 @@ def test_any_number_of_rows(dev, lengths, kv, hd, kind):
     c.write(lengths, rows(9, new.sum(), kv * hd), rows(10, new.sum(), kv * hd), np.concatenate([[0], np.cumsum(new)]))
     c.check()
     c.read(lengths, first[-1], first)
+    dev.free_all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_more_sequences_than_a_wave_looks_at_in_one_go(dev, kind):
+    """Empty, short and long ones on both sides of number 256 and 512, among them some that ranges cut several times"""
+    lengths = [(13 * i) % 29 for i in range(600)]
+    for g, n in ((3, 2500), (255, 1700), (256, 0), (257, 3100), (511, 900), (599, 2000)):
+        lengths[g] = n
+    c = filled(dev, kind, lengths, 16, 1, 128)
+    c.attend(lengths, rows(11, 600, 3 * 128), 3, 128 ** -0.5, kernel="fa_paged_hd128")
     dev.free_all()
 
 
