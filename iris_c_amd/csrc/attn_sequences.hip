@@ -13,20 +13,38 @@
  */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "iris_kernels_hip.h"
 #include "paged_cache.h"
 #include "sequences.h"
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 namespace {
 
-constexpr int QB = 8, KT = 64, DIMS = 512, SLOTS = DIMS / 64;
+constexpr int QB = 8, KT = 64, MOST_DIMS = 512, VEC = 8;
 
 __device__ __forceinline__ float value(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 __device__ __forceinline__ float value(uint8_t v) { return __builtin_amdgcn_cvt_f32_fp8(v, 0); }
+/* eight values from a place that is aligned to their size */
+__device__ __forceinline__ void eight(const uint16_t *p, float (&v)[VEC]) {
+    const u32x4 w = *reinterpret_cast<const u32x4 *>(p);
+#pragma unroll
+    for (int i = 0; i < VEC / 2; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ void eight(const uint8_t *p, float (&v)[VEC]) {
+    const u32x2 w = *reinterpret_cast<const u32x2 *>(p);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
+        v[4 * i] = lo[0]; v[4 * i + 1] = lo[1]; v[4 * i + 2] = hi[0]; v[4 * i + 3] = hi[1];
+    }
+}
 __device__ __forceinline__ uint16_t to_bf16(float f) {
     const f32x2 p = {f, 0.0f};
     return (uint16_t)__builtin_bit_cast(uint32_t, __builtin_convertvector(p, bf16x2));
@@ -63,11 +81,17 @@ template <typename V> struct PageKeys {
     __device__ float scale(const uint8_t *s, long offset) const { return s ? paged_scale(s[offset / c.head_dim]) : 1.0f; }
 };
 
-/* nq columns whose queries are q + qat[c]; limit(c): the keys that column c sees are [0, limit(c)); outputs to out + oat[c] */
-template <class Keys, class Q, class Out, class Limit>
-__device__ __forceinline__ void walk(const Keys &keys, int nq, int m, int hd, float scale, const uint16_t *q, Q qat, uint16_t *out, Out oat, Limit limit) {
-    __shared__ float ps[QB][KT];
-    const int lane = threadIdx.x;
+/* nq columns whose queries are q + qat[c]; limit(c): the keys that column c sees are [0, limit(c)); outputs to out + oat[c]. wide: head_dim is a
+ * multiple of 8 and rows of keys are aligned to 8 values */
+template <int SLOTS, class Keys, class Q, class Out, class Limit>
+__device__ __forceinline__ void walk(const Keys &keys, int nq, int m, int hd, float scale, bool wide, const uint16_t *q, Q qat, uint16_t *out, Out oat, Limit limit) {
+    __shared__ __align__(16) float ps[QB][KT];
+    extern __shared__ __align__(16) float qs[];                      /* [QB][head_dim], the first DIMS dims */
+    constexpr int DIMS = 64 * SLOTS;
+    const int lane = threadIdx.x, staged = min(hd, DIMS);
+    for (int c = 0; c < QB; c++)
+        for (int d = lane; d < staged; d += 64) qs[c * staged + d] = value(q[qat(min(c, nq - 1)) + d]);
+    __syncthreads();
     for (int oc = 0; oc < hd; oc += DIMS) {
         float acc[QB][SLOTS], top[QB], sum[QB];
 #pragma unroll
@@ -85,10 +109,20 @@ __device__ __forceinline__ void walk(const Keys &keys, int nq, int m, int hd, fl
 #pragma unroll
             for (int c = 0; c < QB; c++) dot[c] = 0.0f;
             if (at >= 0) {
-                for (int d = 0; d < hd; d++) {
+                int d = 0;
+                if (wide)
+                    for (; d < staged; d += VEC) {
+                        float kd[VEC];
+                        eight(keys.k + at + d, kd);
+#pragma unroll
+                        for (int c = 0; c < QB; c++)
+#pragma unroll
+                            for (int i = 0; i < VEC; i++) dot[c] = fmaf(qs[c * staged + d + i], kd[i], dot[c]);
+                    }
+                for (; d < hd; d++) {
                     const float kd = value(keys.k[at + d]);
 #pragma unroll
-                    for (int c = 0; c < QB; c++) dot[c] = fmaf(value(q[qat(min(c, nq - 1)) + d]), kd, dot[c]);
+                    for (int c = 0; c < QB; c++) dot[c] = fmaf(d < staged ? qs[c * staged + d] : value(q[qat(min(c, nq - 1)) + d]), kd, dot[c]);
                 }
             }
             const float ks = (at >= 0 ? keys.scale(keys.ks, at) : 1.0f) * scale, vs = at >= 0 ? keys.scale(keys.vs, at) : 1.0f;
@@ -106,21 +140,30 @@ __device__ __forceinline__ void walk(const Keys &keys, int nq, int m, int hd, fl
                 ps[c][lane] = sees ? p * vs : -1.0f;            /* -1: not seen (p * vs is never negative) */
             }
             __syncthreads();
-            /* a whole tile's rows one after the other: lane t of the wave knows where row t is */
+            /* the rows of V, eight under way together: lane t of the wave knows where row t is; one that is not there is read as another, and not seen */
+            const unsigned long long any = __ballot(at >= 0);
+            const long some = any ? __shfl(at, __ffsll(any) - 1, 64) : 0;
+#pragma unroll
             for (int t = 0; t < SLOTS; t++) {
-                const int d = oc + lane + 64 * t;
-                if (oc + 64 * t >= hd) break;
+                const int d = oc + lane + 64 * t, dim = min(d, hd - 1);
+                if (!any || oc + 64 * t >= hd) continue;
 #pragma unroll
                 for (int c = 0; c < QB; c++) acc[c][t] *= alpha[c];
-                for (int i = 0; i < nk; i++) {
-                    const long row = __shfl(at, i, 64);
-                    if (row < 0) continue;
-                    const float vd = d < hd ? value(keys.v[row + d]) : 0.0f;
+                for (int i0 = 0; i0 < nk; i0 += VEC) {
+                    typename Keys::T raw[VEC];
 #pragma unroll
-                    for (int c = 0; c < QB; c++) {
-                        const float p = ps[c][i];
-                        acc[c][t] = p < 0.0f ? acc[c][t] : fmaf(p, vd, acc[c][t]);
+                    for (int i = 0; i < VEC; i++) {
+                        const long row = __shfl(at, i0 + i, 64);
+                        raw[i] = keys.v[(row < 0 ? some : row) + dim];
                     }
+#pragma unroll
+                    for (int c = 0; c < QB; c++)
+#pragma unroll
+                        for (int i = 0; i < VEC; i += 4) {
+                            const f32x4 p = *reinterpret_cast<const f32x4 *>(&ps[c][i0 + i]);
+#pragma unroll
+                            for (int j = 0; j < 4; j++) acc[c][t] = p[j] < 0.0f ? acc[c][t] : fmaf(p[j], value(raw[i + j]), acc[c][t]);
+                        }
                 }
             }
         }
@@ -137,9 +180,10 @@ __device__ __forceinline__ void walk(const Keys &keys, int nq, int m, int hd, fl
     }
 }
 
+template <int SLOTS>
 __global__ void __launch_bounds__(64)
 k_sequences_any(uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k, const uint16_t *v, int ldkv, SequencesArg seqs,
-                int kv_heads, int hd, float scale, int causal) {
+                int kv_heads, int hd, float scale, int wide, int causal) {
     SequenceTiles<> tiles;
     const int count = tiles.count(seqs, QB), t = blockIdx.x / kv_heads, kvh = blockIdx.x % kv_heads, group = seqs.per_row;
     if (t >= count) return;
@@ -147,21 +191,30 @@ k_sequences_any(uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16
     const int nq = min(QB, s.n * group - s.c0);
     const RowKeys keys = {k, v, (size_t)ldkv, s.key0, kvh * hd, nullptr, nullptr};
     auto place = [&](int c, int ld) { return (size_t)(s.row0 + (s.c0 + c) / group) * ld + (size_t)(kvh * group + (s.c0 + c) % group) * hd; };
-    walk(keys, nq, s.m, hd, scale, q, [&](int c) { return place(c, ldq); }, out, [&](int c) { return place(c, ldo); },
+    walk<SLOTS>(keys, nq, s.m, hd, scale, wide, q, [&](int c) { return place(c, ldq); }, out, [&](int c) { return place(c, ldo); },
          [&](int c) { return causal ? (s.c0 + c) / group + 1 + s.m - s.n : s.m; });
 }
 
-template <typename T>
+template <typename T, int SLOTS>
 __global__ void __launch_bounds__(64)
 k_paged_any(uint16_t *out, int ldo, const uint16_t *q, int ldq, const T *k, const T *v, const uint8_t *ks, const uint8_t *vs, PagedArg cache,
-            int group, float scale) {
+            int group, float scale, int wide) {
     const int blocks = (group + QB - 1) / QB, c0 = blockIdx.x % blocks * QB, kvh = blockIdx.x / blocks % cache.kv_heads;
     const int g = blockIdx.x / blocks / cache.kv_heads, nq = min(QB, group - c0), hd = cache.head_dim, m = paged_length(cache, g);
     const PageKeys<T> keys = {k, v, ks, vs, cache, g, kvh};
     auto place = [&](int c, int ld) { return (size_t)g * ld + (size_t)(kvh * group + c0 + c) * hd; };
-    walk(keys, nq, m, hd, scale, q, [&](int c) { return place(c, ldq); }, out, [&](int c) { return place(c, ldo); }, [&](int) { return m; });
+    walk<SLOTS>(keys, nq, m, hd, scale, wide, q, [&](int c) { return place(c, ldq); }, out, [&](int c) { return place(c, ldo); }, [&](int) { return m; });
 }
 
+bool aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+size_t staged_bytes(int head_dim) { return (size_t)QB * (head_dim < MOST_DIMS ? head_dim : MOST_DIMS) * sizeof(float); }
+/* f with the output dims of a lane: as many as the head has, at most 8 */
+template <class F> void with_slots(int head_dim, F f) {
+    if (head_dim <= 64) f(std::integral_constant<int, 1>{});
+    else if (head_dim <= 128) f(std::integral_constant<int, 2>{});
+    else if (head_dim <= 256) f(std::integral_constant<int, 4>{});
+    else f(std::integral_constant<int, MOST_DIMS / 64>{});
+}
 bool fits(long wgs) { return wgs <= ((1L << 32) - 1) / 64; }
 
 }  // namespace
@@ -173,8 +226,10 @@ extern "C" int iris_hip_sequences_any(void *stream, uint16_t *out, int ldo, cons
     const long wgs = sequence_tiles_at_most(a, QB) * kv_heads;
     if (!wgs) return 0;
     if (!fits(wgs)) return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL(k_sequences_any, dim3((unsigned)wgs), dim3(64), 0, (hipStream_t)stream, out, ldo, q, ldq, k, v, ldkv, a, kv_heads,
-                       head_dim, scale, causal);
+    with_slots(head_dim, [&](auto slots) {
+        hipLaunchKernelGGL(k_sequences_any<decltype(slots)::value>, dim3((unsigned)wgs), dim3(64), staged_bytes(head_dim), (hipStream_t)stream, out, ldo, q, ldq,
+                           k, v, ldkv, a, kv_heads, head_dim, scale, head_dim % VEC == 0 && ldkv % VEC == 0 && aligned(k, 2 * VEC), causal);
+    });
     return (int)hipGetLastError();
 }
 
@@ -185,11 +240,14 @@ extern "C" int iris_hip_paged_any(void *stream, uint16_t *out, int ldo, const ui
     const int group = heads / kv_heads;
     const long wgs = (long)n * kv_heads * ((group + QB - 1) / QB);
     if (!fits(wgs)) return (int)hipErrorInvalidValue;
-    if (ks)
-        hipLaunchKernelGGL(k_paged_any<uint8_t>, dim3((unsigned)wgs), dim3(64), 0, (hipStream_t)stream, out, ldo, q, ldq, (const uint8_t *)k,
-                           (const uint8_t *)v, ks, vs, c, group, scale);
-    else
-        hipLaunchKernelGGL(k_paged_any<uint16_t>, dim3((unsigned)wgs), dim3(64), 0, (hipStream_t)stream, out, ldo, q, ldq, (const uint16_t *)k,
-                           (const uint16_t *)v, nullptr, nullptr, c, group, scale);
+    with_slots(head_dim, [&](auto slots) {
+        constexpr int SLOTS = decltype(slots)::value;
+        if (ks)
+            hipLaunchKernelGGL((k_paged_any<uint8_t, SLOTS>), dim3((unsigned)wgs), dim3(64), staged_bytes(head_dim), (hipStream_t)stream, out, ldo, q, ldq,
+                               (const uint8_t *)k, (const uint8_t *)v, ks, vs, c, group, scale, head_dim % VEC == 0 && aligned(k, VEC));
+        else
+            hipLaunchKernelGGL((k_paged_any<uint16_t, SLOTS>), dim3((unsigned)wgs), dim3(64), staged_bytes(head_dim), (hipStream_t)stream, out, ldo, q, ldq,
+                               (const uint16_t *)k, (const uint16_t *)v, nullptr, nullptr, c, group, scale, head_dim % VEC == 0 && aligned(k, 2 * VEC));
+    });
     return (int)hipGetLastError();
 }
