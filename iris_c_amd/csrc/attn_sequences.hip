@@ -5,11 +5,13 @@
  *     out[c] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q_c . k_j - max),   j over the keys of the column's sequence, causal:
  *     j <= row + (keys - rows)
  *
- * A column is one query row of one head; those of the heads that share a key-value head lie side by side. One wave takes QB columns of a
- * sequence and walks its keys 64 at a time with a running maximum and sum, all in f32: first a key to a lane (its row dotted with every
- * column's query), then an output dim to a lane. A key that a column does not see is passed over and not multiplied by zero, whatever
- * its row holds. head_dim beyond 512 walks the keys once for each 512 output dims. Bound by the uncoalesced reads of K: 512 causal rows
- * of 64 dims, 32 heads on 8, take 317 us, and one token of each of 48 texts of 1024 721 us; the matrix-core kernels on 128 dims 15 and 39.
+ * A column is one query row of one head; those of the heads that share a key-value head lie side by side. A workgroup takes QB columns of a
+ * sequence; each of its waves walks every fourth 64 of its keys with a running maximum and sum, all in f32: first a key to a lane (its row dotted
+ * with every column's query), then an output dim to a lane; at the end the waves' sums are joined. A key that a column does not see is passed over
+ * and not multiplied by zero, whatever its row holds. head_dim beyond 512 walks the keys once for each 512 output dims.
+ *
+ * Bound by the latency of reads, of which each wave has few under way: 512 causal rows, 32 heads on 8, of 64 dims take 120 us, of 256 273; one
+ * token of each of 48 texts of 1024 143 and 227 (with one wave to a column 204, 695, 450 and 2620). The matrix-core kernels on 128 dims: 14 and 38.
  */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -27,7 +29,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 namespace {
 
-constexpr int QB = 8, KT = 64, MOST_DIMS = 512, VEC = 8;
+constexpr int QB = 8, KT = 64, MOST_DIMS = 512, VEC = 8, WAVES = 4, THREADS = 64 * WAVES;
 
 __device__ __forceinline__ float value(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 __device__ __forceinline__ float value(uint8_t v) { return __builtin_amdgcn_cvt_f32_fp8(v, 0); }
@@ -49,14 +51,23 @@ __device__ __forceinline__ uint16_t to_bf16(float f) {
     const f32x2 p = {f, 0.0f};
     return (uint16_t)__builtin_bit_cast(uint32_t, __builtin_convertvector(p, bf16x2));
 }
-__device__ __forceinline__ float wave_max(float v) {
-    for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
-    return v;
+/* over all lanes, for all of them: in the vector registers (shifts inside rows of 16, then the rows' last lanes to those behind them) */
+template <int CTRL, int ROWS> __device__ __forceinline__ float dpp(float other, float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(__float_as_uint(other), __float_as_uint(v), CTRL, ROWS, 0xf, false));
 }
-__device__ __forceinline__ float wave_sum(float v) {
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
-    return v;
+template <class F> __device__ __forceinline__ float over_wave(float v, float none, F f) {
+    v = f(v, dpp<0x111, 0xf>(none, v));
+    v = f(v, dpp<0x112, 0xf>(none, v));
+    v = f(v, dpp<0x114, 0xf>(none, v));
+    v = f(v, dpp<0x118, 0xf>(none, v));
+    v = f(v, dpp<0x142, 0xa>(none, v));
+    v = f(v, dpp<0x143, 0xc>(none, v));
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63));
 }
+__device__ __forceinline__ float wave_max(float v) { return over_wave(v, -INFINITY, [](float x, float y) { return fmaxf(x, y); }); }
+__device__ __forceinline__ float wave_sum(float v) { return over_wave(v, 0.0f, [](float x, float y) { return x + y; }); }
+/* what this wave has written to the LDS can be read by all of its lanes */
+__device__ __forceinline__ void wave_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 /* where the rows of keys are: offset(j) of key j of the sequence in K and in V, or -1; scale bytes where there are any */
 struct RowKeys {
@@ -85,12 +96,13 @@ template <typename V> struct PageKeys {
  * multiple of 8 and rows of keys are aligned to 8 values */
 template <int SLOTS, class Keys, class Q, class Out, class Limit>
 __device__ __forceinline__ void walk(const Keys &keys, int nq, int m, int hd, float scale, bool wide, const uint16_t *q, Q qat, uint16_t *out, Out oat, Limit limit) {
-    __shared__ __align__(16) float ps[QB][KT];
+    __shared__ __align__(16) float all_ps[WAVES][QB][KT], buf[WAVES][QB][64], tops[WAVES][QB], sums[WAVES][QB];
     extern __shared__ __align__(16) float qs[];                      /* [QB][head_dim], the first DIMS dims */
     constexpr int DIMS = 64 * SLOTS;
-    const int lane = threadIdx.x, staged = min(hd, DIMS);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), staged = min(hd, DIMS);
+    auto &ps = all_ps[wave];
     for (int c = 0; c < QB; c++)
-        for (int d = lane; d < staged; d += 64) qs[c * staged + d] = value(q[qat(min(c, nq - 1)) + d]);
+        for (int d = threadIdx.x; d < staged; d += THREADS) qs[c * staged + d] = value(q[qat(min(c, nq - 1)) + d]);
     __syncthreads();
     for (int oc = 0; oc < hd; oc += DIMS) {
         float acc[QB][SLOTS], top[QB], sum[QB];
@@ -102,8 +114,8 @@ __device__ __forceinline__ void walk(const Keys &keys, int nq, int m, int hd, fl
         }
         int end = 0;
         for (int c = 0; c < nq; c++) end = max(end, min(m, limit(c)));
-        for (int k0 = 0; k0 < end; k0 += KT) {
-            const int j = k0 + lane, nk = min(KT, end - k0);
+        for (int tile = wave, tiles = (end + KT - 1) / KT; tile < tiles; tile += WAVES) {
+            const int k0 = tile * KT, j = k0 + lane, nk = min(KT, end - k0);
             const long at = j < end ? keys.offset(j) : -1;
             float dot[QB];
 #pragma unroll
@@ -111,6 +123,7 @@ __device__ __forceinline__ void walk(const Keys &keys, int nq, int m, int hd, fl
             if (at >= 0) {
                 int d = 0;
                 if (wide)
+#pragma unroll 4
                     for (; d < staged; d += VEC) {
                         float kd[VEC];
                         eight(keys.k + at + d, kd);
@@ -127,7 +140,6 @@ __device__ __forceinline__ void walk(const Keys &keys, int nq, int m, int hd, fl
             }
             const float ks = (at >= 0 ? keys.scale(keys.ks, at) : 1.0f) * scale, vs = at >= 0 ? keys.scale(keys.vs, at) : 1.0f;
             float alpha[QB];
-            __syncthreads();
 #pragma unroll
             for (int c = 0; c < QB; c++) {
                 const bool sees = at >= 0 && c < nq && j < limit(min(c, nq - 1));
@@ -139,7 +151,7 @@ __device__ __forceinline__ void walk(const Keys &keys, int nq, int m, int hd, fl
                 top[c] = high;
                 ps[c][lane] = sees ? p * vs : -1.0f;            /* -1: not seen (p * vs is never negative) */
             }
-            __syncthreads();
+            wave_lds();
             /* the rows of V, eight under way together: lane t of the wave knows where row t is; one that is not there is read as another, and not seen */
             const unsigned long long any = __ballot(at >= 0);
             const long some = any ? __shfl(at, __ffsll(any) - 1, 64) : 0;
@@ -167,21 +179,37 @@ __device__ __forceinline__ void walk(const Keys &keys, int nq, int m, int hd, fl
                 }
             }
         }
+        /* the waves' sums joined, 64 dims at a time, every fourth column by a wave */
+        __syncthreads();
+        if (lane == 0)
 #pragma unroll
-        for (int c = 0; c < QB; c++) {
-            if (c >= nq) break;
-            const float inv = sum[c] == 0.0f ? 0.0f : 1.0f / sum[c];      /* no key: a row of zeros */
+            for (int c = 0; c < QB; c++) { tops[wave][c] = top[c]; sums[wave][c] = sum[c]; }
 #pragma unroll
-            for (int t = 0; t < SLOTS; t++) {
-                const int d = oc + lane + 64 * t;
-                if (d < hd) out[oat(c) + d] = to_bf16(acc[c][t] * inv);
+        for (int t = 0; t < SLOTS; t++) {
+            if (oc + 64 * t >= hd) continue;
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < QB; c++) buf[wave][c][lane] = acc[c][t];
+            __syncthreads();
+            const int d = oc + lane + 64 * t;
+            for (int c = wave; c < nq; c += WAVES) {
+                float high = -INFINITY, den = 0.0f, o = 0.0f;
+                for (int w = 0; w < WAVES; w++) high = fmaxf(high, tops[w][c]);
+                const float base = high == -INFINITY ? 0.0f : high;
+                for (int w = 0; w < WAVES; w++) {
+                    const float f = expf(tops[w][c] - base);
+                    o += f * buf[w][c][lane];
+                    den += f * sums[w][c];
+                }
+                const float inv = den == 0.0f ? 0.0f : 1.0f / den;            /* no key: a row of zeros */
+                if (d < hd) out[oat(c) + d] = to_bf16(o * inv);
             }
         }
     }
 }
 
 template <int SLOTS>
-__global__ void __launch_bounds__(64)
+__global__ void __launch_bounds__(THREADS)
 k_sequences_any(uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k, const uint16_t *v, int ldkv, SequencesArg seqs,
                 int kv_heads, int hd, float scale, int wide, int causal) {
     SequenceTiles<> tiles;
@@ -196,7 +224,7 @@ k_sequences_any(uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16
 }
 
 template <typename T, int SLOTS>
-__global__ void __launch_bounds__(64)
+__global__ void __launch_bounds__(THREADS)
 k_paged_any(uint16_t *out, int ldo, const uint16_t *q, int ldq, const T *k, const T *v, const uint8_t *ks, const uint8_t *vs, PagedArg cache,
             int group, float scale, int wide) {
     const int blocks = (group + QB - 1) / QB, c0 = blockIdx.x % blocks * QB, kvh = blockIdx.x / blocks % cache.kv_heads;
@@ -215,7 +243,7 @@ template <class F> void with_slots(int head_dim, F f) {
     else if (head_dim <= 256) f(std::integral_constant<int, 4>{});
     else f(std::integral_constant<int, MOST_DIMS / 64>{});
 }
-bool fits(long wgs) { return wgs <= ((1L << 32) - 1) / 64; }
+bool fits(long wgs) { return wgs <= ((1L << 32) - 1) / THREADS; }
 
 }  // namespace
 
@@ -227,7 +255,7 @@ extern "C" int iris_hip_sequences_any(void *stream, uint16_t *out, int ldo, cons
     if (!wgs) return 0;
     if (!fits(wgs)) return (int)hipErrorInvalidValue;
     with_slots(head_dim, [&](auto slots) {
-        hipLaunchKernelGGL(k_sequences_any<decltype(slots)::value>, dim3((unsigned)wgs), dim3(64), staged_bytes(head_dim), (hipStream_t)stream, out, ldo, q, ldq,
+        hipLaunchKernelGGL(k_sequences_any<decltype(slots)::value>, dim3((unsigned)wgs), dim3(THREADS), staged_bytes(head_dim), (hipStream_t)stream, out, ldo, q, ldq,
                            k, v, ldkv, a, kv_heads, head_dim, scale, head_dim % VEC == 0 && ldkv % VEC == 0 && aligned(k, 2 * VEC), causal);
     });
     return (int)hipGetLastError();
@@ -243,10 +271,10 @@ extern "C" int iris_hip_paged_any(void *stream, uint16_t *out, int ldo, const ui
     with_slots(head_dim, [&](auto slots) {
         constexpr int SLOTS = decltype(slots)::value;
         if (ks)
-            hipLaunchKernelGGL((k_paged_any<uint8_t, SLOTS>), dim3((unsigned)wgs), dim3(64), staged_bytes(head_dim), (hipStream_t)stream, out, ldo, q, ldq,
+            hipLaunchKernelGGL((k_paged_any<uint8_t, SLOTS>), dim3((unsigned)wgs), dim3(THREADS), staged_bytes(head_dim), (hipStream_t)stream, out, ldo, q, ldq,
                                (const uint8_t *)k, (const uint8_t *)v, ks, vs, c, group, scale, head_dim % VEC == 0 && aligned(k, VEC));
         else
-            hipLaunchKernelGGL((k_paged_any<uint16_t, SLOTS>), dim3((unsigned)wgs), dim3(64), staged_bytes(head_dim), (hipStream_t)stream, out, ldo, q, ldq,
+            hipLaunchKernelGGL((k_paged_any<uint16_t, SLOTS>), dim3((unsigned)wgs), dim3(THREADS), staged_bytes(head_dim), (hipStream_t)stream, out, ldo, q, ldq,
                                (const uint16_t *)k, (const uint16_t *)v, nullptr, nullptr, c, group, scale, head_dim % VEC == 0 && aligned(k, 2 * VEC));
     });
     return (int)hipGetLastError();
