@@ -272,8 +272,8 @@ void iris_dev_linear_mxfp4_bf16_grouped(uint16_t *y, const uint8_t *x, const uin
  * j <= i + (m - n) of m. A row that sees no key gives zeros. What it does not see has no part in its result, infinities and NaN included.
  * head_dim 128 on rows that are 16-byte aligned (out: 8) and scale > 0 run on the matrix cores, everything else on a scalar kernel. P is
  * rounded to bf16 for the P V product and the row sums are those of the rounded values, as in iris_dev_attention. The keys of a few rows
- * over many keys are cut into ranges whose partial results pass through the private memory of the linear layers; under stream capture they
- * are not, and the f32 sums are then taken in another order. A call gives the same bits every time.
+ * over many keys are cut into ranges, by the lengths of all sequences of the call, whose partial results pass through the private memory of
+ * the linear layers; under stream capture they are not, and the f32 sums are then taken in another order. A call gives the same bits every time.
  * Needs rows * heads < 2^31 and keys < 2^31 - 64; larger calls, and those that no launch holds, are reported. */
 void iris_dev_attention_sequences(uint16_t *out, int ldo, const uint16_t *q, int ldq, const uint16_t *k, const uint16_t *v, int ldkv,
                                   const int *first_row, const int *first_key, int sequences, int rows, int keys,
