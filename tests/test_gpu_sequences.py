@@ -276,6 +276,7 @@ CUT = {
     "one row": ([1], [20011], 4, 1), "uneven": ([5, 0, 130, 1, 33], [4000, 77, 64, 1, 9000], 6, 3), "fewer keys than rows": ([40, 20], [10, 5000], 8, 8),
     "no keys": ([3, 9, 4], [0, 3001, 0], 16, 2), "65 sequences": ([1] * 65, [1 + 97 * (i % 41) for i in range(65)], 2, 1), "150 sequences": ([1] * 150, [0] * 90 + [4400] * 60, 1, 1),
     "several tiles": ([300, 77], [3003, 2100], 5, 1), "ten kv heads": ([17], [2222], 20, 10),
+    "more tiles than half the parts": ([10] * 12, [50, 5000, 64, 700, 12, 900, 130, 0, 1500, 800, 10, 600], 24, 24),
 }
 
 
