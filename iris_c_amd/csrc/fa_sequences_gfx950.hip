@@ -381,8 +381,9 @@ k_sequences_hd128(Args a) {
     while (t0 < ntiles) group_of_tiles(std::true_type{});
 
     if (CAUSAL && put_back) {
-        /* what was left out of the tiles that a limit passes through, for the columns that see it */
-        for (int key = max(see_all, 0) / KEYS * KEYS; key < min(see_any, s.m); key++) {
+        /* What was left out of the tiles that a limit passes through, for the columns that see it. Of this part's tiles alone: a column that sees
+         * no key of the part has weight 0 in the join, where an infinity of another part's would be 0 times an infinity. */
+        for (int key = max(max(see_all, 0) / KEYS, tile0) * KEYS; key < min(min(see_any, s.m), ntiles * KEYS); key++) {
             const uint16_t *vp = vbase + (size_t)key * a.ldkv + 4 * lg;
 #pragma unroll
             for (int db = 0; db < 8; db++) {
