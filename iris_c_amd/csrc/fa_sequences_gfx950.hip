@@ -481,14 +481,15 @@ extern "C" void iris_hip_sequences_plan(int n, int rows, int keys, int heads, in
      *     tiles 128, chain 16  21.1 26.6 /  20.7 27.5         32  36.2 35.4 /  35.2 36.0         64  65.2 52.0 / 63.0 50.8
      *     tiles 232, chain 31  40.2 47.1 /  41.1 51.5         93   114  106 /   106  109
      * Where sequences with keys of their own may differ in length, which the host does not know, the longest is waited for: 32 of 16 rows, 376 tiles,
-     * over 500 keys but one of 8000 (chain 11) 121 30, of 20000 288 35; 10 of 100 rows, 328 tiles, over 200 to 16000 keys 139 98, 24 heads on 24 189 94.
-     * They are cut sooner, though all of one length lose by it: 32 of 16 rows over 1024 keys each 27 35, over 2048 52 57.
+     * over 500 keys but one of 8000 (chain 11) 116 29, over 100 to 4000 (11) 59 32, of 20000 (17) 288 35; 10 of 100 rows, 328 tiles, over 200 to 16000
+     * keys 139 98, 24 heads on 24 189 94. They are cut sooner, though all of one length lose by it: 32 of 16 rows over 734 keys each (11) 21 30,
+     * 4 of 64 rows 17 21, 32 of 16 over 1024 27 35, over 2048 52 57.
      * Nothing is cut where there might be more tiles than leave an eighth of the parts to cut with, or more than the 256 sequences that a wave looks
      * at at once. */
     const long tiles = sequence_tiles_at_most({nullptr, nullptr, n, rows, keys, group}, 128) * kv_heads, chain = (long)keys / some / KEYS / (causal && own_keys ? 2 : 1);
     static_assert(MOST_PARTS * (part_floats(128, HD) * sizeof(float) + sizeof(Cut)) <= IRIS_LINEAR_PART_BYTES, "");
     const bool differ = some > 1 && !own_keys;
-    if (n <= 256 && tiles <= MOST_PARTS / 8 * 7 && tiles * ((long)keys / KEYS + 1) < 1L << 30 && (differ ? chain >= 12 : chain * (360 - tiles) >= 4800)) *parts = MOST_PARTS;
+    if (n <= 256 && tiles <= MOST_PARTS / 8 * 7 && tiles * ((long)keys / KEYS + 1) < 1L << 30 && (differ ? chain >= 11 : chain * (360 - tiles) >= 4800)) *parts = MOST_PARTS;
 }
 
 /* part: IRIS_LINEAR_PART_BYTES of private workspace, 16-byte aligned, or null: the keys of a workgroup are then not cut */
