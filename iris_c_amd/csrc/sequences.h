@@ -41,12 +41,27 @@ __device__ __forceinline__ int wave_max_upto(int v) {                    /* of v
     return v;
 }
 
+/* Blocks of keys to a part, at least 4, within a 32nd the fewest that make no more than most_entries entries of `tiles` tiles (fewer than that)
+ * with `work` blocks in all. entries(each) is their number with `each` blocks to a part: one a tile, and one more for every further part. There is such a
+ * number: entries(each) <= work / each + tiles. Host code can call it. */
+template <class Entries> __host__ __device__ __forceinline__ int part_blocks(int work, int tiles, int most_entries, Entries entries) {
+    constexpr int LEAST = 4;
+    const int more = most_entries - tiles;
+    int few = (work / most_entries > LEAST ? work / most_entries : LEAST) - 1, many = (work + more - 1) / more;      /* too few, or not to be tried; enough */
+    if (many < LEAST) many = LEAST;
+    while (many - few > 1 + many / 32) {                                  /* at least 2: `each` lies between them, and takes the place of one */
+        const int each = (few + many) / 2;
+        if (entries(each) <= most_entries) many = each;
+        else few = each;
+    }
+    return many;
+}
+
 /* BY_LENGTH: up to 64 sequences in the order of their keys, the most first, for kernels whose tiles take as long as the keys are many: the
  * last workgroups of a call are then short ones. CUT, up to 256 sequences: every tile is in the list as several parts of at most `each` key
  * blocks of 64, so many that there are about as many entries as wanted, and each about as long as the others. */
 template <bool BY_LENGTH = false, bool CUT = false>
 struct SequenceTiles {
-    static constexpr int LEAST = 4;                                  /* blocks of keys in a part */
     static constexpr int AT_ONCE = 4;                                /* 64 sequences at once: their bounds are one trip to memory */
     SequencesArg a;
     int height;
@@ -108,27 +123,21 @@ struct SequenceTiles {
         for (int base = 0; base < a.n; base += 64 * AT_ONCE) look(base);
         return total;
     }
-    /* Cuts the tiles of count(), for each of `heads` heads: `each` is the least number of blocks, within a 32nd, that makes not more than
-     * most_entries entries for all heads. most_entries is more than there are tiles for them, so that this one does:
-     * entries <= sum of heads (keys / each + 1) over the tiles <= most_entries. */
+    /* Cuts the tiles of count(), for each of `heads` heads, into not more than most_entries entries for all heads; there are fewer tiles than that
+     * for them. */
     __device__ __forceinline__ int cut(int heads, int most_entries) {
         int work = 0;
 #pragma unroll
         for (int i = 0; i < AT_ONCE; i++)
             if (64 * i < a.n) work += __builtin_amdgcn_readlane(wave_sum_upto(tiles(i) * blocks(khi[i] - klo[i])), 63);
-        work *= heads;
-        const int more = most_entries - total * heads;
-        int few = max(LEAST, work / most_entries) - 1, many = max(LEAST, (work + more - 1) / more);      /* too few, or not to be tried, and enough */
-        while (many - few > 1 + many / 32) {                              /* at least 2: `each` lies between them, and takes the place of one */
-            each = (few + many) / 2;
+        each = part_blocks(work * heads, total * heads, most_entries, [&](int blocks_each) {
+            each = blocks_each;
             int entries = 0;
 #pragma unroll
             for (int i = 0; i < AT_ONCE; i++)
                 if (64 * i < a.n) entries += __builtin_amdgcn_readlane(wave_sum_upto(tiles(i) * parts(khi[i] - klo[i])), 63);
-            if (entries * heads <= most_entries) many = each;
-            else few = each;
-        }
-        each = many;
+            return entries * heads;
+        });
         total = 0;
 #pragma unroll
         for (int i = 0; i < AT_ONCE; i++) {

@@ -1,9 +1,13 @@
-"""Which calls of packed attention have their keys cut into parts. Host arithmetic; no GPU."""
+"""Which calls of packed attention have their keys cut into parts, and the search for how many blocks of keys make a part, by the function that the kernel
+uses. Host arithmetic; no GPU."""
+import os
 import random
+import subprocess
 
 import pytest
 
 import iris_c_amd
+from test_half_words import CSRC, HIPCC, ROOT
 from test_sequences_refusals import plan
 
 
@@ -24,3 +28,16 @@ SPREAD = [round(200 * 80 ** random.Random(i).random()) for i in range(10)]
 def test_calls_that_are_cut(lib, rows, keys, heads, kv, cut, causal):
     """Those whose times stand beside the rule"""
     assert plan(lib, len(rows), sum(rows), sum(keys), heads, kv, causal, 0)[2] == (512 if cut else 1)
+
+
+def test_the_search_for_the_blocks_of_a_part(tmp_path):
+    if not os.path.exists(HIPCC):
+        pytest.skip("no hipcc here")
+    program = str(tmp_path / "cut")
+    r = subprocess.run([HIPCC, "-x", "hip", "-O2", "--offload-arch=gfx950", "-std=c++17", "-I" + CSRC, os.path.join(ROOT, "tests", "sequences_cut.cpp"), "-o", program],
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
+    r = subprocess.run([program], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout[-2000:]
+    calls, searched, failed = (int(r.stdout.split("\n")[-2].split()[i]) for i in (0, 2, 4))
+    assert calls > 10 ** 5 and searched > 10 ** 4 and failed == 0
