@@ -9,7 +9,7 @@
  *
  * The work of a call is one list of tiles: sequence by sequence, in it kv head by kv head (and, with more than 16 query heads to a kv
  * head, block of 16 by block). It is cut into as many equal ranges as there are waves, wherever that falls: the balance does not depend
- * on how long the sequences are, which the host does not know. A wave finds its range from the lengths (64 sequences at a time, one to a
+ * on how long the sequences are, which the host does not know. A wave finds its range from the lengths (256 sequences at a time, four to a
  * lane). A list entry that lies in one range as a whole is finished there; of one that is cut, each part leaves its unnormalised sums
  * and their maximum in the workspace and a second launch joins them. It finds what a range's end cuts in the workspace too, written while the range's wave waits for its
  * first pages: looked up from the lengths again the second launch takes 1 to 2 us more. A range cuts its first and its last entry at most: two places each.
@@ -521,15 +521,26 @@ extern "C" int iris_hip_paged_hd128_takes(int pages, int page_shift, int table_l
     return rows < NO_ROW && tiles < (1LL << 31) && ((__int128)table_ld << page_shift) < (1LL << 31) - 64;
 }
 
+/* The launches for these sizes: waves of the first, and threads of a workgroup of the second (0: there is none). Host arithmetic only */
+extern "C" void iris_hip_paged_plan(int fp8, int page_shift, int table_ld, int n, int heads, int kv_heads, int *waves, int *join) {
+    const int group = heads / kv_heads, blocks = (group + COLS - 1) / COLS, keys = fp8 ? Shape<true>::KEYS : Shape<false>::KEYS;
+    const long tiles = ((((long)table_ld << page_shift) + keys - 1) / keys) * n * kv_heads * blocks;
+    const int most = group > 8 ? MOST_WAVES / 4 * 3 : MOST_WAVES;     /* with 16 rows of Q for two list entries three waves have room in a CU's LDS */
+    *waves = tiles < 1 ? 1 : tiles < most ? (int)tiles : most;
+    /* Entries of many parts are joined by more threads: one text of 30000, 8 heads on one kv head, 29.5 us and 21.5 with 512; 16 on 2, 23.5 and 19.6; where the
+     * parts are few the threads only have to be started: 48 texts of 1 to 4096, 32 on 8, 24 and 26 */
+    *join = *waves >= 160L * n * kv_heads * blocks ? 512 : *waves > 1 ? 256 : 0;
+}
+
 extern "C" int iris_hip_paged_hd128(void *stream, float *part, uint16_t *out, int ldo, const uint16_t *q, int ldq, const void *k, const void *v,
                                     const uint8_t *ks, const uint8_t *vs, int pages, int page_shift, const int *table, int table_ld,
                                     const int *lengths, int n, int heads, int kv_heads, float scale) {
-    const int group = heads / kv_heads, blocks = (group + COLS - 1) / COLS, keys = ks ? Shape<true>::KEYS : Shape<false>::KEYS;
+    const int group = heads / kv_heads, blocks = (group + COLS - 1) / COLS;
     const Args a = {out, q, (const unsigned char *)k, (const unsigned char *)v, ks, vs, {table, lengths, table_ld, pages, page_shift, kv_heads, HD},
                     ldo, ldq, n, group, blocks, scale * 1.4426950408889634f, part};
-    const long tiles = ((((long)table_ld << page_shift) + keys - 1) / keys) * n * kv_heads * blocks;
-    const int q_rows = group <= 4 ? 4 : group <= 8 ? 8 : 16;          /* with 16 rows of Q for two list entries three waves have room in a CU's LDS */
-    const int most = q_rows == 16 ? MOST_WAVES / 4 * 3 : MOST_WAVES, waves = tiles < 1 ? 1 : tiles < most ? (int)tiles : most;
+    const int q_rows = group <= 4 ? 4 : group <= 8 ? 8 : 16;
+    int waves, join;
+    iris_hip_paged_plan(ks != nullptr, page_shift, table_ld, n, heads, kv_heads, &waves, &join);
     auto run = [&](auto fp8, auto rows) {
         constexpr int QROWS = decltype(rows)::value, LDS = STAGES * Shape<decltype(fp8)::value>::STAGE + 2 * QROWS * 2 * HD + 512;
         hipLaunchKernelGGL((k_paged_hd128<decltype(fp8)::value, QROWS>), dim3(waves), dim3(64), LDS, (hipStream_t)stream, a);
@@ -541,9 +552,7 @@ extern "C" int iris_hip_paged_hd128(void *stream, float *part, uint16_t *out, in
     };
     if (ks) run_rows(std::true_type{});
     else run_rows(std::false_type{});
-    /* Entries of many parts are joined by more threads: one text of 30000, 8 heads on one kv head, 29.5 us and 21.5 with 512; 16 on 2, 23.5 and 19.6; where the
-     * parts are few the threads only have to be started: 48 texts of 1 to 4096, 32 on 8, 24 and 26 */
-    if (waves >= 160L * n * kv_heads * blocks) hipLaunchKernelGGL(k_paged_join<512>, dim3(waves), dim3(512), 0, (hipStream_t)stream, a);
-    else if (waves > 1) hipLaunchKernelGGL(k_paged_join<256>, dim3(waves), dim3(256), 0, (hipStream_t)stream, a);
+    if (join == 512) hipLaunchKernelGGL(k_paged_join<512>, dim3(waves), dim3(512), 0, (hipStream_t)stream, a);
+    else if (join) hipLaunchKernelGGL(k_paged_join<256>, dim3(waves), dim3(256), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }

@@ -237,9 +237,11 @@ int iris_hip_paged_any(void *stream, uint16_t *out, int ldo, const uint16_t *q, 
                        const uint8_t *vs, int pages, int page_shift, const int *table, int table_ld, const int *lengths, int n, int heads,
                        int kv_heads, int head_dim, float scale);
 /* The same on the matrix cores: head_dim 128, scale > 0, q 16-byte and out 8-byte aligned, ldq % 8 == 0, ldo % 4 == 0, pages 16-byte aligned;
- * `takes`: whether the sizes are ones that it has numbers for. part: iris_hip_paged_workspace() bytes, 16-byte aligned. */
+ * `takes`: whether the sizes are ones that it has numbers for. plan: the waves of its first launch and the threads of a workgroup of its second
+ * (0: none). part: iris_hip_paged_workspace() bytes, 16-byte aligned. */
 size_t iris_hip_paged_workspace(void);
 int iris_hip_paged_hd128_takes(int pages, int page_shift, int table_ld, int n, int heads, int kv_heads);
+void iris_hip_paged_plan(int fp8, int page_shift, int table_ld, int n, int heads, int kv_heads, int *waves, int *join);
 int iris_hip_paged_hd128(void *stream, float *part, uint16_t *out, int ldo, const uint16_t *q, int ldq, const void *k, const void *v,
                          const uint8_t *ks, const uint8_t *vs, int pages, int page_shift, const int *table, int table_ld, const int *lengths,
                          int n, int heads, int kv_heads, float scale);
