@@ -270,6 +270,8 @@ void iris_dev_linear_mxfp4_bf16_grouped(uint16_t *y, const uint8_t *x, const uin
  * first_key[g] <= j < first_key[g + 1] of k and v (limited to 0 .. keys): a prompt that goes on from rows in a cache (iris_dev_cache_read_*).
  * causal: the last row of a sequence sees all of its keys, each row in front of it one key less: row i of n sees the keys
  * j <= i + (m - n) of m. A row that sees no key gives zeros. What it does not see has no part in its result, infinities and NaN included.
+ * An infinity in v that it sees makes its dim that infinity, or NaN where the key's probability is next to nothing in 32 bits (a score more than 70
+ * below the row's largest).
  * head_dim 128 on rows that are 16-byte aligned (out: 8) and scale > 0 run on the matrix cores, everything else on a scalar kernel. P is
  * rounded to bf16 for the P V product and the row sums are those of the rounded values, as in iris_dev_attention. The keys of a few rows
  * over many keys are cut into ranges, by the lengths of all sequences of the call, whose partial results pass through the private memory of
@@ -310,8 +312,8 @@ void iris_dev_cache_read_fp8(uint16_t *k, uint16_t *v, int ld, const uint8_t *k_
 
 /* Attention of one row a sequence, its newest token, over the lengths[g] tokens that the cache holds of it: out[g] = softmax(scale q[g]
  * K^T) V; q and out: rows of heads * head_dim. A sequence without keys gives zeros. What lies in the pages behind a sequence's last
- * token has no part in its result, whatever it is. head_dim 128 on 16-byte aligned rows and pages and scale > 0 run on the matrix cores,
- * everything else on a scalar kernel.
+ * token has no part in its result, whatever it is; an infinity in V that it sees is as in iris_dev_attention_sequences. head_dim 128 on
+ * 16-byte aligned rows and pages and scale > 0 run on the matrix cores, everything else on a scalar kernel.
  * The keys are cut into ranges whose partial results pass through `workspace`, at least iris_dev_attention_paged_workspace() bytes of
  * device memory, 16-byte aligned, that nothing else uses meanwhile; NULL: the library's own, which the library's stream orders. Captured
  * calls that may be replayed beside others therefore take workspaces of their own. The ranges, and with them the order of the f32 sums,

@@ -21,7 +21,7 @@
  * 128 dims: Q is cut into two parts of 4 bits, which together hold its 8 (to 2^-18 of its largest value). Values in 8 bits become bf16,
  * which holds them exactly, behind the LDS reads, and their scales multiply the probabilities.
  *
- * What bounds it: memory in long texts: 131072 + 70001 + 4097 tokens of 8 kv heads in 8 bits (424 MB) take 79 us, 5.4 TB/s, and 6 to join;
+ * What bounds it: memory in long texts: 131072 + 70001 + 4097 tokens of 8 kv heads in 8 bits (424 MB) take 80 us, 5.3 TB/s, and 6 to join;
  * 64 texts of 4096 in bf16 (1.07 GB) 189 us, 5.7 TB/s (with the join). In short ones the instructions around a list entry, some 2 us
  * of a wave that is alone on its SIMD (two waves of half the tile are no faster): 256 texts of up to 2048 in 8 bits (157 MB) 44 us + 5. Calls of one text are a
  * chain of launches and dependent reads (lengths, pages, tiles): 300 tokens 5.5 us + 4.
@@ -441,7 +441,7 @@ k_paged_hd128(Args a) {
                     rest[kg][i] = pack_bf16(__uint_as_float(b0 | last) - __uint_as_float(c0), __uint_as_float(b1 | last) - __uint_as_float(c1));
                 }
             }
-            /* The two products of a sum are not one behind the other, where the second would wait for the first (256 texts 49.5 us and not 47.1) */
+            /* The two products of a sum are not one behind the other, where the second would wait for the first (256 texts take 2.4 us longer so) */
             constexpr int TOGETHER = 2;
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -476,7 +476,7 @@ k_paged_hd128(Args a) {
         if (t + 2 < end) request(next, stage);
         if (t < begin || !done.end) continue;
         /* A V row of scale 255 is not a number, whatever its codes, and so is what it has part in. (A K row's scale is the product's, which makes the
-         * score NaN.) Asked of every p, or of the scores of every tile, 256 texts take 50 us and not 47.1. */
+         * score NaN.) Asked of every p, or of the scores of every tile, 256 texts take 3 us longer. */
         const float den = FP8 && __any(worst == 255) ? __builtin_nanf("") : over_column(sum, [](float x, float y) { return x + y; });
         if (li < done.cols && done.whole) {
             const float inv = den == 0.0f ? 0.0f : 1.0f / den;

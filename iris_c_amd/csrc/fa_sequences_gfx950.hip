@@ -17,14 +17,14 @@
  * What a column does not see: rows behind the sequence's last key are read from a row of zeros; scores behind the causal limit are set to
  * -infinity, so that their p is zero; and because zero times an infinity is not a number, the tile that the limit passes through is
  * multiplied by zeros first, and if that gives anything but zeros its infinities and NaN are taken out of V, and put into the sums of the
- * columns that see them at the end.
+ * columns that see them at the end (keys in parts: by the part that holds the tile).
  *
  * Workgroups: eight kv heads at a time (one to an XCD, whose L2 then holds the K and V of one head); with a causal limit from the last tile
  * of the last sequence down, so that of each sequence the longest come first (those of all sequences first is no faster), otherwise
  * sequence by sequence from the one with the most keys down.
  *
  * What bounds it: 12001 + 4096 + 700 + 1 causal rows, 32 heads on 8, take 1.18 - 1.24 ms, 1.07 - 1.12 PFLOP/s; pictures of 4608,
- * 1536, 2627 and 576 rows, 24 heads, 360 - 414 us (0.92 - 1.05 PFLOP/s). The matrix cores are busy 51 and 44 % of the cycles of all SIMDs, no LDS
+ * 1536, 2627 and 576 rows, 24 heads, 360 - 414 us (0.92 - 1.05 PFLOP/s). The matrix cores are busy 52 and 45 % of the cycles of all SIMDs, no LDS
  * access conflicts, 95 and 86 % of the requests are served by the L2s; as in the kernel for one sequence the rest is the softmax's vector
  * instructions (a thousand cycles beside 1088 of products per wave and tile) and what the chip's power leaves of the clock. 24 prompts of 4
  * to 512 rows take 20 us: workgroups of about 4 us of dependent reads (bounds, first tiles) and up to 8 tiles of 1.1 us and more, two on a CU.
@@ -32,7 +32,7 @@
  * Where there are few columns and many keys, the keys of every workgroup's columns are cut into parts, of as many key blocks each as gives about
  * two workgroups to a CU; the lengths are in device memory, so the kernel itself finds how many (sequences.h). Each part leaves its unnormalised
  * sums, their maximum and denominator in a workspace, and a second launch joins them, as many workgroups as there are parts, which find what
- * they join in the workspace too (looked up anew it would take 3 us more): 64 + 1 + 200 + 17 rows over 8294 keys, 32 heads on 8, 67 us whole, 37 to 40 cut
+ * they join in the workspace too (looked up anew it would take 3 us more): 64 + 1 + 200 + 17 rows over 8294 keys, 32 heads on 8, 67 us whole, 36 to 39 cut
  * (7 of them to join 30 MB); 32 rows over 16000 keys 227 and 31. Equal numbers of parts for all sequences, as many as the host can tell from their
  * average, leave the longest to be waited for: 46 and 53.
  */
